@@ -120,28 +120,67 @@ SIGNATURES = {
  T_GRAD, T_RESTORE) = range(14)
 T_COUNT = 14
 
+# libbattgp_products.so (include/battgp_products.h): name -> (restype, argtypes), every symbol of the header
+PRODUCTS_PATH = os.path.join(_HERE, "libbattgp_products.so")
+F64, F32, BF16, F16 = range(4)
+MAX_GROUPS = 65535
+INT8_MAX_K = 131071
+PRODUCTS_SIGNATURES = {
+    "bgp_products_last_error": (C.c_char_p, []),
+    "bgp_grouped_gemm": (
+        C.c_int,
+        [C.c_int, C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_int64, C.c_int,
+         C.c_void_p, C.c_void_p, C.c_int64, C.c_int],
+    ),
+    "bgp_grouped_gemm_dw": (
+        C.c_int,
+        [C.c_int, C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p,
+         C.c_int64, C.c_int64],
+    ),
+    "bgp_quantize_rows": (
+        C.c_int,
+        [C.c_int, C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int, C.c_void_p, C.c_int64],
+    ),
+    "bgp_int8_gemm": (
+        C.c_int,
+        [C.c_int, C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p,
+         C.c_int64, C.c_void_p, C.c_int64],
+    ),
+}
+
 _lib = None
+_products = None
 
 
 def load() -> C.CDLL:
     """Load libbattgp.so and bind every declared symbol.  Raises if anything is missing."""
     global _lib
-    if _lib is not None:
-        return _lib
-    if not os.path.exists(LIB_PATH):
+    if _lib is None:
+        _lib = _bind(LIB_PATH, SIGNATURES, " --experimental" if EXPERIMENTAL else "")
+    return _lib
+
+
+def load_products() -> C.CDLL:
+    """Load libbattgp_products.so, like :func:`load`."""
+    global _products
+    if _products is None:
+        _products = _bind(PRODUCTS_PATH, PRODUCTS_SIGNATURES)
+    return _products
+
+
+def _bind(path: str, signatures: dict, option: str = "") -> C.CDLL:
+    if not os.path.exists(path):
         raise ImportError(
-            f"{LIB_PATH} is missing: build it with `python -m battgp_amd.build{' --experimental' if EXPERIMENTAL else ''}` "
-            "(hipcc --offload-arch=gfx950).  battgp_amd has no CPU fallback."
+            f"{path} is missing: build it with `python -m battgp_amd.build{option}` (hipcc --offload-arch=gfx950).  battgp_amd has no CPU fallback."
         )
-    lib = C.CDLL(LIB_PATH)
-    for name, (res, args) in SIGNATURES.items():
+    lib = C.CDLL(path)
+    for name, (res, args) in signatures.items():
         try:
             fn = getattr(lib, name)
         except AttributeError as exc:
-            raise ImportError(f"{os.path.basename(LIB_PATH)} does not export `{name}`") from exc
+            raise ImportError(f"{os.path.basename(path)} does not export `{name}`") from exc
         fn.restype = res
         fn.argtypes = args
-    _lib = lib
     return lib
 
 

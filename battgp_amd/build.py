@@ -1,4 +1,4 @@
-"""Build libbattgp.so (HIP, gfx950 only) in-tree with hipcc.  No fallback of any kind.
+"""Build libbattgp.so and libbattgp_products.so (HIP, gfx950 only) in-tree with hipcc.  No fallback of any kind.
 
     python -m battgp_amd.build [--force] [--experimental]
 
@@ -23,6 +23,15 @@ HEADERS = [os.path.join(CSRC, "bgp_internal.h"), os.path.join(CSRC, "bgp_fill_ti
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function"]
 
 
+# libbattgp_products.so: the products of battgp_amd/products.py (include/battgp_products.h)
+PRODUCTS = os.path.join(CSRC, "products")
+LIB_PRODUCTS = os.path.join(HERE, "libbattgp_products.so")
+PRODUCTS_SOURCES = ["grouped.hip", "int8.hip"]
+PRODUCTS_HEADERS = [os.path.join(PRODUCTS, h) for h in ("tile.h", "entry.h")] + [os.path.join(os.path.dirname(HERE), "include", "battgp_products.h")]
+# no packed fp32 arithmetic: some of its forms have given wrong results on gfx950
+PRODUCTS_FLAGS = FLAGS + ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+
+
 def _hipcc() -> str:
     for cand in (shutil.which("hipcc"), "/opt/rocm/bin/hipcc"):
         if cand and os.path.exists(cand):
@@ -43,26 +52,37 @@ def build_lib(force: bool = False, verbose: bool = True, experimental: bool = Fa
     lib = LIB_EXPERIMENTAL if experimental else LIB
     if not force and not needs_build(experimental):
         return lib
+    _compile(CSRC, SOURCES, FLAGS + (["-DBGP_EXPERIMENTAL"] if experimental else []), ".exp.o" if experimental else ".o", lib, verbose)
+    return lib
+
+
+def build_products(force: bool = False, verbose: bool = True) -> str:
+    deps = [os.path.join(PRODUCTS, s) for s in PRODUCTS_SOURCES] + PRODUCTS_HEADERS + [os.path.abspath(__file__)]
+    if force or not os.path.exists(LIB_PRODUCTS) or any(os.path.getmtime(d) > os.path.getmtime(LIB_PRODUCTS) for d in deps):
+        _compile(PRODUCTS, PRODUCTS_SOURCES, PRODUCTS_FLAGS, ".o", LIB_PRODUCTS, verbose)
+    return LIB_PRODUCTS
+
+
+def _compile(folder, sources, flags, suffix, lib, verbose):
     hipcc = _hipcc()
-    flags = FLAGS + (["-DBGP_EXPERIMENTAL"] if experimental else [])
     from concurrent.futures import ThreadPoolExecutor
 
     def compile_one(src):
-        obj = os.path.join(CSRC, src.replace(".hip", ".exp.o" if experimental else ".o"))
-        cmd = [hipcc, *flags, "-c", os.path.join(CSRC, src), "-o", obj]
+        obj = os.path.join(folder, src.replace(".hip", suffix))
+        cmd = [hipcc, *flags, "-c", os.path.join(folder, src), "-o", obj]
         if verbose:
             print(" ".join(cmd), flush=True)
         subprocess.check_call(cmd)
         return obj
 
-    with ThreadPoolExecutor(len(SOURCES)) as pool:  # the three translation units side by side
-        objs = list(pool.map(compile_one, SOURCES))
+    with ThreadPoolExecutor(len(sources)) as pool:  # the translation units side by side
+        objs = list(pool.map(compile_one, sources))
     cmd = [hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", *objs, "-o", lib]
     if verbose:
         print(" ".join(cmd), flush=True)
     subprocess.check_call(cmd)
-    return lib
 
 
 if __name__ == "__main__":
     build_lib(force="--force" in sys.argv, experimental="--experimental" in sys.argv)
+    build_products(force="--force" in sys.argv)

@@ -1,0 +1,36 @@
+// What the C entry points of libbattgp_products.so share: errors, the device of a call, launches.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include "../../../include/battgp_products.h"
+
+// workgroups of 256 threads in one launch: the threads of a launch are counted in 32 bits
+constexpr int64_t MAX_WORKGROUPS = (1 << 24) - 1;
+
+int bgp_products_fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
+
+// makes `device` the current one for the length of a call
+class DeviceScope {
+  int before_ = -1;
+  hipError_t err_;
+
+ public:
+  explicit DeviceScope(int device) {
+    err_ = hipGetDevice(&before_);
+    if (err_ == hipSuccess && before_ != device) err_ = hipSetDevice(device);
+    else if (err_ == hipSuccess) before_ = -1;
+  }
+  ~DeviceScope() {
+    if (before_ >= 0) (void)hipSetDevice(before_);
+  }
+  int check(const char* what) const {
+    return err_ == hipSuccess ? 0 : bgp_products_fail(-2, "%s: %s", what, hipGetErrorString(err_));
+  }
+};
+
+template <class... A> int launch(const char* what, void (*kernel)(A...), dim3 grid, dim3 block, hipStream_t stream, A... args) {
+  void* ptrs[] = {(void*)&args...};
+  const hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, block, ptrs, 0, stream);
+  return e == hipSuccess ? 0 : bgp_products_fail(-2, "%s: launch failed: %s", what, hipGetErrorString(e));
+}

@@ -1,0 +1,237 @@
+"""Matrix products next to the exact-GP engine's own (``ExactGPEngine.gemm_nt_sub_device``: one pair of fp64 operands):
+products grouped by expert with ragged sizes, their gradients, and products in 8-bit integers with one scale per row.
+
+torch tensors on the GPU in and out, in fp64, fp32, bf16 and fp16.  Every function enqueues its kernels on the current
+torch stream of the tensors' device and returns without waiting for them; nothing is kept between calls, so the calls can
+be captured into a graph and come from several threads.  The kernels run in libbattgp_products.so
+(``include/battgp_products.h``); there is no fallback.  Like the engine's ``lml_grad``, gradients are calls of their own:
+no function records an autograd graph, and inputs that ask for one are refused.
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import _lib
+from .engine import EngineError
+
+DTYPES = {torch.float64: _lib.F64, torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+INT8_MAX_K = _lib.INT8_MAX_K
+MAX_GROUPS = _lib.MAX_GROUPS
+
+
+DEVICE_TYPE = "cuda"  # torch's name of the only device there is a kernel for
+
+
+def _check(rc: int) -> None:
+    if rc != 0:
+        raise EngineError(_lib.load_products().bgp_products_last_error().decode())
+
+
+def _gpu_tensor(name: str, t, dim: int, like: torch.Tensor | None = None) -> torch.Tensor:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} is not a torch tensor")
+    if t.layout != torch.strided:
+        raise ValueError(f"{name} is not a dense tensor")
+    if t.dim() != dim:
+        raise ValueError(f"{name} has {t.dim()} dimensions, {dim} are wanted")
+    if t.device.type != DEVICE_TYPE:
+        raise EngineError(f"{name} is on {t.device}: battgp_amd runs on MI355X only")
+    if like is not None and t.device != like.device:
+        raise ValueError(f"{name} is on {t.device}, the other operands are on {like.device}")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient: battgp_amd.products records no autograd graph; detach it and call the gradient's function")
+    return t
+
+
+def _float_type(name: str, dtype) -> int:
+    if dtype not in DTYPES:
+        raise ValueError(f"{name}: {dtype} is not one of float64, float32, bfloat16, float16")
+    return DTYPES[dtype]
+
+
+def _rows(name: str, t: torch.Tensor) -> int:
+    """Leading dimension of a matrix whose rows are contiguous (a dimension of one element has no stride of its own)."""
+    m, n = t.shape
+    if n > 1 and t.stride(1) != 1:
+        raise ValueError(f"{name}: the elements of a row have to be contiguous, strides are {t.stride()}")
+    if m <= 1:
+        return max(n, 1)
+    ld = t.stride(0)
+    if ld < n:
+        raise ValueError(f"{name}: rows overlap, strides are {t.stride()}")
+    return max(ld, 1)
+
+
+def _weights(w: torch.Tensor) -> tuple[int, int, int]:
+    """(stride of a group, leading dimension, 1 if the output axis is the contiguous one) of w[G, N, K]."""
+    g, n, k = w.shape
+    sg = w.stride(0) if g > 1 else 0
+    if (k <= 1 or w.stride(2) == 1) and (n <= 1 or w.stride(1) >= max(k, 1)):
+        return sg, (w.stride(1) if n > 1 else max(k, 1)), 0
+    if (n <= 1 or w.stride(1) == 1) and (k <= 1 or w.stride(2) >= max(n, 1)):
+        return sg, (w.stride(2) if k > 1 else max(n, 1)), 1
+    raise ValueError(f"w: either axis of a group's weights has to be contiguous, strides are {w.stride()}")
+
+
+def _span(t: torch.Tensor) -> tuple[int, int]:
+    if t.numel() == 0:
+        return 0, 0
+    last = sum((s - 1) * st for s, st in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _output(out, name: str, shape, dtype, device, inputs) -> torch.Tensor:
+    if out is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    _gpu_tensor(name, out, len(shape))
+    if out.device != device or out.dtype != dtype or tuple(out.shape) != tuple(shape):
+        raise ValueError(f"{name}: {tuple(shape)} of {dtype} on {device} is wanted, got {tuple(out.shape)} of {out.dtype} on {out.device}")
+    lo, hi = _span(out)
+    for t in inputs:
+        a, b = _span(t)
+        if a < hi and lo < b:
+            raise ValueError(f"{name} overlaps an input")
+    return out
+
+
+def _stream(device) -> C.c_void_p:
+    return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+def _offsets(offsets, groups: int, like: torch.Tensor) -> torch.Tensor:
+    _gpu_tensor("offsets", offsets, 1, like)
+    if offsets.dtype != torch.int64:
+        raise ValueError(f"offsets are {offsets.dtype}, int64 is wanted")
+    if offsets.shape[0] != groups + 1:
+        raise ValueError(f"{offsets.shape[0]} offsets for {groups} groups, {groups + 1} are wanted")
+    if groups > MAX_GROUPS:
+        raise ValueError(f"{groups} groups, at most {MAX_GROUPS} are possible")
+    if offsets.stride(0) != 1:
+        raise ValueError("offsets are not contiguous")
+    return offsets
+
+
+def _grouped(x, w, offsets, out, name):
+    """out[t, :] = x[t, :] w_g^T; w may be any view of [G, N, K] that _weights takes"""
+    t, k = x.shape
+    g, n, _ = w.shape
+    ldx = _rows("x", x)
+    sw, ldw, trans = _weights(w)
+    y = _output(out, name, (t, n), x.dtype, x.device, (x, w, offsets))
+    _check(_lib.load_products().bgp_grouped_gemm(
+        x.device.index, _stream(x.device), DTYPES[x.dtype], t, n, k, g, x.data_ptr(), ldx, w.data_ptr(), sw, ldw, trans, offsets.data_ptr(),
+        y.data_ptr(), _rows(name, y), int(out is None),
+    ))
+    return y
+
+
+def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``y[t] = w[g] @ x[t]`` for the rows ``offsets[g] <= t < offsets[g + 1]`` of every group ``g``.
+
+    ``x [T, K]`` with contiguous rows, sorted by group; ``w [G, N, K]`` with either of its last two axes contiguous
+    (``w.transpose(1, 2)`` of stored ``[G, K, N]`` weights is taken as it is; ``expand`` shares weights); ``offsets
+    [G + 1]`` int64 on the device, ascending, within ``[0, T]`` - they are never read on the host.  Groups may be empty.
+    Rows in no group are 0 in a new output and left as they are in a given ``out``.  Sums are held in fp32 (fp64 for
+    fp64) and rounded once."""
+    _gpu_tensor("x", x, 2)
+    _gpu_tensor("w", w, 3, x)
+    _float_type("x", x.dtype)
+    if w.dtype != x.dtype:
+        raise ValueError(f"x is {x.dtype}, w is {w.dtype}")
+    if w.shape[2] != x.shape[1]:
+        raise ValueError(f"x has {x.shape[1]} columns, w has {w.shape[2]}")
+    _offsets(offsets, w.shape[0], x)
+    return _grouped(x, w, offsets, out, "out")
+
+
+def grouped_matmul_grad(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, need_dx: bool = True, need_dw: bool = True):
+    """Gradients of :func:`grouped_matmul` for ``dy [T, N]``: ``(dx [T, K], dw [G, N, K])``, ``None`` for one that is not
+    needed.  ``dx`` is 0 in rows of no group, ``dw`` is 0 for an empty group; both are new and contiguous, and for shared
+    weights (``expand``) ``dw`` still holds each group's own share."""
+    _gpu_tensor("x", x, 2)
+    _gpu_tensor("dy", dy, 2, x)
+    _gpu_tensor("w", w, 3, x)
+    _float_type("x", x.dtype)
+    if w.dtype != x.dtype or dy.dtype != x.dtype:
+        raise ValueError(f"x is {x.dtype}, w is {w.dtype}, dy is {dy.dtype}")
+    t, k = x.shape
+    g, n, _ = w.shape
+    if w.shape[2] != k or tuple(dy.shape) != (t, n):
+        raise ValueError(f"dy {tuple(dy.shape)}, x {tuple(x.shape)} and w {tuple(w.shape)} do not belong together")
+    _offsets(offsets, g, x)
+    dx = dw = None
+    if need_dx:
+        dx = _grouped(dy, w.transpose(1, 2), offsets, None, "dx")
+    if need_dw:
+        dw = torch.empty((g, n, k), dtype=x.dtype, device=x.device)
+        _check(_lib.load_products().bgp_grouped_gemm_dw(
+            x.device.index, _stream(x.device), DTYPES[x.dtype], t, n, k, g, dy.data_ptr(), _rows("dy", dy), x.data_ptr(), _rows("x", x),
+            offsets.data_ptr(), dw.data_ptr(), n * max(k, 1), max(k, 1),
+        ))
+    return dx, dw
+
+
+def _scale_type(dtype):
+    return torch.float64 if dtype == torch.float64 else torch.float32
+
+
+def quantize_rows(x: torch.Tensor, pow2: bool = False, residual: bool = False):
+    """``(q, scale)`` or ``(q, scale, rest)``: 8-bit codes of the rows of ``x [M, K]``, one scale each, ``x ~ scale * q``.
+
+    ``scale = max |row| / 127`` (fp64 for fp64, else fp32), or with ``pow2`` the smallest power of two ``p`` with
+    ``max |row| <= 127 p``; at least the smallest normal number.  ``q`` is rounded to the nearest, ties to even.
+    ``rest = x - scale * q``, exact with ``pow2``: quantising it again gives the next slice of the row.  A row with an
+    infinity or a NaN has that for its scale, and codes 0."""
+    _gpu_tensor("x", x, 2)
+    code = _float_type("x", x.dtype)
+    m, k = x.shape
+    q = torch.empty((m, k), dtype=torch.int8, device=x.device)
+    scale = torch.empty(m, dtype=_scale_type(x.dtype), device=x.device)
+    rest = torch.empty((m, k), dtype=x.dtype, device=x.device) if residual else None
+    _check(_lib.load_products().bgp_quantize_rows(
+        x.device.index, _stream(x.device), code, m, k, x.data_ptr(), _rows("x", x), q.data_ptr(), max(k, 1), scale.data_ptr(), int(pow2),
+        rest.data_ptr() if residual else None, max(k, 1),
+    ))
+    return (q, scale, rest) if residual else (q, scale)
+
+
+def int8_matmul(
+    a: torch.Tensor, b: torch.Tensor, a_scale: torch.Tensor, b_scale: torch.Tensor, c: torch.Tensor | None = None,
+    dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """``y[i, j] = (c[i, j] +) a_scale[i] * b_scale[j] * sum_k a[i, k] b[j, k]`` in ``dtype``.
+
+    ``a [M, K]`` and ``b [N, K]`` int8 with contiguous rows, ``K <= 131071`` (the sum is exact in 32 bits);
+    scales fp64 for a fp64 result, else fp32; ``c`` and ``out`` of the result's type, ``out`` may be ``c`` itself.  The
+    scaling and the sum with ``c`` are computed in fp64 and rounded once."""
+    _gpu_tensor("a", a, 2)
+    _gpu_tensor("b", b, 2, a)
+    code = _float_type("dtype", dtype)
+    if a.dtype != torch.int8 or b.dtype != torch.int8:
+        raise ValueError(f"a is {a.dtype}, b is {b.dtype}: int8 is wanted")
+    m, k = a.shape
+    n = b.shape[0]
+    if b.shape[1] != k:
+        raise ValueError(f"a has {k} columns, b has {b.shape[1]}")
+    if k > INT8_MAX_K:
+        raise ValueError(f"{k} columns: a sum over more than {INT8_MAX_K} can pass 32 bits")
+    for name, s, rows in (("a_scale", a_scale, m), ("b_scale", b_scale, n)):
+        _gpu_tensor(name, s, 1, a)
+        if s.dtype != _scale_type(dtype) or s.shape[0] != rows or (rows > 1 and s.stride(0) != 1):
+            raise ValueError(f"{name}: {rows} contiguous values of {_scale_type(dtype)} are wanted for a result in {dtype}")
+    if c is not None:
+        _gpu_tensor("c", c, 2, a)
+        if c.dtype != dtype or tuple(c.shape) != (m, n):
+            raise ValueError(f"c: {(m, n)} of {dtype} is wanted, got {tuple(c.shape)} of {c.dtype}")
+    inputs = [a, b, a_scale, b_scale]
+    if c is not None and not (out is not None and out.data_ptr() == c.data_ptr() and out.stride() == c.stride()):
+        inputs.append(c)
+    y = _output(out, "out", (m, n), dtype, a.device, inputs)
+    _check(_lib.load_products().bgp_int8_gemm(
+        a.device.index, _stream(a.device), code, m, n, k, a.data_ptr(), _rows("a", a), b.data_ptr(), _rows("b", b), a_scale.data_ptr(),
+        b_scale.data_ptr(), c.data_ptr() if c is not None else None, _rows("c", c) if c is not None else 0, y.data_ptr(), _rows("out", y),
+    ))
+    return y
