@@ -6,51 +6,21 @@
 
 namespace {
 
-// The group of the `want`-th tile of BM rows.  Groups count their own tiles (a tile never crosses a bound); with
-// `rest` != 0 the rows before the first and behind the last group follow as groups G and G + 1.  Bounds are clamped to
-// [0, T], so wrong ones can name wrong rows but none outside the matrix.  Every wave of the workgroup works it out
-// for itself: 64 groups at a time, one prefix sum over the lanes.
+// The rows are cut into tiles of BM rows, group by group (a tile never crosses a bound); with `rest` != 0 the rows before
+// the first and behind the last group follow as groups G and G + 1.  Bounds are clamped to [0, T], so wrong ones can
+// name wrong rows but none outside the matrix.  Every wave of a workgroup works its own tile out for itself: 64 groups
+// at a time, one prefix sum over the lanes.
 struct RowTile {
-  int g;
+  int g, tn;
   int64_t row0, rows;
 };
 
 __device__ __forceinline__ int64_t clamp64(int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : (v > hi ? hi : v); }
 
-__device__ __forceinline__ RowTile find_row_tile(const int64_t* off, int G, int64_t T, int BM, int want, int rest) {
-  const int lane = threadIdx.x & 63, total = rest ? G + 2 : G;
-  for (int base = 0; base < total; base += 64) {
-    const int g = base + lane;
-    int64_t a = 0, b = 0;
-    if (g < G) {
-      a = clamp64(off[g], 0, T);
-      b = clamp64(off[g + 1], a, T);
-    } else if (g == G && rest) {
-      b = G > 0 ? clamp64(off[0], 0, T) : T;
-    } else if (g == G + 1 && rest && G > 0) {
-      a = clamp64(off[G], 0, T);
-      b = T;
-    }
-    const int tiles = (int)((b - a + BM - 1) / BM);
-    int sum = tiles;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int v = __shfl_up(sum, d);
-      if (lane >= d) sum += v;
-    }
-    const unsigned long long past = __ballot(sum > want);
-    if (past) {
-      const int at = __ffsll(past) - 1;
-      const int64_t row0 = a + (int64_t)(want - (sum - tiles)) * BM;
-      RowTile t;
-      t.g = __builtin_amdgcn_readfirstlane(base + at);
-      t.row0 = __shfl(row0, at);
-      t.rows = __shfl(b - row0 < BM ? b - row0 : (int64_t)BM, at);
-      return t;
-    }
-    want -= __shfl(sum, 63);
-  }
-  return RowTile{-1, 0, 0};
+// one lane's value, in scalar registers
+__device__ __forceinline__ int64_t lane_value(int64_t v, int lane) {
+  const uint32_t lo = __builtin_amdgcn_readlane((int)v, lane), hi = __builtin_amdgcn_readlane((int)(v >> 32), lane);
+  return (int64_t)((uint64_t)hi << 32 | lo);
 }
 
 struct GroupedArgs {
@@ -61,15 +31,71 @@ struct GroupedArgs {
   int G, rest, tiles_n;
 };
 
+struct Bounds {
+  int64_t a, b;
+  int sum;  // row tiles up to and with this lane's group, of this batch of 64 groups
+};
+
+__device__ __forceinline__ Bounds lane_bounds(const GroupedArgs& p, int BM, int g) {
+  const int G = p.G, lane = threadIdx.x & 63;
+  Bounds r{0, 0, 0};
+  if (g < G) {
+    r.a = clamp64(p.off[g], 0, p.T);
+    r.b = clamp64(p.off[g + 1], r.a, p.T);
+  } else if (g == G && p.rest) {
+    r.b = G > 0 ? clamp64(p.off[0], 0, p.T) : p.T;
+  } else if (g == G + 1 && p.rest && G > 0) {
+    r.a = clamp64(p.off[G], 0, p.T);
+    r.b = p.T;
+  }
+  r.sum = (int)((r.b - r.a + BM - 1) / BM);
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int v = __shfl_up(r.sum, d);
+    if (lane >= d) r.sum += v;
+  }
+  return r;
+}
+
+// The tile of this workgroup.  Workgroups go to the 8 XCDs in turn, and each XCD has an L2 of its own: the tiles that
+// exist are dealt in 8 runs, one for each XCD, and inside a run 8 row tiles are gone through before the next column tile,
+// so that the workgroups of an XCD that run together share rows of both operands.
+__device__ __forceinline__ RowTile find_row_tile(const GroupedArgs& p, int BM) {
+  const int lane = threadIdx.x & 63, groups = p.rest ? p.G + 2 : p.G;
+  Bounds r = lane_bounds(p, BM, lane);
+  int tiles_m = __builtin_amdgcn_readlane(r.sum, 63);
+  for (int base = 64; base < groups; base += 64) tiles_m += __builtin_amdgcn_readlane(lane_bounds(p, BM, base + lane).sum, 63);
+  constexpr int XCDS = 8, DEEP = 8;
+  const int64_t total = (int64_t)tiles_m * p.tiles_n, run = (total + XCDS - 1) / XCDS;
+  const int64_t at = blockIdx.x / XCDS, i = blockIdx.x % XCDS * run + at;
+  if (at >= run || i >= total) return RowTile{-1, 0, 0, 0};
+  const int64_t strip = i / (DEEP * p.tiles_n);
+  const int in = (int)(i - strip * DEEP * p.tiles_n), deep = tiles_m - strip * DEEP < DEEP ? (int)(tiles_m - strip * DEEP) : DEEP;
+  RowTile t;
+  t.tn = in / deep;
+  int want = (int)(strip * DEEP) + in % deep;
+  for (int base = 0;;) {
+    const unsigned long long past = __ballot(r.sum > want);
+    if (past) {
+      const int j = __ffsll(past) - 1;
+      const int tiles = (int)((r.b - r.a + BM - 1) / BM);
+      const int64_t row0 = r.a + (int64_t)(want - (r.sum - tiles)) * BM;
+      t.g = base + j;
+      t.row0 = lane_value(row0, j);
+      t.rows = lane_value(r.b - row0 < BM ? r.b - row0 : (int64_t)BM, j);
+      return t;
+    }
+    want -= __builtin_amdgcn_readlane(r.sum, 63);
+    base += 64;
+    r = lane_bounds(p, BM, base + lane);
+  }
+}
+
 // Y[rows of g, :] = X[rows of g, :] W_g^T;  WK: W_g[n, k] = w[g sw + n ldw + k], else w[g sw + k ldw + n]
-template <class T, int BM, int BN, bool WK, bool VEC>
-__global__ __launch_bounds__(256, 2) void grouped_rows_kernel(GroupedArgs p) {
-  using P = Tile<T, BM, BN, 2, 2, true, WK, VEC>;
-  __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
-  const int tn = blockIdx.x % p.tiles_n, tm = blockIdx.x / p.tiles_n;
-  const RowTile t = find_row_tile(p.off, p.G, p.T, BM, tm, p.rest);
+template <class T, class P, int BM, int BN, bool WK> __device__ __forceinline__ void rows_tile(const GroupedArgs& p, char* lds) {
+  const RowTile t = find_row_tile(p, BM);
   if (t.g < 0) return;
-  const int64_t n0 = (int64_t)tn * BN;
+  const int64_t n0 = (int64_t)t.tn * BN;
   T* y = static_cast<T*>(p.y) + t.row0 * p.ldy + n0;
   P tile;
   const Operand<T> x{static_cast<const T*>(p.x) + t.row0 * p.ldx, p.ldx, t.rows};
@@ -81,23 +107,50 @@ __global__ __launch_bounds__(256, 2) void grouped_rows_kernel(GroupedArgs p) {
   });
 }
 
-// dW_g[n, k] = sum over the rows t of g of dY[t, n] X[t, k]
-template <class T, int BM, int BN, bool VEC>
-__global__ __launch_bounds__(256, 2) void grouped_dw_kernel(GroupedArgs p) {
-  using P = Tile<T, BM, BN, 2, 2, false, false, VEC>;
+// any operands, through registers
+template <class T, int BM, int BN, bool WK> __global__ __launch_bounds__(256, 2) void grouped_rows_kernel(GroupedArgs p) {
+  using P = Tile<T, BM, BN, 2, 2, true, WK, false>;
   __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
+  rows_tile<T, P, BM, BN, WK>(p, lds);
+}
+
+// operands in whole chunks, pipelined: 256 x 256 by 8 waves (one workgroup per CU), smaller ones by 4 (two and more)
+template <class T, int BM, int BN, bool WK> __global__ __launch_bounds__(BM == 256 ? 512 : 256, 2) void grouped_rows_pipe_kernel(GroupedArgs p) {
+  using P = PipeTile<T, BM, BN, 2, BM == 256 ? 4 : 2, true, WK>;
+  __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
+  rows_tile<T, P, BM, BN, WK>(p, lds);
+}
+
+// dW_g[n, k] = sum over the rows t of g of dY[t, n] X[t, k]
+template <class T, class P, int BM, int BN> __device__ __forceinline__ void dw_tile(const GroupedArgs& p, char* lds) {
   const int tiles_k = (int)((p.K + BN - 1) / BN), tiles = p.tiles_n * tiles_k;
-  const int g = blockIdx.x / tiles, i = blockIdx.x % tiles;
-  const int64_t n0 = (int64_t)(i / tiles_k) * BM, k0 = (int64_t)(i % tiles_k) * BN;
+  // each XCD takes whole runs of tiles: they share a group's rows
+  constexpr int XCDS = 8;
+  const int64_t total = (int64_t)tiles * p.G, run = (total + XCDS - 1) / XCDS, at = blockIdx.x / XCDS, i = blockIdx.x % XCDS * run + at;
+  if (at >= run || i >= total) return;
+  const int g = (int)(i / tiles), j = (int)(i % tiles);
+  const int64_t n0 = (int64_t)(j / tiles_k) * BM, k0 = (int64_t)(j % tiles_k) * BN;
   const int64_t a = clamp64(p.off[g], 0, p.T), b = clamp64(p.off[g + 1], a, p.T);
   P tile;
   const Operand<T> dy{static_cast<const T*>(p.y) + a * p.ldy + n0, p.ldy, p.N - n0};
   const Operand<T> x{static_cast<const T*>(p.x) + a * p.ldx + k0, p.ldx, p.K - k0};
   tile.run(dy, x, b - a, lds);
   T* dw = static_cast<T*>(const_cast<void*>(p.w)) + g * p.sw + n0 * p.ldw + k0;
-  tile.each([&](int r, int j, int step, const typename P::acc_t& v) {
-    if (r < p.N - n0) store_row(dw + r * p.ldw, j, step, v, p.K - k0);
+  tile.each([&](int r, int c, int step, const typename P::acc_t& v) {
+    if (r < p.N - n0) store_row(dw + r * p.ldw, c, step, v, p.K - k0);
   });
+}
+
+template <class T, int BM, int BN> __global__ __launch_bounds__(256, 2) void grouped_dw_kernel(GroupedArgs p) {
+  using P = Tile<T, BM, BN, 2, 2, false, false, false>;
+  __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
+  dw_tile<T, P, BM, BN>(p, lds);
+}
+
+template <class T, int BM, int BN> __global__ __launch_bounds__(BM == 256 ? 512 : 256, 2) void grouped_dw_pipe_kernel(GroupedArgs p) {
+  using P = PipeTile<T, BM, BN, 2, BM == 256 ? 4 : 2, false, false>;
+  __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
+  dw_tile<T, P, BM, BN>(p, lds);
 }
 
 int size_of(int dtype) {
@@ -115,28 +168,47 @@ bool chunked(const void* p, int64_t ld, int64_t extent, int size) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (ld * size) % 16 == 0 && (extent * size) % 16 == 0;
 }
 
-template <class T, int B, bool WK> int run_rows(const GroupedArgs& p0, bool vec, hipStream_t st) {
+// row tiles there can be at most: a group adds less than one to its share of the rows
+template <class T, int B, bool WK, bool PIPE> int run_rows(const GroupedArgs& p0, hipStream_t st) {
   GroupedArgs p = p0;
   p.tiles_n = (int)((p.N + B - 1) / B);
-  const int64_t tiles = (p.T / B + p.G + (p.rest ? 2 : 0)) * p.tiles_n;
-  if (tiles > MAX_WORKGROUPS) return bgp_products_fail(-1, "bgp_grouped_gemm: %lld tiles are more than one launch holds", (long long)tiles);
-  return launch("bgp_grouped_gemm", vec ? grouped_rows_kernel<T, B, B, WK, true> : grouped_rows_kernel<T, B, B, WK, false>, dim3((unsigned)tiles),
-                dim3(256), st, p);
+  const int64_t tiles = (p.T / B + p.G + (p.rest ? 2 : 0)) * p.tiles_n + 7;
+  if (tiles > MAX_WORKGROUPS / 2) return bgp_products_fail(-1, "bgp_grouped_gemm: %lld tiles are more than one launch holds", (long long)tiles);
+  const dim3 grid((unsigned)tiles);
+  if constexpr (PIPE) return launch("bgp_grouped_gemm", grouped_rows_pipe_kernel<T, B, B, WK>, grid, dim3(B == 256 ? 512 : 256), st, p);
+  else return launch("bgp_grouped_gemm", grouped_rows_kernel<T, B, B, WK>, grid, dim3(256), st, p);
+}
+
+template <class T, bool WK> int rows_by_tile(const GroupedArgs& p, bool vec, hipStream_t st) {
+  vec = vec && pipe_fits(p.ldx, sizeof(T), true, 256) && pipe_fits(p.ldw, sizeof(T), WK, 256);
+  const bool small = p.T < (int64_t)p.G * 96;
+  if (!vec) return small ? run_rows<T, 64, WK, false>(p, st) : run_rows<T, 128, WK, false>(p, st);
+  if constexpr (sizeof(T) == 2)
+    if (p.T >= (int64_t)p.G * 256 && p.N >= 512) return run_rows<T, 256, WK, true>(p, st);
+  return small ? run_rows<T, 64, WK, true>(p, st) : run_rows<T, 128, WK, true>(p, st);
 }
 
 template <class T> int rows_by_type(const GroupedArgs& p, bool trans, bool vec, hipStream_t st) {
-  const bool small = p.T < (int64_t)p.G * 96;
-  if (small) return trans ? run_rows<T, 64, false>(p, vec, st) : run_rows<T, 64, true>(p, vec, st);
-  return trans ? run_rows<T, 128, false>(p, vec, st) : run_rows<T, 128, true>(p, vec, st);
+  return trans ? rows_by_tile<T, false>(p, vec, st) : rows_by_tile<T, true>(p, vec, st);
 }
 
-template <class T> int dw_by_type(const GroupedArgs& p0, bool vec, hipStream_t st) {
+template <class T, int B, bool PIPE> int run_dw(const GroupedArgs& p0, hipStream_t st) {
   GroupedArgs p = p0;
-  constexpr int B = 128;
   p.tiles_n = (int)((p.N + B - 1) / B);
-  const int64_t tiles = (int64_t)p.G * p.tiles_n * ((p.K + B - 1) / B);
-  if (tiles > MAX_WORKGROUPS) return bgp_products_fail(-1, "bgp_grouped_gemm_dw: %lld tiles are more than one launch holds", (long long)tiles);
-  return launch("bgp_grouped_gemm_dw", vec ? grouped_dw_kernel<T, B, B, true> : grouped_dw_kernel<T, B, B, false>, dim3((unsigned)tiles), dim3(256), st, p);
+  const int64_t tiles = (int64_t)p.G * p.tiles_n * ((p.K + B - 1) / B) + 7;
+  if (tiles > MAX_WORKGROUPS / 2) return bgp_products_fail(-1, "bgp_grouped_gemm_dw: %lld tiles are more than one launch holds", (long long)tiles);
+  const dim3 grid((unsigned)tiles);
+  if constexpr (PIPE) return launch("bgp_grouped_gemm_dw", grouped_dw_pipe_kernel<T, B, B>, grid, dim3(B == 256 ? 512 : 256), st, p);
+  else return launch("bgp_grouped_gemm_dw", grouped_dw_kernel<T, B, B>, grid, dim3(256), st, p);
+}
+
+template <class T> int dw_by_type(const GroupedArgs& p, bool vec, hipStream_t st) {
+  vec = vec && pipe_fits(p.ldx, sizeof(T), false, 256) && pipe_fits(p.ldy, sizeof(T), false, 256);
+  const bool small = (int64_t)p.G * ((p.N + 127) / 128) * ((p.K + 127) / 128) < 256;
+  if (!vec) return small ? run_dw<T, 64, false>(p, st) : run_dw<T, 128, false>(p, st);
+  if constexpr (sizeof(T) == 2)
+    if ((int64_t)p.G * (p.N / 256) * (p.K / 256) >= 256) return run_dw<T, 256, true>(p, st);
+  return small ? run_dw<T, 64, true>(p, st) : run_dw<T, 128, true>(p, st);
 }
 
 int check_sizes(const char* what, int dtype, int64_t T, int64_t N, int64_t K, int64_t G, const void* off) {

@@ -106,11 +106,16 @@ struct Int8Args {
 };
 
 // Y[i, j] = (C[i, j] +) sa[i] sb[j] sum_k A[i, k] B[j, k]: the sum exact in 32 bits, the rest in 64, one rounding
-template <class T, int BM, int BN, bool VEC> __global__ __launch_bounds__(256, 2) void int8_gemm_kernel(Int8Args p) {
-  using P = Tile<int8_t, BM, BN, 2, 2, true, true, VEC>;
+template <class T, class P, int BM, int BN> __device__ __forceinline__ void int8_tile(const Int8Args& p, char* lds) {
   using S = typename ScaleOf<T>::type;
-  __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
-  const int64_t m0 = (int64_t)(blockIdx.x / p.tiles_n) * BM, n0 = (int64_t)(blockIdx.x % p.tiles_n) * BN;
+  // each XCD takes a run of tiles, 8 row tiles deep (workgroups go to the 8 XCDs in turn; each has an L2 of its own)
+  constexpr int XCDS = 8, DEEP = 8;
+  const int tiles_m = (int)((p.M + BM - 1) / BM);
+  const int64_t total = (int64_t)tiles_m * p.tiles_n, run = (total + XCDS - 1) / XCDS, at = blockIdx.x / XCDS, t = blockIdx.x % XCDS * run + at;
+  if (at >= run || t >= total) return;
+  const int64_t strip = t / (DEEP * p.tiles_n);
+  const int in = (int)(t - strip * DEEP * p.tiles_n), deep = tiles_m - strip * DEEP < DEEP ? (int)(tiles_m - strip * DEEP) : DEEP;
+  const int64_t m0 = (strip * DEEP + in % deep) * BM, n0 = (int64_t)(in / deep) * BN;
   P tile;
   tile.run(Operand<int8_t>{p.a + m0 * p.lda, p.lda, p.M - m0}, Operand<int8_t>{p.b + n0 * p.ldb, p.ldb, p.N - n0}, p.K, lds);
   tile.each([&](int i, int j, int step, const v4i& v) {
@@ -130,14 +135,37 @@ template <class T, int BM, int BN, bool VEC> __global__ __launch_bounds__(256, 2
   });
 }
 
-template <class T> int int8_by_type(const Int8Args& p0, hipStream_t st) {
+// any operands, through registers
+template <class T, int BM, int BN> __global__ __launch_bounds__(256, 2) void int8_gemm_kernel(Int8Args p) {
+  using P = Tile<int8_t, BM, BN, 2, 2, true, true, false>;
+  __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
+  int8_tile<T, P, BM, BN>(p, lds);
+}
+
+// operands in whole chunks, pipelined
+template <class T, int BM, int BN> __global__ __launch_bounds__(BM == 256 ? 512 : 256, 2) void int8_gemm_pipe_kernel(Int8Args p) {
+  using P = PipeTile<int8_t, BM, BN, 2, BM == 256 ? 4 : 2, true, true>;
+  __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
+  int8_tile<T, P, BM, BN>(p, lds);
+}
+
+template <class T, int B, bool PIPE> int run_int8(const Int8Args& p0, hipStream_t st) {
   Int8Args p = p0;
-  constexpr int B = 128;
   p.tiles_n = (int)((p.N + B - 1) / B);
-  const int64_t tiles = (p.M + B - 1) / B * p.tiles_n;
-  if (tiles > MAX_WORKGROUPS) return bgp_products_fail(-1, "bgp_int8_gemm: %lld tiles are more than one launch holds", (long long)tiles);
-  const bool vec = reinterpret_cast<uintptr_t>(p.a) % 16 == 0 && reinterpret_cast<uintptr_t>(p.b) % 16 == 0 && p.lda % 16 == 0 && p.ldb % 16 == 0 && p.K % 16 == 0;
-  return launch("bgp_int8_gemm", vec ? int8_gemm_kernel<T, B, B, true> : int8_gemm_kernel<T, B, B, false>, dim3((unsigned)tiles), dim3(256), st, p);
+  const int64_t tiles = (p.M + B - 1) / B * p.tiles_n + 7;
+  if (tiles > MAX_WORKGROUPS / 2) return bgp_products_fail(-1, "bgp_int8_gemm: %lld tiles are more than one launch holds", (long long)tiles);
+  const dim3 grid((unsigned)tiles);
+  if constexpr (PIPE) return launch("bgp_int8_gemm", int8_gemm_pipe_kernel<T, B, B>, grid, dim3(B == 256 ? 512 : 256), st, p);
+  else return launch("bgp_int8_gemm", int8_gemm_kernel<T, B, B>, grid, dim3(256), st, p);
+}
+
+template <class T> int int8_by_type(const Int8Args& p, hipStream_t st) {
+  const bool vec = reinterpret_cast<uintptr_t>(p.a) % 16 == 0 && reinterpret_cast<uintptr_t>(p.b) % 16 == 0 && p.lda % 16 == 0 && p.ldb % 16 == 0 &&
+                   p.K % 16 == 0 && pipe_fits(p.lda, 1, true, 256) && pipe_fits(p.ldb, 1, true, 256);
+  const int64_t tiles = ((p.M + 127) / 128) * ((p.N + 127) / 128);
+  if (!vec) return tiles < 256 ? run_int8<T, 64, false>(p, st) : run_int8<T, 128, false>(p, st);
+  if (tiles >= 1024) return run_int8<T, 256, true>(p, st);
+  return tiles < 256 ? run_int8<T, 64, true>(p, st) : run_int8<T, 128, true>(p, st);
 }
 
 }  // namespace

@@ -134,6 +134,12 @@ template <class T, bool VEC> __device__ __forceinline__ uint4 load_chunk(const T
   return v;
 }
 
+// a value that all lanes hold, in scalar registers
+__device__ __forceinline__ int64_t scalar64(int64_t v) {
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((int)v), hi = __builtin_amdgcn_readfirstlane((int)(v >> 32));
+  return (int64_t)((uint64_t)hi << 32 | lo);
+}
+
 // one operand's share of a stage: ROWS x 128 bytes, fetched into registers by all NT threads, then stored to LDS
 template <class T, int ROWS, bool ALONG_K, bool VEC, int NT> struct Stage {
   static constexpr int CHUNKS = ROWS * 8, NL = CHUNKS / NT;
@@ -255,6 +261,150 @@ template <class T, int BM, int BN, int WX, int WW, bool XK, bool WK, bool VEC> s
       }
   }
 };
+
+__device__ __attribute__((aligned(16))) const uint4 zero_chunk = {0, 0, 0, 0};
+
+// The same tile for operands in whole aligned 16-byte chunks, as a pipeline: two buffers of a stage each, filled by loads
+// that write LDS themselves (global_load_lds, 16 bytes a lane: no registers, no LDS stores, one 32-bit offset per lane
+// and load against a scalar base) and issued a whole stage ahead; the fragments of the next half stage are read while the
+// matrix instructions of this one run.
+//   first half of stage b:   read the fragments of its second half; multiply those of the first.
+//   second half:             wait until stage b + 1 has arrived and this wave's own fragment reads of stage b are done;
+//                            barrier: both hold for every wave, so b's buffer is free; issue stage b + 2 into it; read
+//                            the fragments of b + 1's first half; multiply those of b's second.
+// A stage is 128 bytes of k, a whole cache line.  If k ends inside a stage, that last part comes first, through
+// registers and filled up with zeros; all others are whole.  Rows (columns) past the operand's end repeat its last one:
+// they only reach elements of D that are not stored.
+// Offsets inside a stage have 32 bits: pipe_fits() says whether an operand's do.
+template <class T, int BM, int BN, int WX, int WW, bool XK, bool WK> struct PipeTile {
+  static constexpr int NW = WX * WW, NT = 64 * NW, FA = BM / WX / 16, FB = BN / WW / 16;
+  static constexpr int KE = KSTAGE<T>;
+  static constexpr int XL = BM / 8 / NW, WL = BN / 8 / NW;  // loads of a wave per stage
+  static constexpr int BUF = (BM + BN) * 128, LDS_BYTES = 2 * BUF;
+  static_assert(BM / 8 % NW == 0 && BN / 8 % NW == 0, "every wave loads the same share of either operand");
+  using acc_t = typename Num<T>::acc;
+  acc_t acc[FB][FA];
+
+  __device__ __forceinline__ int wave() const { return __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); }
+  __device__ __forceinline__ int x0() const { return wave() / WW * (BM / WX); }
+  __device__ __forceinline__ int w0() const { return wave() % WW * (BN / WW); }
+
+  // a wave's loads of one operand: load l brings the 64 chunks from (wave + l NW) 64 on
+  template <int ROWS, bool ALONG_K> struct Source {
+    static constexpr int L = ROWS / 8 / NW;
+    const char* p;  // the stage's first byte
+    int64_t step;
+    uint32_t at[L];
+    __device__ __forceinline__ void start(const Operand<T>& o, int wave) {
+      constexpr int CPR = ALONG_K ? 8 : ROWS / CHE<T>;
+      p = reinterpret_cast<const char*>(scalar64(reinterpret_cast<int64_t>(o.p)));
+      step = scalar64((ALONG_K ? (int64_t)KE : KE * o.ld) * (int)sizeof(T));
+#pragma unroll
+      for (int l = 0; l < L; ++l) {
+        const int i = (wave + l * NW) * 64 + (int)(threadIdx.x & 63), row = i / CPR, c = swizzle<T, ALONG_K>(row, i % CPR, CPR);
+        const int last = o.rows < ROWS ? (int)o.rows - 1 : ROWS - 1;
+        if (ALONG_K) at[l] = (uint32_t)(row < last ? row : last) * (uint32_t)(o.ld * (int)sizeof(T)) + c * 16;
+        else at[l] = (uint32_t)row * (uint32_t)(o.ld * (int)sizeof(T)) + (c < last / CHE<T> ? c : last / CHE<T>) * 16;
+      }
+    }
+    __device__ __forceinline__ void issue(uint32_t lds) {
+#pragma unroll
+      for (int l = 0; l < L; ++l)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds + l * NW * 1024), "v"(at[l]), "s"(p) : "memory");
+      p += step;
+    }
+  };
+
+  __device__ __forceinline__ void run(const Operand<T>& x, const Operand<T>& w, int64_t k_length, char* lds) {
+#pragma unroll
+    for (int b = 0; b < FB; ++b)
+#pragma unroll
+      for (int a = 0; a < FA; ++a) acc[b][a] = acc_t{};
+    const int64_t klen = scalar64(k_length);
+    if (klen <= 0) return;
+    const int64_t whole = klen / KE * KE;
+    const bool tail = whole < klen;
+    const int stages = (int)(klen / KE) + tail;
+    const uint32_t base = (uint32_t)(uintptr_t)(BGP_LDS char*)lds + wave() * 1024;
+    Source<BM, XK> sx;
+    Source<BN, WK> sw;
+    sx.start(x, wave());
+    sw.start(w, wave());
+    auto issue = [&](int buf) {
+      sx.issue(base + buf * BUF);
+      sw.issue(base + buf * BUF + BM * 128);
+    };
+    if (tail) {
+      Stage<T, BM, XK, true, NT> tx;
+      Stage<T, BN, WK, true, NT> tw;
+      tx.fetch(x, whole, klen);
+      tw.fetch(w, whole, klen);
+      tx.store(lds);
+      tw.store(lds + BM * 128);
+    } else {
+      issue(0);
+    }
+    if (stages > 1) issue(1);
+    if (stages > 1 && !tail) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(XL + WL) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    uint4 fx[2][FA], fw[2][FB];
+    auto read = [&](int buf, int half) {
+      const char* at = lds + buf * BUF;
+#pragma unroll
+      for (int a = 0; a < FA; ++a) fx[half][a] = fragment<T, BM, XK>(at, x0() + a * 16, half);
+#pragma unroll
+      for (int b = 0; b < FB; ++b) fw[half][b] = fragment<T, BN, WK>(at + BM * 128, w0() + b * 16, half);
+    };
+    auto multiply = [&](int half) {
+#pragma unroll
+      for (int b = 0; b < FB; ++b)
+#pragma unroll
+        for (int a = 0; a < FA; ++a) acc[b][a] = Num<T>::mma(fw[half][b], fx[half][a], acc[b][a]);
+      interleave();
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    read(0, 0);
+    for (int s = 0, buf = 0; s < stages; ++s, buf ^= 1) {
+      __builtin_amdgcn_sched_barrier(0);
+      read(buf, 1);
+      multiply(0);
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      if (s + 2 < stages) issue(buf);
+      __builtin_amdgcn_sched_barrier(0);
+      read(buf ^ 1, 0);  // behind the last stage: whatever is there, not used
+      multiply(1);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  }
+
+  // the order the scheduler is to give an iteration: the LDS reads spread evenly over the matrix instructions
+  static constexpr int reads_of(bool along_k) { return along_k ? 1 : sizeof(T) == 2 ? 2 : CHE<T>; }
+  __device__ __forceinline__ void interleave() const {
+    constexpr int R = FA * reads_of(XK) + FB * reads_of(WK), M = FA * FB * (sizeof(T) == 8 ? 2 : sizeof(T) == 4 ? 4 : 1);
+    constexpr int EACH = M / R > 0 ? M / R : 1;
+#pragma unroll
+    for (int i = 0; i < (R < M ? R : M); ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x100, R > M ? (R + M - 1) / M : 1, 0);  // LDS reads
+      __builtin_amdgcn_sched_group_barrier(0x008, EACH, 0);                         // matrix instructions
+    }
+  }
+
+  template <class F> __device__ __forceinline__ void each(F&& f) const {
+    const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+#pragma unroll
+    for (int a = 0; a < FA; ++a)
+#pragma unroll
+      for (int b = 0; b < FB; ++b) {
+        if (sizeof(T) == 8) f(x0() + a * 16 + r, w0() + b * 16 + q, 4, acc[b][a]);
+        else f(x0() + a * 16 + r, w0() + b * 16 + q * 4, 1, acc[b][a]);
+      }
+  }
+};
+
+// whether an operand's offsets inside a stage fit 32 bits: up to `rows` rows of it along k, a stage's rows of k otherwise
+inline bool pipe_fits(int64_t ld, int size, bool along_k, int rows) {
+  return (along_k ? rows : 128 / size) * ld * size < (int64_t)1 << 32;
+}
 
 // D[j .. j + 3 step] = values where they are inside n columns
 template <class T, class A> __device__ __forceinline__ void store_row(T* row, int64_t j, int step, const A& v, int64_t n) {
