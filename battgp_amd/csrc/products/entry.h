@@ -34,3 +34,10 @@ template <class... A> int launch(const char* what, void (*kernel)(A...), dim3 gr
   const hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, block, ptrs, 0, stream);
   return e == hipSuccess ? 0 : bgp_products_fail(-2, "%s: launch failed: %s", what, hipGetErrorString(e));
 }
+
+// How a product is cut: straight from memory in tiles of 16 or 32, through registers (any operands) or pipelined (whole
+// chunks) in tiles of 64, 128 or 256.
+enum Cut { DIRECT16, DIRECT32, PLAIN64, PLAIN128, PIPE64, PIPE128, PIPE256 };
+constexpr int tile_of(int cut) {
+  return cut == DIRECT16 ? 16 : cut == DIRECT32 ? 32 : cut == PLAIN64 || cut == PIPE64 ? 64 : cut == PIPE256 ? 256 : 128;
+}

@@ -121,6 +121,13 @@ template <class T, int BM, int BN, bool WK> __global__ __launch_bounds__(BM == 2
   rows_tile<T, P, BM, BN, WK>(p, lds);
 }
 
+// small ones, straight from memory
+template <class T, int F, bool WK> __global__ __launch_bounds__(256) void grouped_rows_direct_kernel(GroupedArgs p) {
+  using P = DirectTile<T, F, F, true, WK>;
+  __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
+  rows_tile<T, P, 16 * F, 16 * F, WK>(p, lds);
+}
+
 // dW_g[n, k] = sum over the rows t of g of dY[t, n] X[t, k]
 template <class T, class P, int BM, int BN> __device__ __forceinline__ void dw_tile(const GroupedArgs& p, char* lds) {
   const int tiles_k = (int)((p.K + BN - 1) / BN), tiles = p.tiles_n * tiles_k;
@@ -153,6 +160,12 @@ template <class T, int BM, int BN> __global__ __launch_bounds__(BM == 256 ? 512 
   dw_tile<T, P, BM, BN>(p, lds);
 }
 
+template <class T, int F> __global__ __launch_bounds__(256) void grouped_dw_direct_kernel(GroupedArgs p) {
+  using P = DirectTile<T, F, F, false, false>;
+  __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
+  dw_tile<T, P, 16 * F, 16 * F>(p, lds);
+}
+
 int size_of(int dtype) {
   switch (dtype) {
     case BGP_F64: return 8;
@@ -168,47 +181,81 @@ bool chunked(const void* p, int64_t ld, int64_t extent, int size) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (ld * size) % 16 == 0 && (extent * size) % 16 == 0;
 }
 
-// row tiles there can be at most: a group adds less than one to its share of the rows
-template <class T, int B, bool WK, bool PIPE> int run_rows(const GroupedArgs& p0, hipStream_t st) {
+int pick_rows(int size, bool direct, bool vec, int64_t T, int64_t N, int64_t K, int64_t G) {
+  const int64_t t64 = (T / 64 + G) * ((N + 63) / 64);
+  if (direct && t64 < 256) return T <= 16 * G ? DIRECT16 : DIRECT32;
+  const bool small = T < G * 96;
+  if (!vec) return small ? PLAIN64 : PLAIN128;
+  if (size == 2 && T >= G * 256 && N >= 512) return PIPE256;
+  return small ? PIPE64 : PIPE128;
+}
+
+int pick_dw(int size, bool vec, int64_t T, int64_t N, int64_t K, int64_t G) {
+  const int64_t t128 = G * ((N + 127) / 128) * ((K + 127) / 128);
+  if (size >= 4 && t128 < 128) return DIRECT32;
+  if (!vec) return t128 < 256 ? PLAIN64 : PLAIN128;
+  if (size == 2 && G * (N / 256) * (K / 256) >= 256) return PIPE256;
+  return t128 < 256 ? PIPE64 : PIPE128;
+}
+
+template <class T, bool WK, int CUT> int run_rows(const GroupedArgs& p0, hipStream_t st) {
+  const char* what = "bgp_grouped_gemm";
+  constexpr int B = tile_of(CUT);
   GroupedArgs p = p0;
   p.tiles_n = (int)((p.N + B - 1) / B);
+  // row tiles there can be at most: a group adds less than one to its share of the rows
   const int64_t tiles = (p.T / B + p.G + (p.rest ? 2 : 0)) * p.tiles_n + 7;
-  if (tiles > MAX_WORKGROUPS / 2) return bgp_products_fail(-1, "bgp_grouped_gemm: %lld tiles are more than one launch holds", (long long)tiles);
+  if (tiles > MAX_WORKGROUPS / 2) return bgp_products_fail(-1, "%s: %lld tiles are more than one launch holds", what, (long long)tiles);
   const dim3 grid((unsigned)tiles);
-  if constexpr (PIPE) return launch("bgp_grouped_gemm", grouped_rows_pipe_kernel<T, B, B, WK>, grid, dim3(B == 256 ? 512 : 256), st, p);
-  else return launch("bgp_grouped_gemm", grouped_rows_kernel<T, B, B, WK>, grid, dim3(256), st, p);
+  if constexpr (CUT <= DIRECT32) return launch(what, grouped_rows_direct_kernel<T, B / 16, WK>, grid, dim3(256), st, p);
+  else if constexpr (CUT <= PLAIN128) return launch(what, grouped_rows_kernel<T, B, B, WK>, grid, dim3(256), st, p);
+  else return launch(what, grouped_rows_pipe_kernel<T, B, B, WK>, grid, dim3(B == 256 ? 512 : 256), st, p);
 }
 
 template <class T, bool WK> int rows_by_tile(const GroupedArgs& p, bool vec, hipStream_t st) {
+  constexpr bool direct = WK || sizeof(T) >= 4;
   vec = vec && pipe_fits(p.ldx, sizeof(T), true, 256) && pipe_fits(p.ldw, sizeof(T), WK, 256);
-  const bool small = p.T < (int64_t)p.G * 96;
-  if (!vec) return small ? run_rows<T, 64, WK, false>(p, st) : run_rows<T, 128, WK, false>(p, st);
+  int cut = pick_rows(sizeof(T), direct, vec, p.T, p.N, p.K, p.G);
+  if constexpr (direct) {
+    if (cut == DIRECT16) return run_rows<T, WK, DIRECT16>(p, st);
+    if (cut == DIRECT32) return run_rows<T, WK, DIRECT32>(p, st);
+  }
+  if (cut == PLAIN64) return run_rows<T, WK, PLAIN64>(p, st);
+  if (cut == PLAIN128) return run_rows<T, WK, PLAIN128>(p, st);
   if constexpr (sizeof(T) == 2)
-    if (p.T >= (int64_t)p.G * 256 && p.N >= 512) return run_rows<T, 256, WK, true>(p, st);
-  return small ? run_rows<T, 64, WK, true>(p, st) : run_rows<T, 128, WK, true>(p, st);
+    if (cut == PIPE256) return run_rows<T, WK, PIPE256>(p, st);
+  return cut == PIPE64 ? run_rows<T, WK, PIPE64>(p, st) : run_rows<T, WK, PIPE128>(p, st);
 }
 
 template <class T> int rows_by_type(const GroupedArgs& p, bool trans, bool vec, hipStream_t st) {
   return trans ? rows_by_tile<T, false>(p, vec, st) : rows_by_tile<T, true>(p, vec, st);
 }
 
-template <class T, int B, bool PIPE> int run_dw(const GroupedArgs& p0, hipStream_t st) {
+template <class T, int CUT> int run_dw(const GroupedArgs& p0, hipStream_t st) {
+  const char* what = "bgp_grouped_gemm_dw";
+  constexpr int B = tile_of(CUT);
   GroupedArgs p = p0;
   p.tiles_n = (int)((p.N + B - 1) / B);
   const int64_t tiles = (int64_t)p.G * p.tiles_n * ((p.K + B - 1) / B) + 7;
-  if (tiles > MAX_WORKGROUPS / 2) return bgp_products_fail(-1, "bgp_grouped_gemm_dw: %lld tiles are more than one launch holds", (long long)tiles);
+  if (tiles > MAX_WORKGROUPS / 2) return bgp_products_fail(-1, "%s: %lld tiles are more than one launch holds", what, (long long)tiles);
   const dim3 grid((unsigned)tiles);
-  if constexpr (PIPE) return launch("bgp_grouped_gemm_dw", grouped_dw_pipe_kernel<T, B, B>, grid, dim3(B == 256 ? 512 : 256), st, p);
-  else return launch("bgp_grouped_gemm_dw", grouped_dw_kernel<T, B, B>, grid, dim3(256), st, p);
+  if constexpr (CUT <= DIRECT32) return launch(what, grouped_dw_direct_kernel<T, B / 16>, grid, dim3(256), st, p);
+  else if constexpr (CUT <= PLAIN128) return launch(what, grouped_dw_kernel<T, B, B>, grid, dim3(256), st, p);
+  else return launch(what, grouped_dw_pipe_kernel<T, B, B>, grid, dim3(B == 256 ? 512 : 256), st, p);
 }
 
 template <class T> int dw_by_type(const GroupedArgs& p, bool vec, hipStream_t st) {
   vec = vec && pipe_fits(p.ldx, sizeof(T), false, 256) && pipe_fits(p.ldy, sizeof(T), false, 256);
-  const bool small = (int64_t)p.G * ((p.N + 127) / 128) * ((p.K + 127) / 128) < 256;
-  if (!vec) return small ? run_dw<T, 64, false>(p, st) : run_dw<T, 128, false>(p, st);
+  const int cut = pick_dw(sizeof(T), vec, p.T, p.N, p.K, p.G);
+  if constexpr (sizeof(T) >= 4) {
+    if (cut == DIRECT16) return run_dw<T, DIRECT16>(p, st);
+    if (cut == DIRECT32) return run_dw<T, DIRECT32>(p, st);
+  }
+  if (cut == PLAIN64) return run_dw<T, PLAIN64>(p, st);
+  if (cut == PLAIN128) return run_dw<T, PLAIN128>(p, st);
   if constexpr (sizeof(T) == 2)
-    if ((int64_t)p.G * (p.N / 256) * (p.K / 256) >= 256) return run_dw<T, 256, true>(p, st);
-  return small ? run_dw<T, 64, true>(p, st) : run_dw<T, 128, true>(p, st);
+    if (cut == PIPE256) return run_dw<T, PIPE256>(p, st);
+  return cut == PIPE64 ? run_dw<T, PIPE64>(p, st) : run_dw<T, PIPE128>(p, st);
 }
 
 int check_sizes(const char* what, int dtype, int64_t T, int64_t N, int64_t K, int64_t G, const void* off) {

@@ -47,54 +47,186 @@ struct QuantArgs {
   int8_t* q;
   void *scale, *rest;
   int64_t M, K, ldx, ldq, ldr;
-  int pow2;
 };
 
-// One workgroup per row: the largest magnitude, then the codes.  The second pass finds the row in the caches.
-template <class T> __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantArgs p) {
-  using S = typename ScaleOf<T>::type;
-  __shared__ double part[4];
-  for (int64_t row = blockIdx.x; row < p.M; row += gridDim.x) {
-    const T* x = static_cast<const T*>(p.x) + row * p.ldx;
-    double top = 0.0;
-    for (int64_t k = threadIdx.x; k < p.K; k += 256) {
-      const double v = fabs(widen(x[k]));
-      top = v > top || v != v ? v : top;  // a NaN stays
-      if (top != top) break;
+// Quantisation computes in fp32 for the types up to 32 bits and in fp64 for fp64.  The largest magnitude is found on the
+// bit patterns without their sign, where an infinity is above every number and a NaN above that.
+template <class T> struct Quant {
+  using F = float;
+  using B = uint32_t;
+  static constexpr F tiny = 0x1p-126f;
+  static constexpr B inf = 0x7f800000u;
+};
+template <> struct Quant<double> {
+  using F = double;
+  using B = uint64_t;
+  static constexpr F tiny = 0x1p-1022;
+  static constexpr B inf = 0x7ff0000000000000ull;
+};
+template <class A, class C> __device__ __forceinline__ A bits_as(C v) {
+  static_assert(sizeof(A) == sizeof(C), "same size");
+  A r;
+  __builtin_memcpy(&r, &v, sizeof(A));
+  return r;
+}
+template <class T> __device__ __forceinline__ typename Quant<T>::B magnitude(typename Quant<T>::F v) {
+  using B = typename Quant<T>::B;
+  return bits_as<B>(v) & (~(B)0 >> 1);
+}
+
+// A row by TPR threads, 8 elements to a unit, U units a thread: the row stays in registers between the search for its
+// scale and the codes, so x is read once.  LONG: rows of more than 8 U TPR elements, read twice (the second time out
+// of the caches).
+template <class T, bool POW2, int TPR, int U, bool LONG> __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void quantize_rows_kernel(QuantArgs p) {
+  using F = typename Quant<T>::F;
+  using B = typename Quant<T>::B;
+  constexpr int NT = TPR > 256 ? TPR : 256, RPW = NT / TPR, WPR = TPR / 64;
+  __shared__ B part[NT / 64];
+  const int lane = threadIdx.x % TPR;
+  const int64_t row = (int64_t)blockIdx.x * RPW + threadIdx.x / TPR;
+  const bool mine = row < p.M;
+  const T* x = static_cast<const T*>(p.x) + (mine ? row : 0) * p.ldx;
+  const int64_t K = mine ? p.K : 0;
+  F v[U][8];
+  auto load = [&](int64_t k, F* f) {
+    T e[8] = {};
+    if (k + 8 <= K) {
+      constexpr int N = (int)sizeof(T) / 2;  // 16-byte chunks
+#pragma unroll
+      for (int c = 0; c < N; ++c) {
+        const uint4 u = load_chunk<T, false>(x + k + c * CHE<T>, CHE<T>);
+        __builtin_memcpy(e + c * CHE<T>, &u, 16);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (k + j < K) e[j] = x[k + j];
     }
 #pragma unroll
-    for (int d = 32; d > 0; d >>= 1) {
-      const double v = __shfl_xor(top, d);
-      top = v > top || v != v ? v : top;
+    for (int j = 0; j < 8; ++j) f[j] = (F)widen(e[j]);
+  };
+  B top = 0;
+  auto look = [&](const F* f) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = magnitude<T>(f[j]) > top ? magnitude<T>(f[j]) : top;
+  };
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    load((int64_t)(u * TPR + lane) * 8, v[u]);
+    look(v[u]);
+  }
+  if (LONG)
+    for (int64_t k = (int64_t)(U * TPR + lane) * 8; k < K; k += TPR * 8) {
+      F f[8];
+      load(k, f);
+      look(f);
     }
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) {
+    const B o = __shfl_xor(top, d);
+    top = o > top ? o : top;
+  }
+  if (WPR > 1) {
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
     __syncthreads();
-    top = part[0];
+    const int first = threadIdx.x / TPR * WPR;
 #pragma unroll
-    for (int w = 1; w < 4; ++w) top = part[w] > top || part[w] != part[w] ? part[w] : top;
-    constexpr double tiny = sizeof(S) == 8 ? 0x1p-1022 : 0x1p-126;
-    double scale;
-    const bool finite = top - top == 0.0;
-    if (!finite) {
-      scale = top;
-    } else if (p.pow2) {
-      int e;
-      const double m = frexp(top, &e);  // top = m 2^e, 1/2 <= m < 1
-      scale = top > 0.0 ? ldexp(1.0, e - 7 + (m > 127.0 / 128.0)) : 0.0;
-    } else {
-      scale = (double)(S)(top / 127.0);
-    }
-    if (finite && scale < tiny) scale = tiny;
-    if (threadIdx.x == 0) static_cast<S*>(p.scale)[row] = (S)scale;
-    for (int64_t k = threadIdx.x; k < p.K; k += 256) {
-      const double v = widen(x[k]);
-      double q = finite ? rint(v / scale) : 0.0;
-      q = fmin(fmax(q, -127.0), 127.0);
-      p.q[row * p.ldq + k] = (int8_t)q;
-      if (p.rest) static_cast<T*>(p.rest)[row * p.ldr + k] = narrow<T>(v - q * scale);
-    }
-    __syncthreads();  // the next row's maxima overwrite part[]
+    for (int w = 0; w < WPR; ++w) top = part[first + w] > top ? part[first + w] : top;
   }
+  const bool finite = top < Quant<T>::inf;
+  F scale = bits_as<F>(top);
+  if (finite) {
+    if (POW2) {
+      // top = m 2^e with 1/2 <= m < 1: the smallest p with top <= 127 p is 2^(e - 7) or twice that
+      int e;
+      const F m = sizeof(F) == 8 ? (F)frexp((double)scale, &e) : (F)frexpf((float)scale, &e);
+      scale = scale > 0 ? (F)ldexp(1.0, e - 7 + (m > (F)(127.0 / 128.0))) : (F)0;
+    } else {
+      scale = scale / (F)127;
+    }
+    if (scale < Quant<T>::tiny) scale = Quant<T>::tiny;
+  }
+  if (lane == 0 && mine) static_cast<F*>(p.scale)[row] = scale;
+  const F inv = (F)1 / scale;
+  auto put = [&](int64_t k, const F* f) {
+    int8_t q[8];
+    T r[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      F t = 0, left = f[j];
+      if (finite) {
+        if (sizeof(F) == 8 && !POW2) {
+          t = rint(f[j] / scale);
+          left = fma(-t, scale, f[j]);
+        } else {
+          // The product with the reciprocal is a hair off the quotient, so t may be the wrong neighbour where the quotient
+          // lies next to a half; what is left over says so, and it is exact: a multiple of half the last place of
+          // the scale, not larger than the scale.  (A power of two: the product is exact, and t right.)
+          t = rint(f[j] * inv);
+          left = fma(-t, scale, f[j]);
+          if (!POW2) {
+            const F twice = fabs(left) * 2;
+            if (twice > scale || (twice == scale && ((int)t & 1))) {
+              const F up = left > 0 ? (F)1 : (F)-1;
+              t += up;
+              left = fma(-up, scale, left);
+            }
+          }
+        }
+      } else {
+        left = f[j] - f[j] + bits_as<F>(~(B)0);  // no number
+      }
+      q[j] = (int8_t)t;
+      r[j] = round_to<T, F>(left);
+    }
+    int8_t* out = p.q + row * p.ldq + k;
+    T* rest = p.rest ? static_cast<T*>(p.rest) + row * p.ldr + k : nullptr;
+    if (k + 8 <= K) {
+      struct __attribute__((packed, aligned(1))) Eight { int8_t e[8]; } o;
+      __builtin_memcpy(&o, q, 8);
+      *reinterpret_cast<Eight*>(out) = o;
+      if (rest) {
+        constexpr int N = (int)sizeof(T) / 2;
+#pragma unroll
+        for (int c = 0; c < N; ++c) {
+          Chunk<sizeof(T)> u;
+          __builtin_memcpy(&u, r + c * CHE<T>, 16);
+          *reinterpret_cast<Chunk<sizeof(T)>*>(rest + c * CHE<T>) = u;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (k + j < K) {
+          out[j] = q[j];
+          if (rest) rest[j] = r[j];
+        }
+    }
+  };
+#pragma unroll
+  for (int u = 0; u < U; ++u) put((int64_t)(u * TPR + lane) * 8, v[u]);
+  if (LONG)
+    for (int64_t k = (int64_t)(U * TPR + lane) * 8; k < K; k += TPR * 8) {
+      F f[8];
+      load(k, f);
+      put(k, f);
+    }
+}
+
+template <class T, bool POW2> int quantize_by_length(const QuantArgs& p, hipStream_t st) {
+  const char* what = "bgp_quantize_rows";
+  // a wave per row up to 2048 elements, a workgroup of 4 waves up to 8192, of 16 beyond
+  const int rows = p.K <= 2048 ? 4 : 1;
+  const int64_t groups = (p.M + rows - 1) / rows;
+  if (groups > MAX_WORKGROUPS / 4) return bgp_products_fail(-1, "%s: %lld rows are more than one launch holds", what, (long long)p.M);
+  const dim3 grid((unsigned)groups);
+  if (p.K <= 2048) return launch(what, quantize_rows_kernel<T, POW2, 64, 4, false>, grid, dim3(256), st, p);
+  if (p.K <= 8192) return launch(what, quantize_rows_kernel<T, POW2, 256, 4, false>, grid, dim3(256), st, p);
+  return launch(what, quantize_rows_kernel<T, POW2, 1024, 4, true>, grid, dim3(1024), st, p);
+}
+
+template <class T> int quantize_by_type(const QuantArgs& p, int pow2, hipStream_t st) {
+  return pow2 ? quantize_by_length<T, true>(p, st) : quantize_by_length<T, false>(p, st);
 }
 
 struct Int8Args {
@@ -149,23 +281,47 @@ template <class T, int BM, int BN> __global__ __launch_bounds__(BM == 256 ? 512 
   int8_tile<T, P, BM, BN>(p, lds);
 }
 
-template <class T, int B, bool PIPE> int run_int8(const Int8Args& p0, hipStream_t st) {
+// small ones, straight from memory
+template <class T, int F> __global__ __launch_bounds__(256) void int8_gemm_direct_kernel(Int8Args p) {
+  using P = DirectTile<int8_t, F, F, true, true>;
+  __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
+  int8_tile<T, P, 16 * F, 16 * F>(p, lds);
+}
+
+template <class T, int CUT> int run_int8(const Int8Args& p0, hipStream_t st) {
+  const char* what = "bgp_int8_gemm";
+  constexpr int B = tile_of(CUT);
   Int8Args p = p0;
   p.tiles_n = (int)((p.N + B - 1) / B);
   const int64_t tiles = (p.M + B - 1) / B * p.tiles_n + 7;
-  if (tiles > MAX_WORKGROUPS / 2) return bgp_products_fail(-1, "bgp_int8_gemm: %lld tiles are more than one launch holds", (long long)tiles);
+  if (tiles > MAX_WORKGROUPS / 2) return bgp_products_fail(-1, "%s: %lld tiles are more than one launch holds", what, (long long)tiles);
   const dim3 grid((unsigned)tiles);
-  if constexpr (PIPE) return launch("bgp_int8_gemm", int8_gemm_pipe_kernel<T, B, B>, grid, dim3(B == 256 ? 512 : 256), st, p);
-  else return launch("bgp_int8_gemm", int8_gemm_kernel<T, B, B>, grid, dim3(256), st, p);
+  if constexpr (CUT <= DIRECT32) return launch(what, int8_gemm_direct_kernel<T, B / 16>, grid, dim3(256), st, p);
+  else if constexpr (CUT <= PLAIN128) return launch(what, int8_gemm_kernel<T, B, B>, grid, dim3(256), st, p);
+  else return launch(what, int8_gemm_pipe_kernel<T, B, B>, grid, dim3(B == 256 ? 512 : 256), st, p);
+}
+
+int pick_int8(bool vec, int64_t M, int64_t N, int64_t K) {
+  const int64_t t64 = ((M + 63) / 64) * ((N + 63) / 64), t128 = ((M + 127) / 128) * ((N + 127) / 128);
+  if (M <= 16) return DIRECT16;
+  if (t64 < 256) return DIRECT32;
+  if (!vec) return t128 < 256 ? PLAIN64 : PLAIN128;
+  if (t128 >= 1024) return PIPE256;
+  return t128 < 256 ? PIPE64 : PIPE128;
 }
 
 template <class T> int int8_by_type(const Int8Args& p, hipStream_t st) {
   const bool vec = reinterpret_cast<uintptr_t>(p.a) % 16 == 0 && reinterpret_cast<uintptr_t>(p.b) % 16 == 0 && p.lda % 16 == 0 && p.ldb % 16 == 0 &&
                    p.K % 16 == 0 && pipe_fits(p.lda, 1, true, 256) && pipe_fits(p.ldb, 1, true, 256);
-  const int64_t tiles = ((p.M + 127) / 128) * ((p.N + 127) / 128);
-  if (!vec) return tiles < 256 ? run_int8<T, 64, false>(p, st) : run_int8<T, 128, false>(p, st);
-  if (tiles >= 1024) return run_int8<T, 256, true>(p, st);
-  return tiles < 256 ? run_int8<T, 64, true>(p, st) : run_int8<T, 128, true>(p, st);
+  switch (pick_int8(vec, p.M, p.N, p.K)) {
+    case DIRECT16: return run_int8<T, DIRECT16>(p, st);
+    case DIRECT32: return run_int8<T, DIRECT32>(p, st);
+    case PLAIN64: return run_int8<T, PLAIN64>(p, st);
+    case PLAIN128: return run_int8<T, PLAIN128>(p, st);
+    case PIPE64: return run_int8<T, PIPE64>(p, st);
+    case PIPE128: return run_int8<T, PIPE128>(p, st);
+    default: return run_int8<T, PIPE256>(p, st);
+  }
 }
 
 }  // namespace
@@ -190,14 +346,13 @@ extern "C" int bgp_quantize_rows(int device, void* stream, int dtype, int64_t M,
   if (ldx < K || ldq < K || (rest && ldr < K)) return bgp_products_fail(-1, "%s: bad strides ldx=%lld ldq=%lld ldr=%lld", what, (long long)ldx, (long long)ldq, (long long)ldr);
   DeviceScope scope(device);
   if (int rc = scope.check(what)) return rc;
-  const QuantArgs p{x, q, scale, rest, M, K, ldx, ldq, ldr, pow2 != 0};
-  const dim3 grid((unsigned)(M < MAX_WORKGROUPS ? M : MAX_WORKGROUPS)), block(256);
+  const QuantArgs p{x, q, scale, rest, M, K, ldx, ldq, ldr};
   const hipStream_t st = static_cast<hipStream_t>(stream);
   switch (dtype) {
-    case BGP_F64: return launch(what, quantize_rows_kernel<double>, grid, block, st, p);
-    case BGP_F32: return launch(what, quantize_rows_kernel<float>, grid, block, st, p);
-    case BGP_BF16: return launch(what, quantize_rows_kernel<bf16_t>, grid, block, st, p);
-    default: return launch(what, quantize_rows_kernel<f16_t>, grid, block, st, p);
+    case BGP_F64: return quantize_by_type<double>(p, pow2, st);
+    case BGP_F32: return quantize_by_type<float>(p, pow2, st);
+    case BGP_BF16: return quantize_by_type<bf16_t>(p, pow2, st);
+    default: return quantize_by_type<f16_t>(p, pow2, st);
   }
 }
 

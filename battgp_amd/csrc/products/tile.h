@@ -401,6 +401,123 @@ template <class T, int BM, int BN, int WX, int WW, bool XK, bool WK> struct Pipe
   }
 };
 
+// The tile for small problems, where a wait for every stage costs more than what is multiplied: 16 FA x 16 FB elements of D
+// by 4 waves that split k between them and add up in LDS at the end.  Fragments come straight from memory, several
+// in flight, without a barrier; operands of any alignment.  Along rows the elements are gathered one by one, which
+// suits 32- and 64-bit types (16 lanes read 64 or 128 consecutive bytes).
+template <class T, int FA, int FB, bool XK, bool WK> struct DirectTile {
+  static constexpr int NW = 4, BM = 16 * FA, BN = 16 * FB;
+  static constexpr int KE = KSTAGE<T>, FLIGHT = FA * FB == 1 ? 4 : 2;  // stages of 128 bytes of k whose loads are in flight
+  using acc_t = typename Num<T>::acc;
+  static constexpr int LDS_BYTES = NW * FA * FB * 64 * (int)sizeof(acc_t);
+  static_assert((XK && WK) || sizeof(T) >= 4, "16-bit types along rows need the transposing reads of the LDS tiles");
+  acc_t acc[FB][FA];
+
+  // this lane's 16 bytes of one 16-row block and half stage
+  template <bool ALONG_K> struct Source {
+    const T* p;
+    int64_t ld;
+    __device__ __forceinline__ void start(const Operand<T>& o, int r0) {
+      const int lane = threadIdx.x & 63, r = r0 + (lane & 15), k = (lane >> 4) * CHE<T>;
+      const int64_t row = r < o.rows ? r : o.rows - 1;  // past the end: the last one again, for elements that are not stored
+      ld = o.ld;
+      p = ALONG_K ? o.p + row * o.ld + k : o.p + row + k * o.ld;
+    }
+    __device__ __forceinline__ uint4 load(int64_t k) const {
+      if constexpr (ALONG_K) {
+        return load_chunk<T, false>(p + k, CHE<T>);
+      } else {
+        T e[CHE<T>];
+#pragma unroll
+        for (int j = 0; j < CHE<T>; ++j) e[j] = p[(k + j) * ld];
+        uint4 v;
+        __builtin_memcpy(&v, e, 16);
+        return v;
+      }
+    }
+    __device__ __forceinline__ uint4 load_end(int64_t k, int64_t klen) const {
+      const int64_t left = klen - k - ((threadIdx.x & 63) >> 4) * CHE<T>;
+      if constexpr (ALONG_K) {
+        return load_chunk<T, false>(p + k, left);
+      } else {
+        T e[CHE<T>] = {};
+#pragma unroll
+        for (int j = 0; j < CHE<T>; ++j)
+          if (j < left) e[j] = p[(k + j) * ld];
+        uint4 v;
+        __builtin_memcpy(&v, e, 16);
+        return v;
+      }
+    }
+  };
+
+  __device__ __forceinline__ void run(const Operand<T>& x, const Operand<T>& w, int64_t klen, char* lds) {
+#pragma unroll
+    for (int b = 0; b < FB; ++b)
+#pragma unroll
+      for (int a = 0; a < FA; ++a) acc[b][a] = acc_t{};
+    const int wave = threadIdx.x >> 6;
+    const int64_t share = ((klen + KE - 1) / KE + NW - 1) / NW * KE, end = (wave + 1) * share < klen ? (wave + 1) * share : klen;
+    int64_t k = wave * share;
+    if (k < end) {
+      Source<XK> sx[FA];
+      Source<WK> sw[FB];
+#pragma unroll
+      for (int a = 0; a < FA; ++a) sx[a].start(x, a * 16);
+#pragma unroll
+      for (int b = 0; b < FB; ++b) sw[b].start(w, b * 16);
+      for (; k + FLIGHT * KE <= end; k += FLIGHT * KE) {
+        uint4 fx[2 * FLIGHT][FA], fw[2 * FLIGHT][FB];
+#pragma unroll
+        for (int s = 0; s < 2 * FLIGHT; ++s) {
+#pragma unroll
+          for (int b = 0; b < FB; ++b) fw[s][b] = sw[b].load(k + s * (KE / 2));
+#pragma unroll
+          for (int a = 0; a < FA; ++a) fx[s][a] = sx[a].load(k + s * (KE / 2));
+        }
+#pragma unroll
+        for (int s = 0; s < 2 * FLIGHT; ++s)
+#pragma unroll
+          for (int b = 0; b < FB; ++b)
+#pragma unroll
+            for (int a = 0; a < FA; ++a) acc[b][a] = Num<T>::mma(fw[s][b], fx[s][a], acc[b][a]);
+      }
+      for (; k < end; k += KE / 2) {
+        uint4 fx[FA], fw[FB];
+#pragma unroll
+        for (int b = 0; b < FB; ++b) fw[b] = sw[b].load_end(k, end);
+#pragma unroll
+        for (int a = 0; a < FA; ++a) fx[a] = sx[a].load_end(k, end);
+#pragma unroll
+        for (int b = 0; b < FB; ++b)
+#pragma unroll
+          for (int a = 0; a < FA; ++a) acc[b][a] = Num<T>::mma(fw[b], fx[a], acc[b][a]);
+      }
+    }
+    acc_t* part = reinterpret_cast<acc_t*>(lds) + (threadIdx.x & 63);
+#pragma unroll
+    for (int b = 0; b < FB; ++b)
+#pragma unroll
+      for (int a = 0; a < FA; ++a) part[((wave * FB + b) * FA + a) * 64] = acc[b][a];
+    __syncthreads();
+    sums = part;
+  }
+  const acc_t* sums;
+
+  // every wave adds up and hands out its share of the 16 x 16 blocks
+  template <class F> __device__ __forceinline__ void each(F&& f) const {
+    const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+    for (int i = threadIdx.x >> 6; i < FA * FB; i += NW) {
+      acc_t v = sums[i * 64];
+#pragma unroll
+      for (int w = 1; w < NW; ++w) v += sums[(w * FA * FB + i) * 64];
+      const int a = i % FA, b = i / FA;
+      if (sizeof(T) == 8) f(a * 16 + r, b * 16 + q, 4, v);
+      else f(a * 16 + r, b * 16 + q * 4, 1, v);
+    }
+  }
+};
+
 // whether an operand's offsets inside a stage fit 32 bits: up to `rows` rows of it along k, a stage's rows of k otherwise
 inline bool pipe_fits(int64_t ld, int size, bool along_k, int rows) {
   return (along_k ? rows : 128 / size) * ld * size < (int64_t)1 << 32;
