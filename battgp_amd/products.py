@@ -10,8 +10,6 @@ no function records an autograd graph, and inputs that ask for one are refused.
 
 from __future__ import annotations
 
-import ctypes as C
-
 import torch
 
 from . import _lib
@@ -22,7 +20,7 @@ INT8_MAX_K = _lib.INT8_MAX_K
 MAX_GROUPS = _lib.MAX_GROUPS
 
 
-DEVICE_TYPE = "cuda"  # torch's name of the only device there is a kernel for
+FIRST_DEVICE = 0  # torch's index of the first device there is a kernel for; the CPU's is below it
 
 
 def _check(rc: int) -> None:
@@ -30,49 +28,53 @@ def _check(rc: int) -> None:
         raise EngineError(_lib.load_products().bgp_products_last_error().decode())
 
 
-def _gpu_tensor(name: str, t, dim: int, like: torch.Tensor | None = None) -> torch.Tensor:
+def _gpu_tensor(name: str, t, dim: int, device: int | None = None) -> int:
+    """the index of the device that ``t`` is on (checks are written for the call that passes: they cost a call its time)"""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} is not a torch tensor")
-    if t.layout != torch.strided:
+    if t.layout is not torch.strided:
         raise ValueError(f"{name} is not a dense tensor")
     if t.dim() != dim:
         raise ValueError(f"{name} has {t.dim()} dimensions, {dim} are wanted")
-    if t.device.type != DEVICE_TYPE:
-        raise EngineError(f"{name} is on {t.device}: battgp_amd runs on MI355X only")
-    if like is not None and t.device != like.device:
-        raise ValueError(f"{name} is on {t.device}, the other operands are on {like.device}")
+    at = t.get_device()
+    if at != device:
+        if at < FIRST_DEVICE:
+            raise EngineError(f"{name} is on {t.device}: battgp_amd runs on MI355X only")
+        if device is not None:
+            raise ValueError(f"{name} is on {t.device}, the other operands are on device {device}")
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} requires a gradient: battgp_amd.products records no autograd graph; detach it and call the gradient's function")
-    return t
+    return at
 
 
 def _float_type(name: str, dtype) -> int:
-    if dtype not in DTYPES:
+    code = DTYPES.get(dtype)
+    if code is None:
         raise ValueError(f"{name}: {dtype} is not one of float64, float32, bfloat16, float16")
-    return DTYPES[dtype]
+    return code
 
 
-def _rows(name: str, t: torch.Tensor) -> int:
-    """Leading dimension of a matrix whose rows are contiguous (a dimension of one element has no stride of its own)."""
-    m, n = t.shape
-    if n > 1 and t.stride(1) != 1:
+def _rows(name: str, t: torch.Tensor, m: int, n: int) -> int:
+    """Leading dimension of t[m, n], whose rows are contiguous (a dimension of one element has no stride of its own)."""
+    ld, inner = t.stride()
+    if inner != 1 and n > 1:
         raise ValueError(f"{name}: the elements of a row have to be contiguous, strides are {t.stride()}")
     if m <= 1:
-        return max(n, 1)
-    ld = t.stride(0)
+        return n or 1
     if ld < n:
         raise ValueError(f"{name}: rows overlap, strides are {t.stride()}")
-    return max(ld, 1)
+    return ld or 1
 
 
-def _weights(w: torch.Tensor) -> tuple[int, int, int]:
-    """(stride of a group, leading dimension, 1 if the output axis is the contiguous one) of w[G, N, K]."""
-    g, n, k = w.shape
-    sg = w.stride(0) if g > 1 else 0
-    if (k <= 1 or w.stride(2) == 1) and (n <= 1 or w.stride(1) >= max(k, 1)):
-        return sg, (w.stride(1) if n > 1 else max(k, 1)), 0
-    if (n <= 1 or w.stride(1) == 1) and (k <= 1 or w.stride(2) >= max(n, 1)):
-        return sg, (w.stride(2) if k > 1 else max(n, 1)), 1
+def _weights(w: torch.Tensor, g: int, n: int, k: int) -> tuple[int, int, int]:
+    """(stride of a group, leading dimension, 1 if the output axis is the contiguous one) of w[g, n, k]."""
+    sg, sn, sk = w.stride()
+    if g <= 1:
+        sg = 0
+    if (sk == 1 or k <= 1) and (sn >= (k or 1) or n <= 1):
+        return sg, (sn if n > 1 else k or 1), 0
+    if (sn == 1 or n <= 1) and (sk >= (n or 1) or k <= 1):
+        return sg, (sk if k > 1 else n or 1), 1
     raise ValueError(f"w: either axis of a group's weights has to be contiguous, strides are {w.stride()}")
 
 
@@ -83,12 +85,9 @@ def _span(t: torch.Tensor) -> tuple[int, int]:
     return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
 
 
-def _output(out, name: str, shape, dtype, device, inputs) -> torch.Tensor:
-    if out is None:
-        return torch.empty(shape, dtype=dtype, device=device)
-    _gpu_tensor(name, out, len(shape))
-    if out.device != device or out.dtype != dtype or tuple(out.shape) != tuple(shape):
-        raise ValueError(f"{name}: {tuple(shape)} of {dtype} on {device} is wanted, got {tuple(out.shape)} of {out.dtype} on {out.device}")
+def _output(out, name: str, shape, dtype, device: int, inputs) -> torch.Tensor:
+    if _gpu_tensor(name, out, len(shape)) != device or out.dtype is not dtype or tuple(out.shape) != shape:
+        raise ValueError(f"{name}: {shape} of {dtype} on device {device} is wanted, got {tuple(out.shape)} of {out.dtype} on {out.device}")
     lo, hi = _span(out)
     for t in inputs:
         a, b = _span(t)
@@ -97,33 +96,33 @@ def _output(out, name: str, shape, dtype, device, inputs) -> torch.Tensor:
     return out
 
 
-def _stream(device) -> C.c_void_p:
-    return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+def _stream(device: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(device)  # current_stream(device).cuda_stream, without the objects around it
 
 
-def _offsets(offsets, groups: int, like: torch.Tensor) -> torch.Tensor:
-    _gpu_tensor("offsets", offsets, 1, like)
-    if offsets.dtype != torch.int64:
+def _offsets(offsets, groups: int, device: int) -> None:
+    _gpu_tensor("offsets", offsets, 1, device)
+    if offsets.dtype is not torch.int64:
         raise ValueError(f"offsets are {offsets.dtype}, int64 is wanted")
     if offsets.shape[0] != groups + 1:
         raise ValueError(f"{offsets.shape[0]} offsets for {groups} groups, {groups + 1} are wanted")
     if groups > MAX_GROUPS:
         raise ValueError(f"{groups} groups, at most {MAX_GROUPS} are possible")
-    if offsets.stride(0) != 1:
+    if groups and offsets.stride(0) != 1:
         raise ValueError("offsets are not contiguous")
-    return offsets
 
 
-def _grouped(x, w, offsets, out, name):
+def _grouped(device, dtype, x, w, offsets, out, t, n, k, g):
     """out[t, :] = x[t, :] w_g^T; w may be any view of [G, N, K] that _weights takes"""
-    t, k = x.shape
-    g, n, _ = w.shape
-    ldx = _rows("x", x)
-    sw, ldw, trans = _weights(w)
-    y = _output(out, name, (t, n), x.dtype, x.device, (x, w, offsets))
+    sw, ldw, trans = _weights(w, g, n, k)
+    ldx = _rows("x", x, t, k)
+    if out is None:
+        y, ldy = x.new_empty((t, n)), n or 1
+    else:
+        y = _output(out, "out", (t, n), x.dtype, device, (x, w, offsets))
+        ldy = _rows("out", y, t, n)
     _check(_lib.load_products().bgp_grouped_gemm(
-        x.device.index, _stream(x.device), DTYPES[x.dtype], t, n, k, g, x.data_ptr(), ldx, w.data_ptr(), sw, ldw, trans, offsets.data_ptr(),
-        y.data_ptr(), _rows(name, y), int(out is None),
+        device, _stream(device), dtype, t, n, k, g, x.data_ptr(), ldx, w.data_ptr(), sw, ldw, trans, offsets.data_ptr(), y.data_ptr(), ldy, out is None,
     ))
     return y
 
@@ -136,46 +135,48 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, out:
     [G + 1]`` int64 on the device, ascending, within ``[0, T]`` - they are never read on the host.  Groups may be empty.
     Rows in no group are 0 in a new output and left as they are in a given ``out``.  Sums are held in fp32 (fp64 for
     fp64) and rounded once."""
-    _gpu_tensor("x", x, 2)
-    _gpu_tensor("w", w, 3, x)
-    _float_type("x", x.dtype)
-    if w.dtype != x.dtype:
+    device = _gpu_tensor("x", x, 2)
+    _gpu_tensor("w", w, 3, device)
+    dtype = _float_type("x", x.dtype)
+    if w.dtype is not x.dtype:
         raise ValueError(f"x is {x.dtype}, w is {w.dtype}")
-    if w.shape[2] != x.shape[1]:
-        raise ValueError(f"x has {x.shape[1]} columns, w has {w.shape[2]}")
-    _offsets(offsets, w.shape[0], x)
-    return _grouped(x, w, offsets, out, "out")
+    t, k = x.shape
+    g, n, wk = w.shape
+    if wk != k:
+        raise ValueError(f"x has {k} columns, w has {wk}")
+    _offsets(offsets, g, device)
+    return _grouped(device, dtype, x, w, offsets, out, t, n, k, g)
 
 
 def grouped_matmul_grad(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, need_dx: bool = True, need_dw: bool = True):
     """Gradients of :func:`grouped_matmul` for ``dy [T, N]``: ``(dx [T, K], dw [G, N, K])``, ``None`` for one that is not
     needed.  ``dx`` is 0 in rows of no group, ``dw`` is 0 for an empty group; both are new and contiguous, and for shared
     weights (``expand``) ``dw`` still holds each group's own share."""
-    _gpu_tensor("x", x, 2)
-    _gpu_tensor("dy", dy, 2, x)
-    _gpu_tensor("w", w, 3, x)
-    _float_type("x", x.dtype)
-    if w.dtype != x.dtype or dy.dtype != x.dtype:
+    device = _gpu_tensor("x", x, 2)
+    _gpu_tensor("dy", dy, 2, device)
+    _gpu_tensor("w", w, 3, device)
+    dtype = _float_type("x", x.dtype)
+    if w.dtype is not x.dtype or dy.dtype is not x.dtype:
         raise ValueError(f"x is {x.dtype}, w is {w.dtype}, dy is {dy.dtype}")
     t, k = x.shape
-    g, n, _ = w.shape
-    if w.shape[2] != k or tuple(dy.shape) != (t, n):
+    g, n, wk = w.shape
+    if wk != k or tuple(dy.shape) != (t, n):
         raise ValueError(f"dy {tuple(dy.shape)}, x {tuple(x.shape)} and w {tuple(w.shape)} do not belong together")
-    _offsets(offsets, g, x)
+    _offsets(offsets, g, device)
+    lddy, ldx = _rows("dy", dy, t, n), _rows("x", x, t, k)
     dx = dw = None
     if need_dx:
-        dx = _grouped(dy, w.transpose(1, 2), offsets, None, "dx")
+        dx = _grouped(device, dtype, dy, w.transpose(1, 2), offsets, None, t, k, n, g)
     if need_dw:
-        dw = torch.empty((g, n, k), dtype=x.dtype, device=x.device)
+        dw = x.new_empty((g, n, k))
         _check(_lib.load_products().bgp_grouped_gemm_dw(
-            x.device.index, _stream(x.device), DTYPES[x.dtype], t, n, k, g, dy.data_ptr(), _rows("dy", dy), x.data_ptr(), _rows("x", x),
-            offsets.data_ptr(), dw.data_ptr(), n * max(k, 1), max(k, 1),
+            device, _stream(device), dtype, t, n, k, g, dy.data_ptr(), lddy, x.data_ptr(), ldx, offsets.data_ptr(), dw.data_ptr(), n * (k or 1), k or 1,
         ))
     return dx, dw
 
 
 def _scale_type(dtype):
-    return torch.float64 if dtype == torch.float64 else torch.float32
+    return torch.float64 if dtype is torch.float64 else torch.float32
 
 
 def quantize_rows(x: torch.Tensor, pow2: bool = False, residual: bool = False):
@@ -185,15 +186,16 @@ def quantize_rows(x: torch.Tensor, pow2: bool = False, residual: bool = False):
     ``max |row| <= 127 p``; at least the smallest normal number.  ``q`` is rounded to the nearest, ties to even.
     ``rest = x - scale * q``, exact with ``pow2``: quantising it again gives the next slice of the row.  A row with an
     infinity or a NaN has that for its scale, and codes 0."""
-    _gpu_tensor("x", x, 2)
-    code = _float_type("x", x.dtype)
+    device = _gpu_tensor("x", x, 2)
+    dtype = _float_type("x", x.dtype)
     m, k = x.shape
-    q = torch.empty((m, k), dtype=torch.int8, device=x.device)
-    scale = torch.empty(m, dtype=_scale_type(x.dtype), device=x.device)
-    rest = torch.empty((m, k), dtype=x.dtype, device=x.device) if residual else None
+    ldx = _rows("x", x, m, k)
+    q = x.new_empty((m, k), dtype=torch.int8)
+    scale = x.new_empty(m, dtype=_scale_type(x.dtype))
+    rest = x.new_empty((m, k)) if residual else None
     _check(_lib.load_products().bgp_quantize_rows(
-        x.device.index, _stream(x.device), code, m, k, x.data_ptr(), _rows("x", x), q.data_ptr(), max(k, 1), scale.data_ptr(), int(pow2),
-        rest.data_ptr() if residual else None, max(k, 1),
+        device, _stream(device), dtype, m, k, x.data_ptr(), ldx, q.data_ptr(), k or 1, scale.data_ptr(), bool(pow2), rest.data_ptr() if residual else None,
+        k or 1,
     ))
     return (q, scale, rest) if residual else (q, scale)
 
@@ -207,31 +209,37 @@ def int8_matmul(
     ``a [M, K]`` and ``b [N, K]`` int8 with contiguous rows, ``K <= 131071`` (the sum is exact in 32 bits);
     scales fp64 for a fp64 result, else fp32; ``c`` and ``out`` of the result's type, ``out`` may be ``c`` itself.  The
     scaling and the sum with ``c`` are computed in fp64 and rounded once."""
-    _gpu_tensor("a", a, 2)
-    _gpu_tensor("b", b, 2, a)
+    device = _gpu_tensor("a", a, 2)
+    _gpu_tensor("b", b, 2, device)
     code = _float_type("dtype", dtype)
-    if a.dtype != torch.int8 or b.dtype != torch.int8:
+    if a.dtype is not torch.int8 or b.dtype is not torch.int8:
         raise ValueError(f"a is {a.dtype}, b is {b.dtype}: int8 is wanted")
     m, k = a.shape
-    n = b.shape[0]
-    if b.shape[1] != k:
-        raise ValueError(f"a has {k} columns, b has {b.shape[1]}")
+    n, bk = b.shape
+    if bk != k:
+        raise ValueError(f"a has {k} columns, b has {bk}")
     if k > INT8_MAX_K:
         raise ValueError(f"{k} columns: a sum over more than {INT8_MAX_K} can pass 32 bits")
     for name, s, rows in (("a_scale", a_scale, m), ("b_scale", b_scale, n)):
-        _gpu_tensor(name, s, 1, a)
-        if s.dtype != _scale_type(dtype) or s.shape[0] != rows or (rows > 1 and s.stride(0) != 1):
+        _gpu_tensor(name, s, 1, device)
+        if s.dtype is not _scale_type(dtype) or s.shape[0] != rows or (rows > 1 and s.stride(0) != 1):
             raise ValueError(f"{name}: {rows} contiguous values of {_scale_type(dtype)} are wanted for a result in {dtype}")
+    cp, ldc = None, 0
     if c is not None:
-        _gpu_tensor("c", c, 2, a)
-        if c.dtype != dtype or tuple(c.shape) != (m, n):
+        _gpu_tensor("c", c, 2, device)
+        if c.dtype is not dtype or tuple(c.shape) != (m, n):
             raise ValueError(f"c: {(m, n)} of {dtype} is wanted, got {tuple(c.shape)} of {c.dtype}")
-    inputs = [a, b, a_scale, b_scale]
-    if c is not None and not (out is not None and out.data_ptr() == c.data_ptr() and out.stride() == c.stride()):
-        inputs.append(c)
-    y = _output(out, "out", (m, n), dtype, a.device, inputs)
+        cp, ldc = c.data_ptr(), _rows("c", c, m, n)
+    lda, ldb = _rows("a", a, m, k), _rows("b", b, n, k)
+    if out is None:
+        y, ldy = a.new_empty((m, n), dtype=dtype), n or 1
+    else:
+        inputs = [a, b, a_scale, b_scale]
+        if c is not None and not (out.data_ptr() == cp and out.stride() == c.stride()):
+            inputs.append(c)
+        y = _output(out, "out", (m, n), dtype, device, inputs)
+        ldy = _rows("out", y, m, n)
     _check(_lib.load_products().bgp_int8_gemm(
-        a.device.index, _stream(a.device), code, m, n, k, a.data_ptr(), _rows("a", a), b.data_ptr(), _rows("b", b), a_scale.data_ptr(),
-        b_scale.data_ptr(), c.data_ptr() if c is not None else None, _rows("c", c) if c is not None else 0, y.data_ptr(), _rows("out", y),
+        device, _stream(device), code, m, n, k, a.data_ptr(), lda, b.data_ptr(), ldb, a_scale.data_ptr(), b_scale.data_ptr(), cp, ldc, y.data_ptr(), ldy,
     ))
     return y

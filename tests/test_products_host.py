@@ -114,7 +114,7 @@ class Recorder:
 @pytest.fixture
 def recorder(monkeypatch):
     rec = Recorder()
-    monkeypatch.setattr(products, "DEVICE_TYPE", "cpu")
+    monkeypatch.setattr(products, "FIRST_DEVICE", -1)
     monkeypatch.setattr(products, "_stream", lambda device: None)
     monkeypatch.setattr(_lib, "load_products", lambda: rec)
     return rec
