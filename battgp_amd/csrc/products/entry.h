@@ -41,3 +41,8 @@ enum Cut { DIRECT16, DIRECT32, PLAIN64, PLAIN128, PIPE64, PIPE128, PIPE256 };
 constexpr int tile_of(int cut) {
   return cut == DIRECT16 ? 16 : cut == DIRECT32 ? 32 : cut == PLAIN64 || cut == PIPE64 ? 64 : cut == PIPE256 ? 256 : 128;
 }
+
+// Waves of a pipelined tile: 2 x 4 of 128 x 64 on 256 x 256; 2 x 2 below, but 2 x 4 of 64 x 32 for fp64 on 128 x 128, whose
+// accumulators take twice the registers.
+constexpr int pipe_waves_w(int tile, int size) { return tile == 256 || (size == 8 && tile == 128) ? 4 : 2; }
+constexpr int pipe_threads(int tile, int size) { return 128 * pipe_waves_w(tile, size); }

@@ -114,9 +114,9 @@ template <class T, int BM, int BN, bool WK> __global__ __launch_bounds__(256, 2)
   rows_tile<T, P, BM, BN, WK>(p, lds);
 }
 
-// operands in whole chunks, pipelined: 256 x 256 by 8 waves (one workgroup per CU), smaller ones by 4 (two and more)
-template <class T, int BM, int BN, bool WK> __global__ __launch_bounds__(BM == 256 ? 512 : 256, 2) void grouped_rows_pipe_kernel(GroupedArgs p) {
-  using P = PipeTile<T, BM, BN, 2, BM == 256 ? 4 : 2, true, WK>;
+// operands in whole chunks, pipelined
+template <class T, int BM, int BN, bool WK> __global__ __launch_bounds__(pipe_threads(BM, sizeof(T)), 2) void grouped_rows_pipe_kernel(GroupedArgs p) {
+  using P = PipeTile<T, BM, BN, 2, pipe_waves_w(BM, sizeof(T)), true, WK>;
   __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
   rows_tile<T, P, BM, BN, WK>(p, lds);
 }
@@ -154,8 +154,8 @@ template <class T, int BM, int BN> __global__ __launch_bounds__(256, 2) void gro
   dw_tile<T, P, BM, BN>(p, lds);
 }
 
-template <class T, int BM, int BN> __global__ __launch_bounds__(BM == 256 ? 512 : 256, 2) void grouped_dw_pipe_kernel(GroupedArgs p) {
-  using P = PipeTile<T, BM, BN, 2, BM == 256 ? 4 : 2, false, false>;
+template <class T, int BM, int BN> __global__ __launch_bounds__(pipe_threads(BM, sizeof(T)), 2) void grouped_dw_pipe_kernel(GroupedArgs p) {
+  using P = PipeTile<T, BM, BN, 2, pipe_waves_w(BM, sizeof(T)), false, false>;
   __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
   dw_tile<T, P, BM, BN>(p, lds);
 }
@@ -209,7 +209,7 @@ template <class T, bool WK, int CUT> int run_rows(const GroupedArgs& p0, hipStre
   const dim3 grid((unsigned)tiles);
   if constexpr (CUT <= DIRECT32) return launch(what, grouped_rows_direct_kernel<T, B / 16, WK>, grid, dim3(256), st, p);
   else if constexpr (CUT <= PLAIN128) return launch(what, grouped_rows_kernel<T, B, B, WK>, grid, dim3(256), st, p);
-  else return launch(what, grouped_rows_pipe_kernel<T, B, B, WK>, grid, dim3(B == 256 ? 512 : 256), st, p);
+  else return launch(what, grouped_rows_pipe_kernel<T, B, B, WK>, grid, dim3(pipe_threads(B, sizeof(T))), st, p);
 }
 
 template <class T, bool WK> int rows_by_tile(const GroupedArgs& p, bool vec, hipStream_t st) {
@@ -241,7 +241,7 @@ template <class T, int CUT> int run_dw(const GroupedArgs& p0, hipStream_t st) {
   const dim3 grid((unsigned)tiles);
   if constexpr (CUT <= DIRECT32) return launch(what, grouped_dw_direct_kernel<T, B / 16>, grid, dim3(256), st, p);
   else if constexpr (CUT <= PLAIN128) return launch(what, grouped_dw_kernel<T, B, B>, grid, dim3(256), st, p);
-  else return launch(what, grouped_dw_pipe_kernel<T, B, B>, grid, dim3(B == 256 ? 512 : 256), st, p);
+  else return launch(what, grouped_dw_pipe_kernel<T, B, B>, grid, dim3(pipe_threads(B, sizeof(T))), st, p);
 }
 
 template <class T> int dw_by_type(const GroupedArgs& p, bool vec, hipStream_t st) {

@@ -237,6 +237,22 @@ struct Int8Args {
   int tiles_n;
 };
 
+// 4 neighbours of a row, at the alignment of one
+template <class T> struct __attribute__((packed, aligned(sizeof(T)))) Four { T e[4]; };
+
+template <class T, bool ADD> __device__ __forceinline__ void int8_out(const v4i& v, typename ScaleOf<T>::type sa, const typename ScaleOf<T>::type* sb, const T* c, T* y) {
+  using S = typename ScaleOf<T>::type;
+  const Four<S> s = *reinterpret_cast<const Four<S>*>(sb);
+  Four<T> add, o;
+  if (ADD) add = *reinterpret_cast<const Four<T>*>(c);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const double r = (double)v[e] * ((double)sa * (double)s.e[e]);
+    o.e[e] = narrow<T>(ADD ? r + widen(add.e[e]) : r);
+  }
+  *reinterpret_cast<Four<T>*>(y) = o;
+}
+
 // Y[i, j] = (C[i, j] +) sa[i] sb[j] sum_k A[i, k] B[j, k]: the sum exact in 32 bits, the rest in 64, one rounding
 template <class T, class P, int BM, int BN> __device__ __forceinline__ void int8_tile(const Int8Args& p, char* lds) {
   using S = typename ScaleOf<T>::type;
@@ -250,21 +266,26 @@ template <class T, class P, int BM, int BN> __device__ __forceinline__ void int8
   const int64_t m0 = (strip * DEEP + in % deep) * BM, n0 = (int64_t)(in / deep) * BN;
   P tile;
   tile.run(Operand<int8_t>{p.a + m0 * p.lda, p.lda, p.M - m0}, Operand<int8_t>{p.b + n0 * p.ldb, p.ldb, p.N - n0}, p.K, lds);
-  tile.each([&](int i, int j, int step, const v4i& v) {
-    const int64_t row = m0 + i;
-    if (row >= p.M) return;
-    const double si = (double)static_cast<const S*>(p.sa)[row];
-    T* y = static_cast<T*>(p.y) + row * p.ldy;
-    const T* c = p.c ? static_cast<const T*>(p.c) + row * p.ldc : nullptr;
+  const S *sa = static_cast<const S*>(p.sa) + m0, *sb = static_cast<const S*>(p.sb) + n0;
+  T* y = static_cast<T*>(p.y) + m0 * p.ldy + n0;
+  const T* c = p.c ? static_cast<const T*>(p.c) + m0 * p.ldc + n0 : nullptr;
+  const int64_t rows = p.M - m0, cols = p.N - n0;
+  if (rows >= BM && cols >= BN && !c) {  // whole tiles without a branch per element, so that loads and stores run ahead
+    tile.each([&](int i, int j, int, const v4i& v) { int8_out<T, false>(v, sa[i], sb + j, nullptr, y + i * p.ldy + j); });
+  } else if (rows >= BM && cols >= BN) {
+    tile.each([&](int i, int j, int, const v4i& v) { int8_out<T, true>(v, sa[i], sb + j, c + i * p.ldc + j, y + i * p.ldy + j); });
+  } else {
+    tile.each([&](int i, int j, int, const v4i& v) {
+      if (i >= rows) return;
+      const double si = (double)sa[i];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int64_t col = n0 + j + e * step;
-      if (col >= p.N) break;
-      double r = (double)v[e] * (si * (double)static_cast<const S*>(p.sb)[col]);
-      if (c) r += widen(c[col]);
-      y[col] = narrow<T>(r);
-    }
-  });
+      for (int e = 0; e < 4; ++e)
+        if (j + e < cols) {
+          const double r = (double)v[e] * (si * (double)sb[j + e]);
+          y[i * p.ldy + j + e] = narrow<T>(c ? r + widen(c[i * p.ldc + j + e]) : r);
+        }
+    });
+  }
 }
 
 // any operands, through registers
@@ -275,8 +296,8 @@ template <class T, int BM, int BN> __global__ __launch_bounds__(256, 2) void int
 }
 
 // operands in whole chunks, pipelined
-template <class T, int BM, int BN> __global__ __launch_bounds__(BM == 256 ? 512 : 256, 2) void int8_gemm_pipe_kernel(Int8Args p) {
-  using P = PipeTile<int8_t, BM, BN, 2, BM == 256 ? 4 : 2, true, true>;
+template <class T, int BM, int BN> __global__ __launch_bounds__(pipe_threads(BM, 1), 2) void int8_gemm_pipe_kernel(Int8Args p) {
+  using P = PipeTile<int8_t, BM, BN, 2, pipe_waves_w(BM, 1), true, true>;
   __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
   int8_tile<T, P, BM, BN>(p, lds);
 }
@@ -298,7 +319,7 @@ template <class T, int CUT> int run_int8(const Int8Args& p0, hipStream_t st) {
   const dim3 grid((unsigned)tiles);
   if constexpr (CUT <= DIRECT32) return launch(what, int8_gemm_direct_kernel<T, B / 16>, grid, dim3(256), st, p);
   else if constexpr (CUT <= PLAIN128) return launch(what, int8_gemm_kernel<T, B, B>, grid, dim3(256), st, p);
-  else return launch(what, int8_gemm_pipe_kernel<T, B, B>, grid, dim3(B == 256 ? 512 : 256), st, p);
+  else return launch(what, int8_gemm_pipe_kernel<T, B, B>, grid, dim3(pipe_threads(B, 1)), st, p);
 }
 
 int pick_int8(bool vec, int64_t M, int64_t N, int64_t K) {

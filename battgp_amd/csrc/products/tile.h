@@ -148,15 +148,19 @@ template <class T, int ROWS, bool ALONG_K, bool VEC, int NT> struct Stage {
   uint4 r[NL];
 
   __device__ __forceinline__ void fetch(const Operand<T>& o, int64_t k0, int64_t klen) {
+    if (k0 + KSTAGE<T> <= klen && o.rows >= ROWS) fetch_part<true>(o, k0, klen);  // without a branch per chunk
+    else fetch_part<false>(o, k0, klen);
+  }
+  template <bool WHOLE> __device__ __forceinline__ void fetch_part(const Operand<T>& o, int64_t k0, int64_t klen) {
 #pragma unroll
     for (int l = 0; l < NL; ++l) {
       const int i = threadIdx.x + l * NT, row = i / CPR, c = swizzle<T, ALONG_K>(row, i % CPR, CPR);
       if (ALONG_K) {
         const int64_t k = k0 + c * CHE<T>;
-        r[l] = load_chunk<T, VEC>(o.p + row * o.ld + k, row < o.rows ? klen - k : 0);
+        r[l] = load_chunk<T, VEC>(o.p + row * o.ld + k, WHOLE ? CHE<T> : row < o.rows ? klen - k : 0);
       } else {
         const int64_t k = k0 + row;
-        r[l] = load_chunk<T, VEC>(o.p + k * o.ld + c * CHE<T>, k < klen ? o.rows - c * CHE<T> : 0);
+        r[l] = load_chunk<T, VEC>(o.p + k * o.ld + c * CHE<T>, WHOLE ? CHE<T> : k < klen ? o.rows - c * CHE<T> : 0);
       }
     }
   }
