@@ -128,23 +128,23 @@ INT8_MAX_K = 131071
 PRODUCTS_SIGNATURES = {
     "bgp_products_last_error": (C.c_char_p, []),
     "bgp_grouped_gemm": (
-        C.c_int,
+        C.c_int64,
         [C.c_int, C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_int64, C.c_int,
-         C.c_void_p, C.c_void_p, C.c_int64, C.c_int],
+         C.c_void_p, C.c_void_p, C.c_int64, C.c_int, C.c_void_p, C.c_int64],
     ),
     "bgp_grouped_gemm_dw": (
-        C.c_int,
+        C.c_int64,
         [C.c_int, C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p,
-         C.c_int64, C.c_int64],
+         C.c_int64, C.c_int64, C.c_void_p, C.c_int64],
     ),
     "bgp_quantize_rows": (
         C.c_int,
         [C.c_int, C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int, C.c_void_p, C.c_int64],
     ),
     "bgp_int8_gemm": (
-        C.c_int,
+        C.c_int64,
         [C.c_int, C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p,
-         C.c_int64, C.c_void_p, C.c_int64],
+         C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64],
     ),
 }
 

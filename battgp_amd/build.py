@@ -27,7 +27,7 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-u
 PRODUCTS = os.path.join(CSRC, "products")
 LIB_PRODUCTS = os.path.join(HERE, "libbattgp_products.so")
 PRODUCTS_SOURCES = ["grouped.hip", "int8.hip"]
-PRODUCTS_HEADERS = [os.path.join(PRODUCTS, h) for h in ("tile.h", "entry.h")] + [os.path.join(os.path.dirname(HERE), "include", "battgp_products.h")]
+PRODUCTS_HEADERS = [os.path.join(PRODUCTS, h) for h in ("tile.h", "entry.h", "plan.h")] + [os.path.join(os.path.dirname(HERE), "include", "battgp_products.h")]
 # no packed fp32 arithmetic: some of its forms have given wrong results on gfx950
 PRODUCTS_FLAGS = FLAGS + ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 

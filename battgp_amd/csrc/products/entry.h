@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 
 #include "../../../include/battgp_products.h"
+#include "plan.h"
 
 // workgroups of 256 threads in one launch: the threads of a launch are counted in 32 bits
 constexpr int64_t MAX_WORKGROUPS = (1 << 24) - 1;
@@ -35,14 +36,34 @@ template <class... A> int launch(const char* what, void (*kernel)(A...), dim3 gr
   return e == hipSuccess ? 0 : bgp_products_fail(-2, "%s: launch failed: %s", what, hipGetErrorString(e));
 }
 
-// How a product is cut: straight from memory in tiles of 16 or 32, through registers (any operands) or pipelined (whole
-// chunks) in tiles of 64, 128 or 256.
-enum Cut { DIRECT16, DIRECT32, PLAIN64, PLAIN128, PIPE64, PIPE128, PIPE256 };
-constexpr int tile_of(int cut) {
-  return cut == DIRECT16 ? 16 : cut == DIRECT32 ? 32 : cut == PLAIN64 || cut == PIPE64 ? 64 : cut == PIPE256 ? 256 : 128;
-}
-
 // Waves of a pipelined tile: 2 x 4 of 128 x 64 on 256 x 256; 2 x 2 below, but 2 x 4 of 64 x 32 for fp64 on 128 x 128, whose
 // accumulators take twice the registers.
 constexpr int pipe_waves_w(int tile, int size) { return tile == 256 || (size == 8 && tile == 128) ? 4 : 2; }
 constexpr int pipe_threads(int tile, int size) { return 128 * pipe_waves_w(tile, size); }
+
+// ---- what a call lays out in the caller's workspace ----
+
+// rows of `extent` elements, `per` of them to a batch, copied to rows of ld_to elements (16-byte aligned) back to back
+struct PackJob {
+  const void* from;
+  void* to;
+  int64_t rows, per, stride, ld, extent, ld_to;
+};
+// at most two operands in one launch
+int launch_pack(const char* what, int size, const PackJob* jobs, int count, hipStream_t st);
+constexpr int64_t padded_row(int64_t extent, int size) { return (extent * size + 127) / 128 * 128 / size; }
+
+// Takes pieces of the workspace, or only adds up what they come to.
+class Workspace {
+  char* at_;
+  int64_t used_ = 0;
+
+ public:
+  explicit Workspace(void* at) : at_(static_cast<char*>(at)) {}
+  void* take(int64_t bytes) {
+    void* p = at_ ? at_ + used_ : nullptr;
+    used_ += (bytes + 255) / 256 * 256;
+    return p;
+  }
+  int64_t used() const { return used_; }
+};

@@ -29,7 +29,18 @@ struct GroupedArgs {
   const int64_t* off;
   int64_t T, N, K, ldx, ldw, sw, ldy;
   int G, rest, tiles_n;
+  int split;   // k is cut in this many parts,
+  void* part;  // whose sums go here: [split][rows of D][columns of D], fp32 (fp64)
 };
+
+// one part of k: from `from` on, `length` long
+struct Part {
+  int64_t from, length;
+};
+__device__ __forceinline__ Part part_of(int64_t k, int stage, int split, int i) {
+  const int64_t stages = (k + stage - 1) / stage, each = (stages + split - 1) / split * stage, from = i * each;
+  return Part{from, from >= k ? 0 : k - from < each ? k - from : each};
+}
 
 struct Bounds {
   int64_t a, b;
@@ -93,18 +104,30 @@ __device__ __forceinline__ RowTile find_row_tile(const GroupedArgs& p, int BM) {
 
 // Y[rows of g, :] = X[rows of g, :] W_g^T;  WK: W_g[n, k] = w[g sw + n ldw + k], else w[g sw + k ldw + n]
 template <class T, class P, int BM, int BN, bool WK> __device__ __forceinline__ void rows_tile(const GroupedArgs& p, char* lds) {
+  using A = typename Sum<T>::type;
   const RowTile t = find_row_tile(p, BM);
-  if (t.g < 0) return;
+  if (t.g < 0 || (p.split > 1 && t.g >= p.G)) return;
   const int64_t n0 = (int64_t)t.tn * BN;
-  T* y = static_cast<T*>(p.y) + t.row0 * p.ldy + n0;
   P tile;
-  const Operand<T> x{static_cast<const T*>(p.x) + t.row0 * p.ldx, p.ldx, t.rows};
+  Operand<T> x{static_cast<const T*>(p.x) + t.row0 * p.ldx, p.ldx, t.rows};
   Operand<T> w{static_cast<const T*>(p.w), p.ldw, p.N - n0};
   if (t.g < p.G) w.p += t.g * p.sw + (WK ? n0 * p.ldw : n0);
-  tile.run(x, w, t.g < p.G ? p.K : 0, lds);
-  tile.each([&](int i, int j, int step, const typename P::acc_t& v) {
-    if (i < t.rows) store_row(y + i * p.ldy, j, step, v, p.N - n0);
-  });
+  if (p.split == 1) {
+    tile.run(x, w, t.g < p.G ? p.K : 0, lds);
+    T* y = static_cast<T*>(p.y) + t.row0 * p.ldy + n0;
+    tile.each([&](int i, int j, int step, const typename P::acc_t& v) {
+      if (i < t.rows) store_row(y + i * p.ldy, j, step, v, p.N - n0);
+    });
+  } else {
+    const Part k = part_of(p.K, KSTAGE<T>, p.split, blockIdx.y);
+    x.p += k.from;
+    w.p += WK ? k.from : k.from * p.ldw;
+    tile.run(x, w, k.length, lds);
+    A* y = static_cast<A*>(p.part) + (blockIdx.y * p.T + t.row0) * p.N + n0;
+    tile.each([&](int i, int j, int step, const typename P::acc_t& v) {
+      if (i < t.rows) store_row(y + i * p.N, j, step, v, p.N - n0);
+    });
+  }
 }
 
 // any operands, through registers
@@ -130,6 +153,7 @@ template <class T, int F, bool WK> __global__ __launch_bounds__(256) void groupe
 
 // dW_g[n, k] = sum over the rows t of g of dY[t, n] X[t, k]
 template <class T, class P, int BM, int BN> __device__ __forceinline__ void dw_tile(const GroupedArgs& p, char* lds) {
+  using A = typename Sum<T>::type;
   const int tiles_k = (int)((p.K + BN - 1) / BN), tiles = p.tiles_n * tiles_k;
   // each XCD takes whole runs of tiles: they share a group's rows
   constexpr int XCDS = 8;
@@ -139,13 +163,24 @@ template <class T, class P, int BM, int BN> __device__ __forceinline__ void dw_t
   const int64_t n0 = (int64_t)(j / tiles_k) * BM, k0 = (int64_t)(j % tiles_k) * BN;
   const int64_t a = clamp64(p.off[g], 0, p.T), b = clamp64(p.off[g + 1], a, p.T);
   P tile;
-  const Operand<T> dy{static_cast<const T*>(p.y) + a * p.ldy + n0, p.ldy, p.N - n0};
-  const Operand<T> x{static_cast<const T*>(p.x) + a * p.ldx + k0, p.ldx, p.K - k0};
-  tile.run(dy, x, b - a, lds);
-  T* dw = static_cast<T*>(const_cast<void*>(p.w)) + g * p.sw + n0 * p.ldw + k0;
-  tile.each([&](int r, int c, int step, const typename P::acc_t& v) {
-    if (r < p.N - n0) store_row(dw + r * p.ldw, c, step, v, p.K - k0);
-  });
+  Operand<T> dy{static_cast<const T*>(p.y) + a * p.ldy + n0, p.ldy, p.N - n0};
+  Operand<T> x{static_cast<const T*>(p.x) + a * p.ldx + k0, p.ldx, p.K - k0};
+  if (p.split == 1) {
+    tile.run(dy, x, b - a, lds);
+    T* dw = static_cast<T*>(const_cast<void*>(p.w)) + g * p.sw + n0 * p.ldw + k0;
+    tile.each([&](int r, int c, int step, const typename P::acc_t& v) {
+      if (r < p.N - n0) store_row(dw + r * p.ldw, c, step, v, p.K - k0);
+    });
+  } else {
+    const Part t = part_of(b - a, KSTAGE<T>, p.split, blockIdx.y);
+    dy.p += t.from * p.ldy;
+    x.p += t.from * p.ldx;
+    tile.run(dy, x, t.length, lds);
+    A* dw = static_cast<A*>(p.part) + (((int64_t)blockIdx.y * p.G + g) * p.N + n0) * p.K + k0;
+    tile.each([&](int r, int c, int step, const typename P::acc_t& v) {
+      if (r < p.N - n0) store_row(dw + r * p.K, c, step, v, p.K - k0);
+    });
+  }
 }
 
 template <class T, int BM, int BN> __global__ __launch_bounds__(256, 2) void grouped_dw_kernel(GroupedArgs p) {
@@ -166,6 +201,35 @@ template <class T, int F> __global__ __launch_bounds__(256) void grouped_dw_dire
   dw_tile<T, P, 16 * F, 16 * F>(p, lds);
 }
 
+// out[r, c] = the parts' sum, in their order; rows of no group (off != NULL) as bgp_grouped_gemm leaves them
+struct JoinArgs {
+  const void* part;
+  void* out;
+  int64_t rows, cols, per, stride, ld;  // row r of `out` is at (r / per) stride + (r % per) ld
+  int split;
+  const int64_t* off;
+  int G, rest;
+};
+template <class T> __global__ __launch_bounds__(256) void join_kernel(JoinArgs p) {
+  using A = typename Sum<T>::type;
+  const int64_t c = ((int64_t)blockIdx.x * 64 + threadIdx.x) * 4;
+  if (c >= p.cols) return;
+  const A* part = static_cast<const A*>(p.part);
+  for (int64_t r = (int64_t)blockIdx.y * 4 + threadIdx.y; r < p.rows; r += (int64_t)gridDim.y * 4) {
+    A sum[4] = {0, 0, 0, 0};
+    const bool none = p.off && (r < p.off[0] || r >= p.off[p.G]);
+    if (none && !p.rest) continue;
+    if (!none)
+      for (int s = 0; s < p.split; ++s) {
+        const A* q = part + (s * p.rows + r) * p.cols + c;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (c + e < p.cols) sum[e] += q[e];
+      }
+    store_row(static_cast<T*>(p.out) + r / p.per * p.stride + r % p.per * p.ld, c, 1, sum, p.cols);
+  }
+}
+
 int size_of(int dtype) {
   switch (dtype) {
     case BGP_F64: return 8;
@@ -176,26 +240,34 @@ int size_of(int dtype) {
   return 0;
 }
 
-// whole 16-byte chunks: base, leading dimension and contiguous extent are multiples of 16 bytes
-bool chunked(const void* p, int64_t ld, int64_t extent, int size) {
-  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (ld * size) % 16 == 0 && (extent * size) % 16 == 0;
+// rows that start on 16 bytes, and for an operand along rows no chunk that reaches past a row's end
+bool aligned(const void* p, int64_t ld, int64_t stride, int size, bool along_k, int64_t extent) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * size % 16 == 0 && stride * size % 16 == 0 && (along_k || extent * size % 16 == 0) &&
+         pipe_fits(ld, size, along_k, 256);
 }
 
-int pick_rows(int size, bool direct, bool vec, int64_t T, int64_t N, int64_t K, int64_t G) {
-  const int64_t t64 = (T / 64 + G) * ((N + 63) / 64);
-  if (direct && t64 < 256) return T <= 16 * G ? DIRECT16 : DIRECT32;
-  const bool small = T < G * 96;
-  if (!vec) return small ? PLAIN64 : PLAIN128;
-  if (size == 2 && T >= G * 256 && N >= 512) return PIPE256;
-  return small ? PIPE64 : PIPE128;
-}
+// one operand: what it is now, and what it would be in the workspace
+struct Laid {
+  const void* p;
+  int64_t stride, ld, rows, per, extent;
+  bool along_k, ok;
+  Laid(const void* at, int64_t batches, int64_t stride_, int64_t per_, int64_t ld_, int64_t extent_, int size, bool along)
+      : p(at), stride(stride_), ld(ld_), rows(batches * per_), per(per_), extent(extent_), along_k(along), ok(aligned(at, ld_, stride_, size, along, extent_)) {}
+  int64_t bytes(int size) const { return ok ? 0 : rows * padded_row(extent, size) * size; }
+  void move(Workspace& ws, int size, PackJob* jobs, int* count) {
+    if (ok) return;
+    const int64_t to = padded_row(extent, size);
+    void* at = ws.take(rows * to * size);
+    jobs[(*count)++] = PackJob{p, at, rows, per, stride, ld, extent, to};
+    p = at;
+    ld = to;
+    stride = per * to;
+  }
+};
 
-int pick_dw(int size, bool vec, int64_t T, int64_t N, int64_t K, int64_t G) {
-  const int64_t t128 = G * ((N + 127) / 128) * ((K + 127) / 128);
-  if (size >= 4 && t128 < 128) return DIRECT32;
-  if (!vec) return t128 < 256 ? PLAIN64 : PLAIN128;
-  if (size == 2 && G * (N / 256) * (K / 256) >= 256) return PIPE256;
-  return t128 < 256 ? PIPE64 : PIPE128;
+template <class T> int join(const char* what, const JoinArgs& j, hipStream_t st) {
+  const int64_t y = (j.rows + 3) / 4;
+  return launch(what, join_kernel<T>, dim3((unsigned)((j.cols + 255) / 256), (unsigned)(y < 65535 ? y : 65535)), dim3(64, 4), st, j);
 }
 
 template <class T, bool WK, int CUT> int run_rows(const GroupedArgs& p0, hipStream_t st) {
@@ -206,17 +278,14 @@ template <class T, bool WK, int CUT> int run_rows(const GroupedArgs& p0, hipStre
   // row tiles there can be at most: a group adds less than one to its share of the rows
   const int64_t tiles = (p.T / B + p.G + (p.rest ? 2 : 0)) * p.tiles_n + 7;
   if (tiles > MAX_WORKGROUPS / 2) return bgp_products_fail(-1, "%s: %lld tiles are more than one launch holds", what, (long long)tiles);
-  const dim3 grid((unsigned)tiles);
+  const dim3 grid((unsigned)tiles, p.split);
   if constexpr (CUT <= DIRECT32) return launch(what, grouped_rows_direct_kernel<T, B / 16, WK>, grid, dim3(256), st, p);
   else if constexpr (CUT <= PLAIN128) return launch(what, grouped_rows_kernel<T, B, B, WK>, grid, dim3(256), st, p);
   else return launch(what, grouped_rows_pipe_kernel<T, B, B, WK>, grid, dim3(pipe_threads(B, sizeof(T))), st, p);
 }
 
-template <class T, bool WK> int rows_by_tile(const GroupedArgs& p, bool vec, hipStream_t st) {
-  constexpr bool direct = WK || sizeof(T) >= 4;
-  vec = vec && pipe_fits(p.ldx, sizeof(T), true, 256) && pipe_fits(p.ldw, sizeof(T), WK, 256);
-  int cut = pick_rows(sizeof(T), direct, vec, p.T, p.N, p.K, p.G);
-  if constexpr (direct) {
+template <class T, bool WK> int rows_by_cut(const GroupedArgs& p, int cut, hipStream_t st) {
+  if constexpr (WK || sizeof(T) >= 4) {
     if (cut == DIRECT16) return run_rows<T, WK, DIRECT16>(p, st);
     if (cut == DIRECT32) return run_rows<T, WK, DIRECT32>(p, st);
   }
@@ -227,8 +296,10 @@ template <class T, bool WK> int rows_by_tile(const GroupedArgs& p, bool vec, hip
   return cut == PIPE64 ? run_rows<T, WK, PIPE64>(p, st) : run_rows<T, WK, PIPE128>(p, st);
 }
 
-template <class T> int rows_by_type(const GroupedArgs& p, bool trans, bool vec, hipStream_t st) {
-  return trans ? rows_by_tile<T, false>(p, vec, st) : rows_by_tile<T, true>(p, vec, st);
+template <class T> int run_rows_plan(const GroupedArgs& p, bool trans, const Plan& plan, hipStream_t st) {
+  const int rc = trans ? rows_by_cut<T, false>(p, plan.cut, st) : rows_by_cut<T, true>(p, plan.cut, st);
+  if (rc || p.split == 1) return rc;
+  return join<T>("bgp_grouped_gemm", JoinArgs{p.part, p.y, p.T, p.N, p.T, 0, p.ldy, p.split, p.off, p.G, p.rest}, st);
 }
 
 template <class T, int CUT> int run_dw(const GroupedArgs& p0, hipStream_t st) {
@@ -238,15 +309,13 @@ template <class T, int CUT> int run_dw(const GroupedArgs& p0, hipStream_t st) {
   p.tiles_n = (int)((p.N + B - 1) / B);
   const int64_t tiles = (int64_t)p.G * p.tiles_n * ((p.K + B - 1) / B) + 7;
   if (tiles > MAX_WORKGROUPS / 2) return bgp_products_fail(-1, "%s: %lld tiles are more than one launch holds", what, (long long)tiles);
-  const dim3 grid((unsigned)tiles);
+  const dim3 grid((unsigned)tiles, p.split);
   if constexpr (CUT <= DIRECT32) return launch(what, grouped_dw_direct_kernel<T, B / 16>, grid, dim3(256), st, p);
   else if constexpr (CUT <= PLAIN128) return launch(what, grouped_dw_kernel<T, B, B>, grid, dim3(256), st, p);
   else return launch(what, grouped_dw_pipe_kernel<T, B, B>, grid, dim3(pipe_threads(B, sizeof(T))), st, p);
 }
 
-template <class T> int dw_by_type(const GroupedArgs& p, bool vec, hipStream_t st) {
-  vec = vec && pipe_fits(p.ldx, sizeof(T), false, 256) && pipe_fits(p.ldy, sizeof(T), false, 256);
-  const int cut = pick_dw(sizeof(T), vec, p.T, p.N, p.K, p.G);
+template <class T> int dw_by_cut(const GroupedArgs& p, int cut, hipStream_t st) {
   if constexpr (sizeof(T) >= 4) {
     if (cut == DIRECT16) return run_dw<T, DIRECT16>(p, st);
     if (cut == DIRECT32) return run_dw<T, DIRECT32>(p, st);
@@ -256,6 +325,18 @@ template <class T> int dw_by_type(const GroupedArgs& p, bool vec, hipStream_t st
   if constexpr (sizeof(T) == 2)
     if (cut == PIPE256) return run_dw<T, PIPE256>(p, st);
   return cut == PIPE64 ? run_dw<T, PIPE64>(p, st) : run_dw<T, PIPE128>(p, st);
+}
+
+template <class T> int run_dw_plan(const GroupedArgs& p, const Plan& plan, hipStream_t st) {
+  const int rc = dw_by_cut<T>(p, plan.cut, st);
+  if (rc || p.split == 1) return rc;
+  return join<T>("bgp_grouped_gemm_dw", JoinArgs{p.part, const_cast<void*>(p.w), p.G * p.N, p.K, p.N, p.sw, p.ldw, p.split, nullptr, p.G, 0}, st);
+}
+
+// Row tiles of b rows that are expected: every group with rows has one at least and half of one to spare.
+double expected_tiles(int64_t T, int64_t G, int b) {
+  const double used = (double)(G < T ? G : T), even = (double)T / b + 0.5 * used;
+  return even > used ? even : used;
 }
 
 int check_sizes(const char* what, int dtype, int64_t T, int64_t N, int64_t K, int64_t G, const void* off) {
@@ -268,46 +349,79 @@ int check_sizes(const char* what, int dtype, int64_t T, int64_t N, int64_t K, in
 
 }  // namespace
 
-extern "C" int bgp_grouped_gemm(int device, void* stream, int dtype, int64_t T, int64_t N, int64_t K, int64_t G, const void* X, int64_t ldx, const void* W,
-                                int64_t strideW, int64_t ldw, int w_trans, const int64_t* offsets, void* Y, int64_t ldy, int zero_rest) {
+extern "C" int64_t bgp_grouped_gemm(int device, void* stream, int dtype, int64_t T, int64_t N, int64_t K, int64_t G, const void* X, int64_t ldx,
+                                    const void* W, int64_t strideW, int64_t ldw, int w_trans, const int64_t* offsets, void* Y, int64_t ldy, int zero_rest,
+                                    void* workspace, int64_t workspace_bytes) {
   const char* what = "bgp_grouped_gemm";
   if (int rc = check_sizes(what, dtype, T, N, K, G, offsets)) return rc;
   if (T == 0 || N == 0 || (G == 0 && !zero_rest)) return 0;
   if (!Y || (K > 0 && G > 0 && (!X || !W))) return bgp_products_fail(-1, "%s: null pointer", what);
   if (ldx < K || ldy < N || ldw < (w_trans ? N : K) || strideW < 0)
     return bgp_products_fail(-1, "%s: bad strides ldx=%lld ldw=%lld strideW=%lld ldy=%lld", what, (long long)ldx, (long long)ldw, (long long)strideW, (long long)ldy);
+  const int size = size_of(dtype);
+  Laid x(X, 1, 0, T, ldx, K, size, true), w(W, strideW ? G : 1, strideW, w_trans ? K : N, ldw, w_trans ? N : K, size, !w_trans);
+  const Question q{size, !w_trans || size >= 4, x.ok && w.ok, pipe_fits(padded_row(x.extent, size), size, true, 256) && pipe_fits(padded_row(w.extent, size), size, !w_trans, 256),
+                   !w.along_k && !w.ok, (double)K, (double)(x.bytes(size) + w.bytes(size)), (double)T * N, G > 0 ? 16 : 1};
+  const Plan plan = make_plan(q, [&](int b) { return expected_tiles(T, G, b) * ((N + b - 1) / b); });
+  Workspace ws(workspace);
+  PackJob jobs[2];
+  int count = 0;
+  if (plan.pack) {
+    x.move(ws, size, jobs, &count);
+    w.move(ws, size, jobs, &count);
+    if (strideW == 0) w.stride = 0;
+  }
+  void* part = plan.split > 1 ? ws.take(plan.split * T * N * (size == 8 ? 8 : 4)) : nullptr;
+  if (ws.used() > 0 && (!workspace || workspace_bytes < ws.used())) return ws.used();
   DeviceScope scope(device);
   if (int rc = scope.check(what)) return rc;
-  GroupedArgs p{X, W, Y, offsets, T, N, K, ldx, ldw, strideW, ldy, (int)G, zero_rest != 0, 0};
-  const int size = size_of(dtype);
-  const bool vec = chunked(X, ldx, K, size) && chunked(W, ldw, w_trans ? N : K, size) && (strideW * size) % 16 == 0;
   const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (count)
+    if (int rc = launch_pack(what, size, jobs, count, st)) return rc;
+  const GroupedArgs p{x.p, w.p, Y, offsets, T, N, K, x.ld, w.ld, w.stride, ldy, (int)G, zero_rest != 0, 0, plan.split, part};
   switch (dtype) {
-    case BGP_F64: return rows_by_type<double>(p, w_trans, vec, st);
-    case BGP_F32: return rows_by_type<float>(p, w_trans, vec, st);
-    case BGP_BF16: return rows_by_type<bf16_t>(p, w_trans, vec, st);
-    default: return rows_by_type<f16_t>(p, w_trans, vec, st);
+    case BGP_F64: return run_rows_plan<double>(p, w_trans, plan, st);
+    case BGP_F32: return run_rows_plan<float>(p, w_trans, plan, st);
+    case BGP_BF16: return run_rows_plan<bf16_t>(p, w_trans, plan, st);
+    default: return run_rows_plan<f16_t>(p, w_trans, plan, st);
   }
 }
 
-extern "C" int bgp_grouped_gemm_dw(int device, void* stream, int dtype, int64_t T, int64_t N, int64_t K, int64_t G, const void* dY, int64_t lddy,
-                                   const void* X, int64_t ldx, const int64_t* offsets, void* dW, int64_t strideW, int64_t ldw) {
+extern "C" int64_t bgp_grouped_gemm_dw(int device, void* stream, int dtype, int64_t T, int64_t N, int64_t K, int64_t G, const void* dY, int64_t lddy,
+                                       const void* X, int64_t ldx, const int64_t* offsets, void* dW, int64_t strideW, int64_t ldw, void* workspace,
+                                       int64_t workspace_bytes) {
   const char* what = "bgp_grouped_gemm_dw";
   if (int rc = check_sizes(what, dtype, T, N, K, G, offsets)) return rc;
   if (N == 0 || K == 0 || G == 0) return 0;
   if (!dW || (T > 0 && (!dY || !X))) return bgp_products_fail(-1, "%s: null pointer", what);
   if (lddy < N || ldx < K || ldw < K || strideW < N * ldw)
     return bgp_products_fail(-1, "%s: bad strides lddy=%lld ldx=%lld ldw=%lld strideW=%lld", what, (long long)lddy, (long long)ldx, (long long)ldw, (long long)strideW);
+  const int size = size_of(dtype);
+  Laid y(dY, 1, 0, T, lddy, N, size, false), x(X, 1, 0, T, ldx, K, size, false);
+  // a group's rows are its length of k: their mean, and as much again for the longest of uneven ones
+  const double used = (double)(G < T ? G : T > 0 ? T : 1);
+  const Question q{size, size >= 4, x.ok && y.ok, pipe_fits(padded_row(N, size), size, false, 256) && pipe_fits(padded_row(K, size), size, false, 256),
+                   !x.ok || !y.ok, ceil(T / used), (double)(x.bytes(size) + y.bytes(size)), (double)G * N * K, 16};
+  const Plan plan = make_plan(q, [&](int b) { return (double)G * ((N + b - 1) / b) * ((K + b - 1) / b); });
+  Workspace ws(workspace);
+  PackJob jobs[2];
+  int count = 0;
+  if (plan.pack) {
+    y.move(ws, size, jobs, &count);
+    x.move(ws, size, jobs, &count);
+  }
+  void* part = plan.split > 1 ? ws.take(plan.split * G * N * K * (size == 8 ? 8 : 4)) : nullptr;
+  if (ws.used() > 0 && (!workspace || workspace_bytes < ws.used())) return ws.used();
   DeviceScope scope(device);
   if (int rc = scope.check(what)) return rc;
-  GroupedArgs p{X, dW, const_cast<void*>(dY), offsets, T, N, K, ldx, ldw, strideW, lddy, (int)G, 0, 0};
-  const int size = size_of(dtype);
-  const bool vec = chunked(dY, lddy, N, size) && chunked(X, ldx, K, size);
   const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (count)
+    if (int rc = launch_pack(what, size, jobs, count, st)) return rc;
+  const GroupedArgs p{x.p, dW, const_cast<void*>(y.p), offsets, T, N, K, x.ld, ldw, strideW, y.ld, (int)G, 0, 0, plan.split, part};
   switch (dtype) {
-    case BGP_F64: return dw_by_type<double>(p, vec, st);
-    case BGP_F32: return dw_by_type<float>(p, vec, st);
-    case BGP_BF16: return dw_by_type<bf16_t>(p, vec, st);
-    default: return dw_by_type<f16_t>(p, vec, st);
+    case BGP_F64: return run_dw_plan<double>(p, plan, st);
+    case BGP_F32: return run_dw_plan<float>(p, plan, st);
+    case BGP_BF16: return run_dw_plan<bf16_t>(p, plan, st);
+    default: return run_dw_plan<f16_t>(p, plan, st);
   }
 }

@@ -3,6 +3,8 @@
 #include <stdarg.h>
 #include <stdio.h>
 
+#include <type_traits>
+
 #include "entry.h"
 #include "tile.h"
 
@@ -322,19 +324,8 @@ template <class T, int CUT> int run_int8(const Int8Args& p0, hipStream_t st) {
   else return launch(what, int8_gemm_pipe_kernel<T, B, B>, grid, dim3(pipe_threads(B, 1)), st, p);
 }
 
-int pick_int8(bool vec, int64_t M, int64_t N, int64_t K) {
-  const int64_t t64 = ((M + 63) / 64) * ((N + 63) / 64), t128 = ((M + 127) / 128) * ((N + 127) / 128);
-  if (M <= 16) return DIRECT16;
-  if (t64 < 256) return DIRECT32;
-  if (!vec) return t128 < 256 ? PLAIN64 : PLAIN128;
-  if (t128 >= 1024) return PIPE256;
-  return t128 < 256 ? PIPE64 : PIPE128;
-}
-
-template <class T> int int8_by_type(const Int8Args& p, hipStream_t st) {
-  const bool vec = reinterpret_cast<uintptr_t>(p.a) % 16 == 0 && reinterpret_cast<uintptr_t>(p.b) % 16 == 0 && p.lda % 16 == 0 && p.ldb % 16 == 0 &&
-                   p.K % 16 == 0 && pipe_fits(p.lda, 1, true, 256) && pipe_fits(p.ldb, 1, true, 256);
-  switch (pick_int8(vec, p.M, p.N, p.K)) {
+template <class T> int run_int8_cut(const Int8Args& p, int cut, hipStream_t st) {
+  switch (cut) {
     case DIRECT16: return run_int8<T, DIRECT16>(p, st);
     case DIRECT32: return run_int8<T, DIRECT32>(p, st);
     case PLAIN64: return run_int8<T, PLAIN64>(p, st);
@@ -342,6 +333,17 @@ template <class T> int int8_by_type(const Int8Args& p, hipStream_t st) {
     case PIPE64: return run_int8<T, PIPE64>(p, st);
     case PIPE128: return run_int8<T, PIPE128>(p, st);
     default: return run_int8<T, PIPE256>(p, st);
+  }
+}
+
+template <int SIZE> __global__ __launch_bounds__(256) void pack_kernel(PackJob a, PackJob b) {
+  using T = typename std::conditional<SIZE == 1, int8_t, typename std::conditional<SIZE == 2, bf16_t, typename std::conditional<SIZE == 4, float, double>::type>::type>::type;
+  const PackJob& p = blockIdx.z ? b : a;
+  const int64_t c = ((int64_t)blockIdx.x * 64 + threadIdx.x) * CHE<T>;
+  if (c >= p.ld_to) return;
+  for (int64_t r = (int64_t)blockIdx.y * 4 + threadIdx.y; r < p.rows; r += (int64_t)gridDim.y * 4) {
+    const T* from = static_cast<const T*>(p.from) + r / p.per * p.stride + r % p.per * p.ld + c;
+    *reinterpret_cast<uint4*>(static_cast<T*>(p.to) + r * p.ld_to + c) = load_chunk<T, false>(from, p.extent - c);
   }
 }
 
@@ -353,6 +355,24 @@ int bgp_products_fail(int code, const char* fmt, ...) {
   vsnprintf(g_error, sizeof(g_error), fmt, ap);
   va_end(ap);
   return code;
+}
+
+int launch_pack(const char* what, int size, const PackJob* jobs, int count, hipStream_t st) {
+  int64_t chunks = 0, rows = 0;
+  for (int i = 0; i < count; ++i) {
+    chunks = jobs[i].ld_to * size / 16 > chunks ? jobs[i].ld_to * size / 16 : chunks;
+    rows = jobs[i].rows > rows ? jobs[i].rows : rows;
+  }
+  if (!chunks || !rows) return 0;
+  const int64_t y = (rows + 3) / 4;
+  const dim3 grid((unsigned)((chunks + 63) / 64), (unsigned)(y < 65535 ? y : 65535), (unsigned)count), block(64, 4);
+  const PackJob a = jobs[0], b = jobs[count - 1];
+  switch (size) {
+    case 1: return launch(what, pack_kernel<1>, grid, block, st, a, b);
+    case 2: return launch(what, pack_kernel<2>, grid, block, st, a, b);
+    case 4: return launch(what, pack_kernel<4>, grid, block, st, a, b);
+    default: return launch(what, pack_kernel<8>, grid, block, st, a, b);
+  }
 }
 
 extern "C" const char* bgp_products_last_error(void) { return g_error; }
@@ -377,8 +397,9 @@ extern "C" int bgp_quantize_rows(int device, void* stream, int dtype, int64_t M,
   }
 }
 
-extern "C" int bgp_int8_gemm(int device, void* stream, int dtype, int64_t M, int64_t N, int64_t K, const int8_t* A, int64_t lda, const int8_t* B, int64_t ldb,
-                             const void* scale_a, const void* scale_b, const void* C, int64_t ldc, void* Y, int64_t ldy) {
+extern "C" int64_t bgp_int8_gemm(int device, void* stream, int dtype, int64_t M, int64_t N, int64_t K, const int8_t* A, int64_t lda, const int8_t* B,
+                                 int64_t ldb, const void* scale_a, const void* scale_b, const void* C, int64_t ldc, void* Y, int64_t ldy, void* workspace,
+                                 int64_t workspace_bytes) {
   const char* what = "bgp_int8_gemm";
   if (dtype < BGP_F64 || dtype > BGP_F16) return bgp_products_fail(-1, "%s: unknown type %d", what, dtype);
   if (M < 0 || N < 0 || K < 0 || K > BGP_INT8_MAX_K)
@@ -387,14 +408,35 @@ extern "C" int bgp_int8_gemm(int device, void* stream, int dtype, int64_t M, int
   if (!Y || !scale_a || !scale_b || (K > 0 && (!A || !B))) return bgp_products_fail(-1, "%s: null pointer", what);
   if (lda < K || ldb < K || ldy < N || (C && ldc < N))
     return bgp_products_fail(-1, "%s: bad strides lda=%lld ldb=%lld ldc=%lld ldy=%lld", what, (long long)lda, (long long)ldb, (long long)ldc, (long long)ldy);
+  const int64_t to = padded_row(K, 1);
+  const bool a_ok = reinterpret_cast<uintptr_t>(A) % 16 == 0 && lda % 16 == 0 && pipe_fits(lda, 1, true, 256);
+  const bool b_ok = reinterpret_cast<uintptr_t>(B) % 16 == 0 && ldb % 16 == 0 && pipe_fits(ldb, 1, true, 256);
+  const Question q{1, true, a_ok && b_ok, true, false, (double)K, (a_ok ? 0.0 : (double)M * to) + (b_ok ? 0.0 : (double)N * to), (double)M * N, 1};
+  const Plan plan = make_plan(q, [&](int b) { return (double)((M + b - 1) / b) * ((N + b - 1) / b); });
+  Int8Args p{A, B, scale_a, scale_b, C, Y, M, N, K, lda, ldb, ldc, ldy, 0};
+  Workspace ws(workspace);
+  PackJob jobs[2];
+  int count = 0;
+  if (plan.pack && !a_ok) {
+    p.a = static_cast<int8_t*>(ws.take(M * to));
+    p.lda = to;
+    jobs[count++] = PackJob{A, const_cast<int8_t*>(p.a), M, M, 0, lda, K, to};
+  }
+  if (plan.pack && !b_ok) {
+    p.b = static_cast<int8_t*>(ws.take(N * to));
+    p.ldb = to;
+    jobs[count++] = PackJob{B, const_cast<int8_t*>(p.b), N, N, 0, ldb, K, to};
+  }
+  if (ws.used() > 0 && (!workspace || workspace_bytes < ws.used())) return ws.used();
   DeviceScope scope(device);
   if (int rc = scope.check(what)) return rc;
-  const Int8Args p{A, B, scale_a, scale_b, C, Y, M, N, K, lda, ldb, ldc, ldy, 0};
   const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (count)
+    if (int rc = launch_pack(what, 1, jobs, count, st)) return rc;
   switch (dtype) {
-    case BGP_F64: return int8_by_type<double>(p, st);
-    case BGP_F32: return int8_by_type<float>(p, st);
-    case BGP_BF16: return int8_by_type<bf16_t>(p, st);
-    default: return int8_by_type<f16_t>(p, st);
+    case BGP_F64: return run_int8_cut<double>(p, plan.cut, st);
+    case BGP_F32: return run_int8_cut<float>(p, plan.cut, st);
+    case BGP_BF16: return run_int8_cut<bf16_t>(p, plan.cut, st);
+    default: return run_int8_cut<f16_t>(p, plan.cut, st);
   }
 }

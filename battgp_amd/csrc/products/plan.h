@@ -1,0 +1,78 @@
+// How a product is cut, chosen by a model of its time.
+#pragma once
+
+#include <math.h>
+#include <stdint.h>
+
+// Straight from memory in tiles of 16 or 32, through registers (any operands) or pipelined (16-byte aligned rows) in tiles
+// of 64, 128 or 256.
+enum Cut { DIRECT16, DIRECT32, PLAIN64, PLAIN128, PIPE64, PIPE128, PIPE256, CUTS };
+constexpr int tile_of(int cut) {
+  return cut == DIRECT16 ? 16 : cut == DIRECT32 ? 32 : cut == PLAIN64 || cut == PIPE64 ? 64 : cut == PIPE256 ? 256 : 128;
+}
+constexpr int kind_of(int size) { return size == 1 ? 0 : size == 2 ? 1 : size == 4 ? 2 : 3; }
+
+// Measured on an MI355X, in us for one stage (128 bytes of k) of one tile: on a CU that is full of such tiles, and the time
+// from stage to stage of a tile that has its CU to itself.  {int8, 16 bits, fp32, fp64}, by Cut.  In TFLOP/s of the whole
+// chip the first row of e.g. PIPE128 is 2138, 925, 148 and 71, of DIRECT32 271, 190, 65 and 41; PLAIN* were measured
+// on operands that are not aligned, since the others are pipelined.
+constexpr float STAGE_US[4][CUTS] = {{0.115f, 0.247f, 0.43f, 1.05f, 0.187f, 0.50f, 1.68f},
+                                     {0.075f, 0.177f, 0.39f, 0.87f, 0.228f, 0.58f, 1.78f},
+                                     {0.090f, 0.260f, 0.61f, 2.20f, 0.476f, 1.82f, 9e9f},
+                                     {0.075f, 0.200f, 0.60f, 2.20f, 0.470f, 1.90f, 9e9f}};
+constexpr float ALONE_US[4][CUTS] = {{0.12f, 0.22f, 0.52f, 1.0f, 0.30f, 0.62f, 1.7f},
+                                     {0.10f, 0.20f, 0.68f, 1.1f, 0.47f, 0.59f, 1.8f},
+                                     {0.12f, 0.27f, 0.85f, 2.5f, 0.61f, 2.06f, 9e9f},
+                                     {0.10f, 0.23f, 0.88f, 2.5f, 0.59f, 1.95f, 9e9f}};
+constexpr float LAUNCH_US = 3.0f, PACK_US = 2.0f, COPY_BYTES_US = 3.5e6f;
+constexpr int CUS = 256;
+// an operand along rows that is not aligned: PLAIN128 takes 99 us instead of 59 with 16-bit types
+constexpr float ROWS_UNALIGNED = 1.6f;
+
+struct Plan {
+  int cut = PLAIN64, split = 1;
+  bool pack = false;
+};
+
+// What the model is asked: D in tiles of b x b has tiles(b) of them; k bytes of k each.
+struct Question {
+  int size;                // of an element
+  bool direct, pipe;       // which cuts the operands allow as they are
+  bool packable;           // the pipelined ones after unaligned operands have been copied into aligned rows
+  bool rows_unaligned;     // an operand along rows is not aligned
+  double k, pack_bytes;    // length of k; bytes of the operands that would be copied
+  double outputs;          // elements of D
+  int most_split;          // 1: k is not cut
+};
+
+// tiles: double(int b)
+template <class F> Plan make_plan(const Question& q, F&& tiles) {
+  Plan best;
+  double least = 1e30;
+  const int kind = kind_of(q.size);
+  const double stages = ceil(q.k * q.size / 128.0);
+  for (int cut = 0; cut < CUTS; ++cut) {
+    if (STAGE_US[kind][cut] > 1e8f || (cut <= DIRECT32 && !q.direct)) continue;
+    const bool pipe = cut >= PIPE64, pack = pipe && !q.pipe;
+    if (pack && !q.packable) continue;
+    if ((cut == PLAIN64 || cut == PLAIN128) && q.pipe) continue;
+    const double unit = tiles(tile_of(cut));
+    for (int split = 1; split <= (cut <= DIRECT32 ? 1 : q.most_split); split *= 2) {
+      if (split > 1 && stages < 4.0 * split) break;
+      const double each = ceil(unit * split / CUS), deep = ceil(stages / split);
+      double stage = each * STAGE_US[kind][cut];
+      if (stage < ALONE_US[kind][cut]) stage = ALONE_US[kind][cut];
+      if (!pipe && cut > DIRECT32 && q.size == 2 && q.rows_unaligned) stage *= ROWS_UNALIGNED;
+      double us = LAUNCH_US + deep * stage;
+      if (split > 1) us += LAUNCH_US + (split + 1) * q.outputs * (q.size == 8 ? 8 : 4) / COPY_BYTES_US;
+      if (pack) us += PACK_US + 2 * q.pack_bytes / COPY_BYTES_US;
+      if (us < least) {
+        least = us;
+        best.cut = cut;
+        best.split = split;
+        best.pack = pack;
+      }
+    }
+  }
+  return best;
+}

@@ -81,6 +81,10 @@ template <> struct Num<int8_t> {
   }
 };
 
+// what sums of a type are held in
+template <class T> struct Sum { using type = float; };
+template <> struct Sum<double> { using type = double; };
+
 // one rounding to the nearest, ties to even, of what was summed in 32 (64) bits
 template <class T, class A> __device__ __forceinline__ T round_to(A v);
 template <> __device__ __forceinline__ double round_to<double, double>(double v) { return v; }

@@ -28,6 +28,15 @@ def _check(rc: int) -> None:
         raise EngineError(_lib.load_products().bgp_products_last_error().decode())
 
 
+def _call(entry, like: torch.Tensor, *args) -> None:
+    """A C entry that may ask for a workspace: torch's allocator gives it, on the stream that the call uses."""
+    rc = entry(*args, None, 0)
+    if rc > 0:
+        work = like.new_empty(rc, dtype=torch.uint8)
+        rc = entry(*args, work.data_ptr(), rc)
+    _check(rc)
+
+
 def _gpu_tensor(name: str, t, dim: int, device: int | None = None) -> int:
     """the index of the device that ``t`` is on (checks are written for the call that passes: they cost a call its time)"""
     if not isinstance(t, torch.Tensor):
@@ -121,9 +130,10 @@ def _grouped(device, dtype, x, w, offsets, out, t, n, k, g):
     else:
         y = _output(out, "out", (t, n), x.dtype, device, (x, w, offsets))
         ldy = _rows("out", y, t, n)
-    _check(_lib.load_products().bgp_grouped_gemm(
-        device, _stream(device), dtype, t, n, k, g, x.data_ptr(), ldx, w.data_ptr(), sw, ldw, trans, offsets.data_ptr(), y.data_ptr(), ldy, out is None,
-    ))
+    _call(
+        _lib.load_products().bgp_grouped_gemm, x, device, _stream(device), dtype, t, n, k, g, x.data_ptr(), ldx, w.data_ptr(), sw, ldw, trans,
+        offsets.data_ptr(), y.data_ptr(), ldy, out is None,
+    )
     return y
 
 
@@ -169,9 +179,10 @@ def grouped_matmul_grad(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, offs
         dx = _grouped(device, dtype, dy, w.transpose(1, 2), offsets, None, t, k, n, g)
     if need_dw:
         dw = x.new_empty((g, n, k))
-        _check(_lib.load_products().bgp_grouped_gemm_dw(
-            device, _stream(device), dtype, t, n, k, g, dy.data_ptr(), lddy, x.data_ptr(), ldx, offsets.data_ptr(), dw.data_ptr(), n * (k or 1), k or 1,
-        ))
+        _call(
+            _lib.load_products().bgp_grouped_gemm_dw, x, device, _stream(device), dtype, t, n, k, g, dy.data_ptr(), lddy, x.data_ptr(), ldx,
+            offsets.data_ptr(), dw.data_ptr(), n * (k or 1), k or 1,
+        )
     return dx, dw
 
 
@@ -239,7 +250,8 @@ def int8_matmul(
             inputs.append(c)
         y = _output(out, "out", (m, n), dtype, device, inputs)
         ldy = _rows("out", y, m, n)
-    _check(_lib.load_products().bgp_int8_gemm(
-        device, _stream(device), code, m, n, k, a.data_ptr(), lda, b.data_ptr(), ldb, a_scale.data_ptr(), b_scale.data_ptr(), cp, ldc, y.data_ptr(), ldy,
-    ))
+    _call(
+        _lib.load_products().bgp_int8_gemm, a, device, _stream(device), code, m, n, k, a.data_ptr(), lda, b.data_ptr(), ldb, a_scale.data_ptr(),
+        b_scale.data_ptr(), cp, ldc, y.data_ptr(), ldy,
+    )
     return y
