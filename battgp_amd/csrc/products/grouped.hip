@@ -11,7 +11,7 @@ namespace {
 // name wrong rows but none outside the matrix.  Every wave of a workgroup works its own tile out for itself: 64 groups
 // at a time, one prefix sum over the lanes.
 struct RowTile {
-  int g, tn;
+  int g;
   int64_t row0, rows;
 };
 
@@ -68,33 +68,24 @@ __device__ __forceinline__ Bounds lane_bounds(const GroupedArgs& p, int BM, int 
   return r;
 }
 
-// The tile of this workgroup.  Workgroups go to the 8 XCDs in turn, and each XCD has an L2 of its own: the tiles that
-// exist are dealt in 8 runs, one for each XCD, and inside a run 8 row tiles are gone through before the next column tile,
-// so that the workgroups of an XCD that run together share rows of both operands.
-__device__ __forceinline__ RowTile find_row_tile(const GroupedArgs& p, int BM) {
+// all groups' row tiles; with them the bounds of this lane's first group
+__device__ __forceinline__ int count_row_tiles(const GroupedArgs& p, int BM, Bounds* first) {
   const int lane = threadIdx.x & 63, groups = p.rest ? p.G + 2 : p.G;
-  Bounds r = lane_bounds(p, BM, lane);
-  int tiles_m = __builtin_amdgcn_readlane(r.sum, 63);
-  for (int base = 64; base < groups; base += 64) tiles_m += __builtin_amdgcn_readlane(lane_bounds(p, BM, base + lane).sum, 63);
-  constexpr int XCDS = 8, DEEP = 8;
-  const int64_t total = (int64_t)tiles_m * p.tiles_n, run = (total + XCDS - 1) / XCDS;
-  const int64_t at = blockIdx.x / XCDS, i = blockIdx.x % XCDS * run + at;
-  if (at >= run || i >= total) return RowTile{-1, 0, 0, 0};
-  const int64_t strip = i / (DEEP * p.tiles_n);
-  const int in = (int)(i - strip * DEEP * p.tiles_n), deep = tiles_m - strip * DEEP < DEEP ? (int)(tiles_m - strip * DEEP) : DEEP;
-  RowTile t;
-  t.tn = in / deep;
-  int want = (int)(strip * DEEP) + in % deep;
+  *first = lane_bounds(p, BM, lane);
+  int tiles = __builtin_amdgcn_readlane(first->sum, 63);
+  for (int base = 64; base < groups; base += 64) tiles += __builtin_amdgcn_readlane(lane_bounds(p, BM, base + lane).sum, 63);
+  return tiles;
+}
+
+__device__ __forceinline__ RowTile find_row_tile(const GroupedArgs& p, int BM, Bounds r, int want) {
+  const int lane = threadIdx.x & 63;
   for (int base = 0;;) {
     const unsigned long long past = __ballot(r.sum > want);
     if (past) {
       const int j = __ffsll(past) - 1;
       const int tiles = (int)((r.b - r.a + BM - 1) / BM);
       const int64_t row0 = r.a + (int64_t)(want - (r.sum - tiles)) * BM;
-      t.g = base + j;
-      t.row0 = lane_value(row0, j);
-      t.rows = lane_value(r.b - row0 < BM ? r.b - row0 : (int64_t)BM, j);
-      return t;
+      return RowTile{base + j, lane_value(row0, j), lane_value(r.b - row0 < BM ? r.b - row0 : (int64_t)BM, j)};
     }
     want -= __builtin_amdgcn_readlane(r.sum, 63);
     base += 64;
@@ -103,11 +94,9 @@ __device__ __forceinline__ RowTile find_row_tile(const GroupedArgs& p, int BM) {
 }
 
 // Y[rows of g, :] = X[rows of g, :] W_g^T;  WK: W_g[n, k] = w[g sw + n ldw + k], else w[g sw + k ldw + n]
-template <class T, class P, int BM, int BN, bool WK> __device__ __forceinline__ void rows_tile(const GroupedArgs& p, char* lds) {
+template <class T, class P, bool WK> __device__ __forceinline__ void rows_tile(const GroupedArgs& p, const RowTile& t, int64_t n0, char* lds) {
   using A = typename Sum<T>::type;
-  const RowTile t = find_row_tile(p, BM);
-  if (t.g < 0 || (p.split > 1 && t.g >= p.G)) return;
-  const int64_t n0 = (int64_t)t.tn * BN;
+  if (p.split > 1 && t.g >= p.G) return;
   P tile;
   Operand<T> x{static_cast<const T*>(p.x) + t.row0 * p.ldx, p.ldx, t.rows};
   Operand<T> w{static_cast<const T*>(p.w), p.ldw, p.N - n0};
@@ -130,37 +119,63 @@ template <class T, class P, int BM, int BN, bool WK> __device__ __forceinline__ 
   }
 }
 
+template <class T, class P, int BM, int BN, bool WK> __device__ __forceinline__ void rows_workgroup(const GroupedArgs& p, char* lds) {
+  Bounds first;
+  const int tiles_m = count_row_tiles(p, BM, &first);
+  const int64_t i = place_runs((int64_t)tiles_m * p.tiles_n);
+  if (i < 0) return;
+  const TileAt at = tile_at(i, tiles_m, p.tiles_n);
+  rows_tile<T, P, WK>(p, find_row_tile(p, BM, first, at.m), (int64_t)at.n * BN, lds);
+}
+
 // any operands, through registers
 template <class T, int BM, int BN, bool WK> __global__ __launch_bounds__(256, 2) void grouped_rows_kernel(GroupedArgs p) {
   using P = Tile<T, BM, BN, 2, 2, true, WK, false>;
   __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
-  rows_tile<T, P, BM, BN, WK>(p, lds);
+  rows_workgroup<T, P, BM, BN, WK>(p, lds);
 }
 
 // operands in whole chunks, pipelined
 template <class T, int BM, int BN, bool WK> __global__ __launch_bounds__(pipe_threads(BM, sizeof(T)), 2) void grouped_rows_pipe_kernel(GroupedArgs p) {
   using P = PipeTile<T, BM, BN, 2, pipe_waves_w(BM, sizeof(T)), true, WK>;
   __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
-  rows_tile<T, P, BM, BN, WK>(p, lds);
+  rows_workgroup<T, P, BM, BN, WK>(p, lds);
+}
+
+// 8 waves on 256 x 256
+template <class T, bool WK> __global__ __launch_bounds__(512, 2) void grouped_rows_pipe256_kernel(GroupedArgs p) {
+  using P = PipeTile<T, 256, 256, 2, 4, true, WK>;
+  __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
+  Bounds first;
+  const int tiles_m = count_row_tiles(p, 256, &first);
+  const Place place = place_256((int64_t)tiles_m * p.tiles_n);
+  if (place.tile < 0) return;
+  const TileAt at = tile_at(place.tile, tiles_m, p.tiles_n);
+  RowTile t = find_row_tile(p, 256, first, at.m);
+  int64_t n0 = (int64_t)at.n * 256;
+  if (place.parts == 1) {
+    rows_tile<T, P, WK>(p, t, n0, lds);
+    return;
+  }
+  const int down = place.parts == 4 ? place.part >> 1 : place.part;
+  t.row0 += down * 128;
+  t.rows = t.rows - down * 128 < 128 ? t.rows - down * 128 : 128;
+  if (place.parts == 4) n0 += (place.part & 1) * 128;
+  if (t.rows <= 0 || n0 >= p.N) return;
+  if (place.parts == 4) rows_tile<T, PipeTile<T, 128, 128, 2, 4, true, WK>, WK>(p, t, n0, lds);
+  else rows_tile<T, PipeTile<T, 128, 256, 2, 4, true, WK>, WK>(p, t, n0, lds);
 }
 
 // small ones, straight from memory
 template <class T, int F, bool WK> __global__ __launch_bounds__(256) void grouped_rows_direct_kernel(GroupedArgs p) {
   using P = DirectTile<T, F, F, true, WK>;
   __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
-  rows_tile<T, P, 16 * F, 16 * F, WK>(p, lds);
+  rows_workgroup<T, P, 16 * F, 16 * F, WK>(p, lds);
 }
 
 // dW_g[n, k] = sum over the rows t of g of dY[t, n] X[t, k]
-template <class T, class P, int BM, int BN> __device__ __forceinline__ void dw_tile(const GroupedArgs& p, char* lds) {
+template <class T, class P> __device__ __forceinline__ void dw_tile(const GroupedArgs& p, int g, int64_t n0, int64_t k0, char* lds) {
   using A = typename Sum<T>::type;
-  const int tiles_k = (int)((p.K + BN - 1) / BN), tiles = p.tiles_n * tiles_k;
-  // each XCD takes whole runs of tiles: they share a group's rows
-  constexpr int XCDS = 8;
-  const int64_t total = (int64_t)tiles * p.G, run = (total + XCDS - 1) / XCDS, at = blockIdx.x / XCDS, i = blockIdx.x % XCDS * run + at;
-  if (at >= run || i >= total) return;
-  const int g = (int)(i / tiles), j = (int)(i % tiles);
-  const int64_t n0 = (int64_t)(j / tiles_k) * BM, k0 = (int64_t)(j % tiles_k) * BN;
   const int64_t a = clamp64(p.off[g], 0, p.T), b = clamp64(p.off[g + 1], a, p.T);
   P tile;
   Operand<T> dy{static_cast<const T*>(p.y) + a * p.ldy + n0, p.ldy, p.N - n0};
@@ -183,22 +198,50 @@ template <class T, class P, int BM, int BN> __device__ __forceinline__ void dw_t
   }
 }
 
+template <class T, class P, int BM, int BN> __device__ __forceinline__ void dw_workgroup(const GroupedArgs& p, char* lds) {
+  const int tiles_k = (int)((p.K + BN - 1) / BN), tiles = p.tiles_n * tiles_k;
+  const int64_t i = place_runs((int64_t)tiles * p.G);
+  if (i < 0) return;
+  const TileAt at = tile_at(i % tiles, p.tiles_n, tiles_k);
+  dw_tile<T, P>(p, (int)(i / tiles), (int64_t)at.m * BM, (int64_t)at.n * BN, lds);
+}
+
 template <class T, int BM, int BN> __global__ __launch_bounds__(256, 2) void grouped_dw_kernel(GroupedArgs p) {
   using P = Tile<T, BM, BN, 2, 2, false, false, false>;
   __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
-  dw_tile<T, P, BM, BN>(p, lds);
+  dw_workgroup<T, P, BM, BN>(p, lds);
 }
 
 template <class T, int BM, int BN> __global__ __launch_bounds__(pipe_threads(BM, sizeof(T)), 2) void grouped_dw_pipe_kernel(GroupedArgs p) {
   using P = PipeTile<T, BM, BN, 2, pipe_waves_w(BM, sizeof(T)), false, false>;
   __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
-  dw_tile<T, P, BM, BN>(p, lds);
+  dw_workgroup<T, P, BM, BN>(p, lds);
+}
+
+template <class T> __global__ __launch_bounds__(512, 2) void grouped_dw_pipe256_kernel(GroupedArgs p) {
+  using P = PipeTile<T, 256, 256, 2, 4, false, false>;
+  __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
+  const int tiles_k = (int)((p.K + 255) / 256), tiles = p.tiles_n * tiles_k;
+  const Place place = place_256((int64_t)tiles * p.G);
+  if (place.tile < 0) return;
+  const int g = (int)(place.tile / tiles);
+  const TileAt at = tile_at(place.tile % tiles, p.tiles_n, tiles_k);
+  int64_t n0 = (int64_t)at.m * 256, k0 = (int64_t)at.n * 256;
+  if (place.parts == 1) {
+    dw_tile<T, P>(p, g, n0, k0, lds);
+    return;
+  }
+  n0 += (place.parts == 4 ? place.part >> 1 : place.part) * 128;
+  if (place.parts == 4) k0 += (place.part & 1) * 128;
+  if (n0 >= p.N || k0 >= p.K) return;
+  if (place.parts == 4) dw_tile<T, PipeTile<T, 128, 128, 2, 4, false, false>>(p, g, n0, k0, lds);
+  else dw_tile<T, PipeTile<T, 128, 256, 2, 4, false, false>>(p, g, n0, k0, lds);
 }
 
 template <class T, int F> __global__ __launch_bounds__(256) void grouped_dw_direct_kernel(GroupedArgs p) {
   using P = DirectTile<T, F, F, false, false>;
   __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
-  dw_tile<T, P, 16 * F, 16 * F>(p, lds);
+  dw_workgroup<T, P, 16 * F, 16 * F>(p, lds);
 }
 
 // out[r, c] = the parts' sum, in their order; rows of no group (off != NULL) as bgp_grouped_gemm leaves them
@@ -276,11 +319,12 @@ template <class T, bool WK, int CUT> int run_rows(const GroupedArgs& p0, hipStre
   GroupedArgs p = p0;
   p.tiles_n = (int)((p.N + B - 1) / B);
   // row tiles there can be at most: a group adds less than one to its share of the rows
-  const int64_t tiles = (p.T / B + p.G + (p.rest ? 2 : 0)) * p.tiles_n + 7;
+  const int64_t tiles = (p.T / B + p.G + (p.rest ? 2 : 0)) * p.tiles_n + (B == 256 ? CUS : 7);
   if (tiles > MAX_WORKGROUPS / 2) return bgp_products_fail(-1, "%s: %lld tiles are more than one launch holds", what, (long long)tiles);
   const dim3 grid((unsigned)tiles, p.split);
   if constexpr (CUT <= DIRECT32) return launch(what, grouped_rows_direct_kernel<T, B / 16, WK>, grid, dim3(256), st, p);
   else if constexpr (CUT <= PLAIN128) return launch(what, grouped_rows_kernel<T, B, B, WK>, grid, dim3(256), st, p);
+  else if constexpr (CUT == PIPE256) return launch(what, grouped_rows_pipe256_kernel<T, WK>, grid, dim3(512), st, p);
   else return launch(what, grouped_rows_pipe_kernel<T, B, B, WK>, grid, dim3(pipe_threads(B, sizeof(T))), st, p);
 }
 
@@ -307,11 +351,12 @@ template <class T, int CUT> int run_dw(const GroupedArgs& p0, hipStream_t st) {
   constexpr int B = tile_of(CUT);
   GroupedArgs p = p0;
   p.tiles_n = (int)((p.N + B - 1) / B);
-  const int64_t tiles = (int64_t)p.G * p.tiles_n * ((p.K + B - 1) / B) + 7;
+  const int64_t tiles = (int64_t)p.G * p.tiles_n * ((p.K + B - 1) / B) + (B == 256 ? CUS : 7);
   if (tiles > MAX_WORKGROUPS / 2) return bgp_products_fail(-1, "%s: %lld tiles are more than one launch holds", what, (long long)tiles);
   const dim3 grid((unsigned)tiles, p.split);
   if constexpr (CUT <= DIRECT32) return launch(what, grouped_dw_direct_kernel<T, B / 16>, grid, dim3(256), st, p);
   else if constexpr (CUT <= PLAIN128) return launch(what, grouped_dw_kernel<T, B, B>, grid, dim3(256), st, p);
+  else if constexpr (CUT == PIPE256) return launch(what, grouped_dw_pipe256_kernel<T>, grid, dim3(512), st, p);
   else return launch(what, grouped_dw_pipe_kernel<T, B, B>, grid, dim3(pipe_threads(B, sizeof(T))), st, p);
 }
 

@@ -256,16 +256,8 @@ template <class T, bool ADD> __device__ __forceinline__ void int8_out(const v4i&
 }
 
 // Y[i, j] = (C[i, j] +) sa[i] sb[j] sum_k A[i, k] B[j, k]: the sum exact in 32 bits, the rest in 64, one rounding
-template <class T, class P, int BM, int BN> __device__ __forceinline__ void int8_tile(const Int8Args& p, char* lds) {
+template <class T, class P, int BM, int BN> __device__ __forceinline__ void int8_tile(const Int8Args& p, int64_t m0, int64_t n0, char* lds) {
   using S = typename ScaleOf<T>::type;
-  // each XCD takes a run of tiles, 8 row tiles deep (workgroups go to the 8 XCDs in turn; each has an L2 of its own)
-  constexpr int XCDS = 8, DEEP = 8;
-  const int tiles_m = (int)((p.M + BM - 1) / BM);
-  const int64_t total = (int64_t)tiles_m * p.tiles_n, run = (total + XCDS - 1) / XCDS, at = blockIdx.x / XCDS, t = blockIdx.x % XCDS * run + at;
-  if (at >= run || t >= total) return;
-  const int64_t strip = t / (DEEP * p.tiles_n);
-  const int in = (int)(t - strip * DEEP * p.tiles_n), deep = tiles_m - strip * DEEP < DEEP ? (int)(tiles_m - strip * DEEP) : DEEP;
-  const int64_t m0 = (strip * DEEP + in % deep) * BM, n0 = (int64_t)(in / deep) * BN;
   P tile;
   tile.run(Operand<int8_t>{p.a + m0 * p.lda, p.lda, p.M - m0}, Operand<int8_t>{p.b + n0 * p.ldb, p.ldb, p.N - n0}, p.K, lds);
   const S *sa = static_cast<const S*>(p.sa) + m0, *sb = static_cast<const S*>(p.sb) + n0;
@@ -290,25 +282,53 @@ template <class T, class P, int BM, int BN> __device__ __forceinline__ void int8
   }
 }
 
+template <class T, class P, int BM, int BN> __device__ __forceinline__ void int8_workgroup(const Int8Args& p, char* lds) {
+  const int tiles_m = (int)((p.M + BM - 1) / BM);
+  const int64_t i = place_runs((int64_t)tiles_m * p.tiles_n);
+  if (i < 0) return;
+  const TileAt at = tile_at(i, tiles_m, p.tiles_n);
+  int8_tile<T, P, BM, BN>(p, (int64_t)at.m * BM, (int64_t)at.n * BN, lds);
+}
+
+// 8 waves on 256 x 256
+template <class T> __global__ __launch_bounds__(512, 2) void int8_gemm_pipe256_kernel(Int8Args p) {
+  using P = PipeTile<int8_t, 256, 256, 2, 4, true, true>;
+  __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
+  const int tiles_m = (int)((p.M + 255) / 256);
+  const Place place = place_256((int64_t)tiles_m * p.tiles_n);
+  if (place.tile < 0) return;
+  const TileAt at = tile_at(place.tile, tiles_m, p.tiles_n);
+  int64_t m0 = (int64_t)at.m * 256, n0 = (int64_t)at.n * 256;
+  if (place.parts == 1) {
+    int8_tile<T, P, 256, 256>(p, m0, n0, lds);
+    return;
+  }
+  m0 += (place.parts == 4 ? place.part >> 1 : place.part) * 128;
+  if (place.parts == 4) n0 += (place.part & 1) * 128;
+  if (m0 >= p.M || n0 >= p.N) return;
+  if (place.parts == 4) int8_tile<T, PipeTile<int8_t, 128, 128, 2, 4, true, true>, 128, 128>(p, m0, n0, lds);
+  else int8_tile<T, PipeTile<int8_t, 128, 256, 2, 4, true, true>, 128, 256>(p, m0, n0, lds);
+}
+
 // any operands, through registers
 template <class T, int BM, int BN> __global__ __launch_bounds__(256, 2) void int8_gemm_kernel(Int8Args p) {
   using P = Tile<int8_t, BM, BN, 2, 2, true, true, false>;
   __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
-  int8_tile<T, P, BM, BN>(p, lds);
+  int8_workgroup<T, P, BM, BN>(p, lds);
 }
 
 // operands in whole chunks, pipelined
 template <class T, int BM, int BN> __global__ __launch_bounds__(pipe_threads(BM, 1), 2) void int8_gemm_pipe_kernel(Int8Args p) {
   using P = PipeTile<int8_t, BM, BN, 2, pipe_waves_w(BM, 1), true, true>;
   __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
-  int8_tile<T, P, BM, BN>(p, lds);
+  int8_workgroup<T, P, BM, BN>(p, lds);
 }
 
 // small ones, straight from memory
 template <class T, int F> __global__ __launch_bounds__(256) void int8_gemm_direct_kernel(Int8Args p) {
   using P = DirectTile<int8_t, F, F, true, true>;
   __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
-  int8_tile<T, P, 16 * F, 16 * F>(p, lds);
+  int8_workgroup<T, P, 16 * F, 16 * F>(p, lds);
 }
 
 template <class T, int CUT> int run_int8(const Int8Args& p0, hipStream_t st) {
@@ -316,11 +336,12 @@ template <class T, int CUT> int run_int8(const Int8Args& p0, hipStream_t st) {
   constexpr int B = tile_of(CUT);
   Int8Args p = p0;
   p.tiles_n = (int)((p.N + B - 1) / B);
-  const int64_t tiles = (p.M + B - 1) / B * p.tiles_n + 7;
+  const int64_t tiles = (p.M + B - 1) / B * p.tiles_n + (B == 256 ? CUS : 7);
   if (tiles > MAX_WORKGROUPS / 2) return bgp_products_fail(-1, "%s: %lld tiles are more than one launch holds", what, (long long)tiles);
   const dim3 grid((unsigned)tiles);
   if constexpr (CUT <= DIRECT32) return launch(what, int8_gemm_direct_kernel<T, B / 16>, grid, dim3(256), st, p);
   else if constexpr (CUT <= PLAIN128) return launch(what, int8_gemm_kernel<T, B, B>, grid, dim3(256), st, p);
+  else if constexpr (CUT == PIPE256) return launch(what, int8_gemm_pipe256_kernel<T>, grid, dim3(512), st, p);
   else return launch(what, int8_gemm_pipe_kernel<T, B, B>, grid, dim3(pipe_threads(B, 1)), st, p);
 }
 

@@ -371,6 +371,14 @@ template <class T, int BM, int BN, int WX, int WW, bool XK, bool WK> struct Pipe
       interleave();
       __builtin_amdgcn_sched_barrier(0);
     };
+    if (x0() >= x.rows || w0() >= w.rows) {  // none of this wave's elements exist: it only loads
+      for (int s = 0, buf = 0; s < stages; ++s, buf ^= 1) {
+        asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+        if (s + 2 < stages) issue(buf);
+      }
+      asm volatile("s_barrier" ::: "memory");
+      return;
+    }
     read(0, 0);
     for (int s = 0, buf = 0; s < stages; ++s, buf ^= 1) {
       __builtin_amdgcn_sched_barrier(0);
