@@ -36,32 +36,33 @@ template <class... A> int launch(const char* what, void (*kernel)(A...), dim3 gr
   return e == hipSuccess ? 0 : bgp_products_fail(-2, "%s: launch failed: %s", what, hipGetErrorString(e));
 }
 
-// Waves of a pipelined tile: 2 x 4 of 128 x 64 on 256 x 256; 2 x 2 below, but 2 x 4 of 64 x 32 for fp64 on 128 x 128, whose
+// Waves of a tile in LDS: 2 x 4 of 128 x 64 on 256 x 256; 2 x 2 below, but 2 x 4 of 64 x 32 for fp64 on 128 x 128, whose
 // accumulators take twice the registers.
-constexpr int pipe_waves_w(int tile, int size) { return tile == 256 || (size == 8 && tile == 128) ? 4 : 2; }
-constexpr int pipe_threads(int tile, int size) { return 128 * pipe_waves_w(tile, size); }
+constexpr int waves_w(int tile, int size) { return tile == 256 || (size == 8 && tile == 128) ? 4 : 2; }
+constexpr int tile_threads(int tile, int size) { return 128 * waves_w(tile, size); }
 
 #ifdef __HIPCC__
 // Tiles of 256 x 256 fill a CU each, so the last round of 256 workgroups may have few: its tiles are cut into 2 or 4 parts
 // (128 x 256, 128 x 128) where that still is one round.  4099 rows of 8 groups to 2816 columns (k = 1000, bf16), about 270
 // tiles: 39.7 us without.  Workgroups go to the 8 XCDs in turn, and each XCD has an L2 of its own: whole rounds are
 // dealt in runs, one for each XCD.
+// (A launch has less than 2^23 tiles: 32 bits do.)
 struct Place {
-  int64_t tile;  // -1: nothing to do
+  int tile;  // -1: nothing to do
   int parts, part;
 };
-__device__ __forceinline__ Place place_256(int64_t total) {
-  constexpr int64_t XCDS = 8;
-  const int64_t whole = total / CUS * CUS, left = total - whole, i = blockIdx.x;
+__device__ __forceinline__ Place place_256(int total) {
+  constexpr int XCDS = 8;
+  const int whole = total / CUS * CUS, left = total - whole, i = blockIdx.x;
   if (i < whole) return Place{i % XCDS * (whole / XCDS) + i / XCDS, 1, 0};
   const int parts = left * 4 <= CUS ? 4 : left * 2 <= CUS ? 2 : 1;
-  const int64_t j = i - whole;
-  return j < left * parts ? Place{whole + j / parts, parts, (int)(j % parts)} : Place{-1, 1, 0};
+  const int j = i - whole;
+  return j < left * parts ? Place{whole + j / parts, parts, j % parts} : Place{-1, 1, 0};
 }
 // smaller tiles: all of them in runs
-__device__ __forceinline__ int64_t place_runs(int64_t total) {
-  constexpr int64_t XCDS = 8;
-  const int64_t run = (total + XCDS - 1) / XCDS, at = blockIdx.x / XCDS, i = blockIdx.x % XCDS * run + at;
+__device__ __forceinline__ int place_runs(int total) {
+  constexpr int XCDS = 8;
+  const int run = (total + XCDS - 1) / XCDS, at = blockIdx.x / XCDS, i = blockIdx.x % XCDS * run + at;
   return at < run && i < total ? i : -1;
 }
 // inside a run 8 row tiles are gone through before the next column tile, so that workgroups that run together share rows
@@ -69,11 +70,10 @@ __device__ __forceinline__ int64_t place_runs(int64_t total) {
 struct TileAt {
   int m, n;
 };
-__device__ __forceinline__ TileAt tile_at(int64_t i, int tiles_m, int tiles_n) {
+__device__ __forceinline__ TileAt tile_at(int i, int tiles_m, int tiles_n) {
   constexpr int DEEP = 8;
-  const int64_t strip = i / (DEEP * tiles_n);
-  const int in = (int)(i - strip * DEEP * tiles_n), deep = tiles_m - strip * DEEP < DEEP ? (int)(tiles_m - strip * DEEP) : DEEP;
-  return TileAt{(int)(strip * DEEP) + in % deep, in / deep};
+  const int strip = i / (DEEP * tiles_n), in = i - strip * DEEP * tiles_n, deep = tiles_m - strip * DEEP < DEEP ? tiles_m - strip * DEEP : DEEP;
+  return TileAt{strip * DEEP + in % deep, in / deep};
 }
 #endif
 

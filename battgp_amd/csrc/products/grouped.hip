@@ -38,8 +38,21 @@ struct Part {
   int64_t from, length;
 };
 __device__ __forceinline__ Part part_of(int64_t k, int stage, int split, int i) {
-  const int64_t stages = (k + stage - 1) / stage, each = (stages + split - 1) / split * stage, from = i * each;
+  if (split == 1) return Part{0, k};
+  const uint32_t stages = (uint32_t)((k + stage - 1) / stage);
+  const int64_t each = (int64_t)((stages + split - 1) / split) * stage, from = i * each;
   return Part{from, from >= k ? 0 : k - from < each ? k - from : each};
+}
+
+// the sum over the lanes up to and with this one: inside rows of 16 lanes, then the last of a row to the rows behind it
+__device__ __forceinline__ int lane_sum(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15 to the second and fourth row
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31 to the upper half
+  return v;
 }
 
 struct Bounds {
@@ -48,7 +61,7 @@ struct Bounds {
 };
 
 __device__ __forceinline__ Bounds lane_bounds(const GroupedArgs& p, int BM, int g) {
-  const int G = p.G, lane = threadIdx.x & 63;
+  const int G = p.G;
   Bounds r{0, 0, 0};
   if (g < G) {
     r.a = clamp64(p.off[g], 0, p.T);
@@ -59,12 +72,7 @@ __device__ __forceinline__ Bounds lane_bounds(const GroupedArgs& p, int BM, int 
     r.a = clamp64(p.off[G], 0, p.T);
     r.b = p.T;
   }
-  r.sum = (int)((r.b - r.a + BM - 1) / BM);
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int v = __shfl_up(r.sum, d);
-    if (lane >= d) r.sum += v;
-  }
+  r.sum = lane_sum((int)((uint64_t)(r.b - r.a + BM - 1) / (unsigned)BM));
   return r;
 }
 
@@ -83,7 +91,7 @@ __device__ __forceinline__ RowTile find_row_tile(const GroupedArgs& p, int BM, B
     const unsigned long long past = __ballot(r.sum > want);
     if (past) {
       const int j = __ffsll(past) - 1;
-      const int tiles = (int)((r.b - r.a + BM - 1) / BM);
+      const int tiles = (int)((uint64_t)(r.b - r.a + BM - 1) / (unsigned)BM);
       const int64_t row0 = r.a + (int64_t)(want - (r.sum - tiles)) * BM;
       return RowTile{base + j, lane_value(row0, j), lane_value(r.b - row0 < BM ? r.b - row0 : (int64_t)BM, j)};
     }
@@ -96,48 +104,41 @@ __device__ __forceinline__ RowTile find_row_tile(const GroupedArgs& p, int BM, B
 // Y[rows of g, :] = X[rows of g, :] W_g^T;  WK: W_g[n, k] = w[g sw + n ldw + k], else w[g sw + k ldw + n]
 template <class T, class P, bool WK> __device__ __forceinline__ void rows_tile(const GroupedArgs& p, const RowTile& t, int64_t n0, char* lds) {
   using A = typename Sum<T>::type;
-  if (p.split > 1 && t.g >= p.G) return;
+  const bool some = t.g < p.G;
+  if (p.split > 1 && !some) return;
+  const Part k = some ? part_of(p.K, KSTAGE<T>, p.split, blockIdx.y) : Part{0, 0};
+  const Operand<T> x{static_cast<const T*>(p.x) + t.row0 * p.ldx + k.from, p.ldx, t.rows, p.K >= CHE<T>};
+  const Operand<T> w{static_cast<const T*>(p.w) + (some ? t.g * p.sw + (WK ? n0 * p.ldw + k.from : n0 + k.from * p.ldw) : 0), p.ldw, p.N - n0,
+                     (WK ? p.K : p.N) >= CHE<T>};
   P tile;
-  Operand<T> x{static_cast<const T*>(p.x) + t.row0 * p.ldx, p.ldx, t.rows};
-  Operand<T> w{static_cast<const T*>(p.w), p.ldw, p.N - n0};
-  if (t.g < p.G) w.p += t.g * p.sw + (WK ? n0 * p.ldw : n0);
+  tile.run(x, w, k.length, lds);
   if (p.split == 1) {
-    tile.run(x, w, t.g < p.G ? p.K : 0, lds);
-    T* y = static_cast<T*>(p.y) + t.row0 * p.ldy + n0;
-    tile.each([&](int i, int j, int step, const typename P::acc_t& v) {
-      if (i < t.rows) store_row(y + i * p.ldy, j, step, v, p.N - n0);
-    });
+    tile.template out<PlainRows<T>::E>(lds, t.rows, PlainRows<T>{static_cast<T*>(p.y) + t.row0 * p.ldy + n0, p.ldy, p.N - n0});
   } else {
-    const Part k = part_of(p.K, KSTAGE<T>, p.split, blockIdx.y);
-    x.p += k.from;
-    w.p += WK ? k.from : k.from * p.ldw;
-    tile.run(x, w, k.length, lds);
     A* y = static_cast<A*>(p.part) + (blockIdx.y * p.T + t.row0) * p.N + n0;
-    tile.each([&](int i, int j, int step, const typename P::acc_t& v) {
-      if (i < t.rows) store_row(y + i * p.N, j, step, v, p.N - n0);
-    });
+    tile.template out<PlainRows<A>::E>(lds, t.rows, PlainRows<A>{y, p.N, p.N - n0});
   }
 }
 
 template <class T, class P, int BM, int BN, bool WK> __device__ __forceinline__ void rows_workgroup(const GroupedArgs& p, char* lds) {
   Bounds first;
   const int tiles_m = count_row_tiles(p, BM, &first);
-  const int64_t i = place_runs((int64_t)tiles_m * p.tiles_n);
+  const int i = place_runs(tiles_m * p.tiles_n);
   if (i < 0) return;
   const TileAt at = tile_at(i, tiles_m, p.tiles_n);
   rows_tile<T, P, WK>(p, find_row_tile(p, BM, first, at.m), (int64_t)at.n * BN, lds);
 }
 
 // any operands, through registers
-template <class T, int BM, int BN, bool WK> __global__ __launch_bounds__(256, 2) void grouped_rows_kernel(GroupedArgs p) {
-  using P = Tile<T, BM, BN, 2, 2, true, WK, false>;
+template <class T, int BM, int BN, bool WK> __global__ __launch_bounds__(tile_threads(BM, sizeof(T)), 2) void grouped_rows_kernel(GroupedArgs p) {
+  using P = Tile<T, BM, BN, 2, waves_w(BM, sizeof(T)), true, WK>;
   __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
   rows_workgroup<T, P, BM, BN, WK>(p, lds);
 }
 
 // operands in whole chunks, pipelined
-template <class T, int BM, int BN, bool WK> __global__ __launch_bounds__(pipe_threads(BM, sizeof(T)), 2) void grouped_rows_pipe_kernel(GroupedArgs p) {
-  using P = PipeTile<T, BM, BN, 2, pipe_waves_w(BM, sizeof(T)), true, WK>;
+template <class T, int BM, int BN, bool WK> __global__ __launch_bounds__(tile_threads(BM, sizeof(T)), 2) void grouped_rows_pipe_kernel(GroupedArgs p) {
+  using P = PipeTile<T, BM, BN, 2, waves_w(BM, sizeof(T)), true, WK>;
   __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
   rows_workgroup<T, P, BM, BN, WK>(p, lds);
 }
@@ -148,7 +149,7 @@ template <class T, bool WK> __global__ __launch_bounds__(512, 2) void grouped_ro
   __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
   Bounds first;
   const int tiles_m = count_row_tiles(p, 256, &first);
-  const Place place = place_256((int64_t)tiles_m * p.tiles_n);
+  const Place place = place_256(tiles_m * p.tiles_n);
   if (place.tile < 0) return;
   const TileAt at = tile_at(place.tile, tiles_m, p.tiles_n);
   RowTile t = find_row_tile(p, 256, first, at.m);
@@ -177,43 +178,36 @@ template <class T, int F, bool WK> __global__ __launch_bounds__(256) void groupe
 template <class T, class P> __device__ __forceinline__ void dw_tile(const GroupedArgs& p, int g, int64_t n0, int64_t k0, char* lds) {
   using A = typename Sum<T>::type;
   const int64_t a = clamp64(p.off[g], 0, p.T), b = clamp64(p.off[g + 1], a, p.T);
+  const Part t = part_of(b - a, KSTAGE<T>, p.split, blockIdx.y);
+  const Operand<T> dy{static_cast<const T*>(p.y) + (a + t.from) * p.ldy + n0, p.ldy, p.N - n0, p.N >= CHE<T>};
+  const Operand<T> x{static_cast<const T*>(p.x) + (a + t.from) * p.ldx + k0, p.ldx, p.K - k0, p.K >= CHE<T>};
   P tile;
-  Operand<T> dy{static_cast<const T*>(p.y) + a * p.ldy + n0, p.ldy, p.N - n0};
-  Operand<T> x{static_cast<const T*>(p.x) + a * p.ldx + k0, p.ldx, p.K - k0};
+  tile.run(dy, x, t.length, lds);
   if (p.split == 1) {
-    tile.run(dy, x, b - a, lds);
     T* dw = static_cast<T*>(const_cast<void*>(p.w)) + g * p.sw + n0 * p.ldw + k0;
-    tile.each([&](int r, int c, int step, const typename P::acc_t& v) {
-      if (r < p.N - n0) store_row(dw + r * p.ldw, c, step, v, p.K - k0);
-    });
+    tile.template out<PlainRows<T>::E>(lds, p.N - n0, PlainRows<T>{dw, p.ldw, p.K - k0});
   } else {
-    const Part t = part_of(b - a, KSTAGE<T>, p.split, blockIdx.y);
-    dy.p += t.from * p.ldy;
-    x.p += t.from * p.ldx;
-    tile.run(dy, x, t.length, lds);
     A* dw = static_cast<A*>(p.part) + (((int64_t)blockIdx.y * p.G + g) * p.N + n0) * p.K + k0;
-    tile.each([&](int r, int c, int step, const typename P::acc_t& v) {
-      if (r < p.N - n0) store_row(dw + r * p.K, c, step, v, p.K - k0);
-    });
+    tile.template out<PlainRows<A>::E>(lds, p.N - n0, PlainRows<A>{dw, p.K, p.K - k0});
   }
 }
 
 template <class T, class P, int BM, int BN> __device__ __forceinline__ void dw_workgroup(const GroupedArgs& p, char* lds) {
   const int tiles_k = (int)((p.K + BN - 1) / BN), tiles = p.tiles_n * tiles_k;
-  const int64_t i = place_runs((int64_t)tiles * p.G);
+  const int i = place_runs(tiles * p.G);
   if (i < 0) return;
   const TileAt at = tile_at(i % tiles, p.tiles_n, tiles_k);
-  dw_tile<T, P>(p, (int)(i / tiles), (int64_t)at.m * BM, (int64_t)at.n * BN, lds);
+  dw_tile<T, P>(p, i / tiles, (int64_t)at.m * BM, (int64_t)at.n * BN, lds);
 }
 
-template <class T, int BM, int BN> __global__ __launch_bounds__(256, 2) void grouped_dw_kernel(GroupedArgs p) {
-  using P = Tile<T, BM, BN, 2, 2, false, false, false>;
+template <class T, int BM, int BN> __global__ __launch_bounds__(tile_threads(BM, sizeof(T)), 2) void grouped_dw_kernel(GroupedArgs p) {
+  using P = Tile<T, BM, BN, 2, waves_w(BM, sizeof(T)), false, false>;
   __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
   dw_workgroup<T, P, BM, BN>(p, lds);
 }
 
-template <class T, int BM, int BN> __global__ __launch_bounds__(pipe_threads(BM, sizeof(T)), 2) void grouped_dw_pipe_kernel(GroupedArgs p) {
-  using P = PipeTile<T, BM, BN, 2, pipe_waves_w(BM, sizeof(T)), false, false>;
+template <class T, int BM, int BN> __global__ __launch_bounds__(tile_threads(BM, sizeof(T)), 2) void grouped_dw_pipe_kernel(GroupedArgs p) {
+  using P = PipeTile<T, BM, BN, 2, waves_w(BM, sizeof(T)), false, false>;
   __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
   dw_workgroup<T, P, BM, BN>(p, lds);
 }
@@ -222,9 +216,9 @@ template <class T> __global__ __launch_bounds__(512, 2) void grouped_dw_pipe256_
   using P = PipeTile<T, 256, 256, 2, 4, false, false>;
   __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
   const int tiles_k = (int)((p.K + 255) / 256), tiles = p.tiles_n * tiles_k;
-  const Place place = place_256((int64_t)tiles * p.G);
+  const Place place = place_256(tiles * p.G);
   if (place.tile < 0) return;
-  const int g = (int)(place.tile / tiles);
+  const int g = place.tile / tiles;
   const TileAt at = tile_at(place.tile % tiles, p.tiles_n, tiles_k);
   int64_t n0 = (int64_t)at.m * 256, k0 = (int64_t)at.n * 256;
   if (place.parts == 1) {
@@ -323,9 +317,9 @@ template <class T, bool WK, int CUT> int run_rows(const GroupedArgs& p0, hipStre
   if (tiles > MAX_WORKGROUPS / 2) return bgp_products_fail(-1, "%s: %lld tiles are more than one launch holds", what, (long long)tiles);
   const dim3 grid((unsigned)tiles, p.split);
   if constexpr (CUT <= DIRECT32) return launch(what, grouped_rows_direct_kernel<T, B / 16, WK>, grid, dim3(256), st, p);
-  else if constexpr (CUT <= PLAIN128) return launch(what, grouped_rows_kernel<T, B, B, WK>, grid, dim3(256), st, p);
+  else if constexpr (CUT <= PLAIN128) return launch(what, grouped_rows_kernel<T, B, B, WK>, grid, dim3(tile_threads(B, sizeof(T))), st, p);
   else if constexpr (CUT == PIPE256) return launch(what, grouped_rows_pipe256_kernel<T, WK>, grid, dim3(512), st, p);
-  else return launch(what, grouped_rows_pipe_kernel<T, B, B, WK>, grid, dim3(pipe_threads(B, sizeof(T))), st, p);
+  else return launch(what, grouped_rows_pipe_kernel<T, B, B, WK>, grid, dim3(tile_threads(B, sizeof(T))), st, p);
 }
 
 template <class T, bool WK> int rows_by_cut(const GroupedArgs& p, int cut, hipStream_t st) {
@@ -355,9 +349,9 @@ template <class T, int CUT> int run_dw(const GroupedArgs& p0, hipStream_t st) {
   if (tiles > MAX_WORKGROUPS / 2) return bgp_products_fail(-1, "%s: %lld tiles are more than one launch holds", what, (long long)tiles);
   const dim3 grid((unsigned)tiles, p.split);
   if constexpr (CUT <= DIRECT32) return launch(what, grouped_dw_direct_kernel<T, B / 16>, grid, dim3(256), st, p);
-  else if constexpr (CUT <= PLAIN128) return launch(what, grouped_dw_kernel<T, B, B>, grid, dim3(256), st, p);
+  else if constexpr (CUT <= PLAIN128) return launch(what, grouped_dw_kernel<T, B, B>, grid, dim3(tile_threads(B, sizeof(T))), st, p);
   else if constexpr (CUT == PIPE256) return launch(what, grouped_dw_pipe256_kernel<T>, grid, dim3(512), st, p);
-  else return launch(what, grouped_dw_pipe_kernel<T, B, B>, grid, dim3(pipe_threads(B, sizeof(T))), st, p);
+  else return launch(what, grouped_dw_pipe_kernel<T, B, B>, grid, dim3(tile_threads(B, sizeof(T))), st, p);
 }
 
 template <class T> int dw_by_cut(const GroupedArgs& p, int cut, hipStream_t st) {
@@ -405,7 +399,8 @@ extern "C" int64_t bgp_grouped_gemm(int device, void* stream, int dtype, int64_t
     return bgp_products_fail(-1, "%s: bad strides ldx=%lld ldw=%lld strideW=%lld ldy=%lld", what, (long long)ldx, (long long)ldw, (long long)strideW, (long long)ldy);
   const int size = size_of(dtype);
   Laid x(X, 1, 0, T, ldx, K, size, true), w(W, strideW ? G : 1, strideW, w_trans ? K : N, ldw, w_trans ? N : K, size, !w_trans);
-  const Question q{size, !w_trans || size >= 4, x.ok && w.ok, pipe_fits(padded_row(x.extent, size), size, true, 256) && pipe_fits(padded_row(w.extent, size), size, !w_trans, 256),
+  const bool wide = K * size >= 16 && (!w_trans || N * size >= 16);
+  const Question q{size, wide && (!w_trans || size >= 4), x.ok && w.ok, pipe_fits(padded_row(x.extent, size), size, true, 256) && pipe_fits(padded_row(w.extent, size), size, !w_trans, 256),
                    !w.along_k && !w.ok, (double)K, (double)(x.bytes(size) + w.bytes(size)), (double)T * N, G > 0 ? 16 : 1};
   const Plan plan = make_plan(q, [&](int b) { return expected_tiles(T, G, b) * ((N + b - 1) / b); });
   Workspace ws(workspace);

@@ -96,7 +96,7 @@ template <class T, bool POW2, int TPR, int U, bool LONG> __global__ __launch_bou
       constexpr int N = (int)sizeof(T) / 2;  // 16-byte chunks
 #pragma unroll
       for (int c = 0; c < N; ++c) {
-        const uint4 u = load_chunk<T, false>(x + k + c * CHE<T>, CHE<T>);
+        const chunk_t u = load_any(x + k + c * CHE<T>);
         __builtin_memcpy(e + c * CHE<T>, &u, 16);
       }
     } else {
@@ -239,52 +239,57 @@ struct Int8Args {
   int tiles_n;
 };
 
-// 4 neighbours of a row, at the alignment of one
-template <class T> struct __attribute__((packed, aligned(sizeof(T)))) Four { T e[4]; };
+// N neighbours of a row, at the alignment of one
+template <class T, int N> struct __attribute__((packed, aligned(sizeof(T)))) Few { T e[N]; };
 
-template <class T, bool ADD> __device__ __forceinline__ void int8_out(const v4i& v, typename ScaleOf<T>::type sa, const typename ScaleOf<T>::type* sb, const T* c, T* y) {
+// scaled sums to D's rows, 16 bytes at a time
+template <class T, bool ADD> struct ScaledRows {
   using S = typename ScaleOf<T>::type;
-  const Four<S> s = *reinterpret_cast<const Four<S>*>(sb);
-  Four<T> add, o;
-  if (ADD) add = *reinterpret_cast<const Four<T>*>(c);
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const double r = (double)v[e] * ((double)sa * (double)s.e[e]);
-    o.e[e] = narrow<T>(ADD ? r + widen(add.e[e]) : r);
+  static constexpr int E = 16 / (int)sizeof(T);
+  T* y;
+  const T* c;
+  const S *sa, *sb;
+  int64_t ldy, ldc, cols;
+  __device__ __forceinline__ void single(int i, int j, int v) const {
+    if (j >= cols) return;
+    const double r = (double)v * ((double)sa[i] * (double)sb[j]);
+    y[i * ldy + j] = narrow<T>(ADD ? r + widen(c[i * ldc + j]) : r);
   }
-  *reinterpret_cast<Four<T>*>(y) = o;
-}
+  __device__ __forceinline__ void operator()(int i, int j, const int* v) const {
+    if (j + E <= cols) {
+      const Few<S, E> s = *reinterpret_cast<const Few<S, E>*>(sb + j);
+      const double si = (double)sa[i];
+      Few<T, E> add, o;
+      if (ADD) add = *reinterpret_cast<const Few<T, E>*>(c + i * ldc + j);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const double r = (double)v[e] * (si * (double)s.e[e]);
+        o.e[e] = narrow<T>(ADD ? r + widen(add.e[e]) : r);
+      }
+      *reinterpret_cast<Few<T, E>*>(y + i * ldy + j) = o;
+    } else {
+#pragma unroll 1
+      for (int e = 0; e < E; ++e) single(i, j + e, v[e]);
+    }
+  }
+};
 
 // Y[i, j] = (C[i, j] +) sa[i] sb[j] sum_k A[i, k] B[j, k]: the sum exact in 32 bits, the rest in 64, one rounding
 template <class T, class P, int BM, int BN> __device__ __forceinline__ void int8_tile(const Int8Args& p, int64_t m0, int64_t n0, char* lds) {
   using S = typename ScaleOf<T>::type;
   P tile;
-  tile.run(Operand<int8_t>{p.a + m0 * p.lda, p.lda, p.M - m0}, Operand<int8_t>{p.b + n0 * p.ldb, p.ldb, p.N - n0}, p.K, lds);
+  tile.run(Operand<int8_t>{p.a + m0 * p.lda, p.lda, p.M - m0, p.K >= 16}, Operand<int8_t>{p.b + n0 * p.ldb, p.ldb, p.N - n0, p.K >= 16}, p.K, lds);
   const S *sa = static_cast<const S*>(p.sa) + m0, *sb = static_cast<const S*>(p.sb) + n0;
   T* y = static_cast<T*>(p.y) + m0 * p.ldy + n0;
   const T* c = p.c ? static_cast<const T*>(p.c) + m0 * p.ldc + n0 : nullptr;
   const int64_t rows = p.M - m0, cols = p.N - n0;
-  if (rows >= BM && cols >= BN && !c) {  // whole tiles without a branch per element, so that loads and stores run ahead
-    tile.each([&](int i, int j, int, const v4i& v) { int8_out<T, false>(v, sa[i], sb + j, nullptr, y + i * p.ldy + j); });
-  } else if (rows >= BM && cols >= BN) {
-    tile.each([&](int i, int j, int, const v4i& v) { int8_out<T, true>(v, sa[i], sb + j, c + i * p.ldc + j, y + i * p.ldy + j); });
-  } else {
-    tile.each([&](int i, int j, int, const v4i& v) {
-      if (i >= rows) return;
-      const double si = (double)sa[i];
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (j + e < cols) {
-          const double r = (double)v[e] * (si * (double)sb[j + e]);
-          y[i * p.ldy + j + e] = narrow<T>(c ? r + widen(c[i * p.ldc + j + e]) : r);
-        }
-    });
-  }
+  if (c) tile.template out<ScaledRows<T, true>::E>(lds, rows, ScaledRows<T, true>{y, c, sa, sb, p.ldy, p.ldc, cols});
+  else tile.template out<ScaledRows<T, false>::E>(lds, rows, ScaledRows<T, false>{y, c, sa, sb, p.ldy, p.ldc, cols});
 }
 
 template <class T, class P, int BM, int BN> __device__ __forceinline__ void int8_workgroup(const Int8Args& p, char* lds) {
   const int tiles_m = (int)((p.M + BM - 1) / BM);
-  const int64_t i = place_runs((int64_t)tiles_m * p.tiles_n);
+  const int i = place_runs(tiles_m * p.tiles_n);
   if (i < 0) return;
   const TileAt at = tile_at(i, tiles_m, p.tiles_n);
   int8_tile<T, P, BM, BN>(p, (int64_t)at.m * BM, (int64_t)at.n * BN, lds);
@@ -295,7 +300,7 @@ template <class T> __global__ __launch_bounds__(512, 2) void int8_gemm_pipe256_k
   using P = PipeTile<int8_t, 256, 256, 2, 4, true, true>;
   __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
   const int tiles_m = (int)((p.M + 255) / 256);
-  const Place place = place_256((int64_t)tiles_m * p.tiles_n);
+  const Place place = place_256(tiles_m * p.tiles_n);
   if (place.tile < 0) return;
   const TileAt at = tile_at(place.tile, tiles_m, p.tiles_n);
   int64_t m0 = (int64_t)at.m * 256, n0 = (int64_t)at.n * 256;
@@ -312,14 +317,14 @@ template <class T> __global__ __launch_bounds__(512, 2) void int8_gemm_pipe256_k
 
 // any operands, through registers
 template <class T, int BM, int BN> __global__ __launch_bounds__(256, 2) void int8_gemm_kernel(Int8Args p) {
-  using P = Tile<int8_t, BM, BN, 2, 2, true, true, false>;
+  using P = Tile<int8_t, BM, BN, 2, 2, true, true>;
   __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
   int8_workgroup<T, P, BM, BN>(p, lds);
 }
 
 // operands in whole chunks, pipelined
-template <class T, int BM, int BN> __global__ __launch_bounds__(pipe_threads(BM, 1), 2) void int8_gemm_pipe_kernel(Int8Args p) {
-  using P = PipeTile<int8_t, BM, BN, 2, pipe_waves_w(BM, 1), true, true>;
+template <class T, int BM, int BN> __global__ __launch_bounds__(tile_threads(BM, 1), 2) void int8_gemm_pipe_kernel(Int8Args p) {
+  using P = PipeTile<int8_t, BM, BN, 2, waves_w(BM, 1), true, true>;
   __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
   int8_workgroup<T, P, BM, BN>(p, lds);
 }
@@ -342,7 +347,7 @@ template <class T, int CUT> int run_int8(const Int8Args& p0, hipStream_t st) {
   if constexpr (CUT <= DIRECT32) return launch(what, int8_gemm_direct_kernel<T, B / 16>, grid, dim3(256), st, p);
   else if constexpr (CUT <= PLAIN128) return launch(what, int8_gemm_kernel<T, B, B>, grid, dim3(256), st, p);
   else if constexpr (CUT == PIPE256) return launch(what, int8_gemm_pipe256_kernel<T>, grid, dim3(512), st, p);
-  else return launch(what, int8_gemm_pipe_kernel<T, B, B>, grid, dim3(pipe_threads(B, 1)), st, p);
+  else return launch(what, int8_gemm_pipe_kernel<T, B, B>, grid, dim3(tile_threads(B, 1)), st, p);
 }
 
 template <class T> int run_int8_cut(const Int8Args& p, int cut, hipStream_t st) {
@@ -364,7 +369,7 @@ template <int SIZE> __global__ __launch_bounds__(256) void pack_kernel(PackJob a
   if (c >= p.ld_to) return;
   for (int64_t r = (int64_t)blockIdx.y * 4 + threadIdx.y; r < p.rows; r += (int64_t)gridDim.y * 4) {
     const T* from = static_cast<const T*>(p.from) + r / p.per * p.stride + r % p.per * p.ld + c;
-    *reinterpret_cast<uint4*>(static_cast<T*>(p.to) + r * p.ld_to + c) = load_chunk<T, false>(from, p.extent - c);
+    *reinterpret_cast<chunk_t*>(static_cast<T*>(p.to) + r * p.ld_to + c) = p.extent - c >= CHE<T> ? load_any(from) : load_few(from, p.extent - c);
   }
 }
 
@@ -432,7 +437,7 @@ extern "C" int64_t bgp_int8_gemm(int device, void* stream, int dtype, int64_t M,
   const int64_t to = padded_row(K, 1);
   const bool a_ok = reinterpret_cast<uintptr_t>(A) % 16 == 0 && lda % 16 == 0 && pipe_fits(lda, 1, true, 256);
   const bool b_ok = reinterpret_cast<uintptr_t>(B) % 16 == 0 && ldb % 16 == 0 && pipe_fits(ldb, 1, true, 256);
-  const Question q{1, true, a_ok && b_ok, true, false, (double)K, (a_ok ? 0.0 : (double)M * to) + (b_ok ? 0.0 : (double)N * to), (double)M * N, 1};
+  const Question q{1, K >= 16, a_ok && b_ok, true, false, (double)K, (a_ok ? 0.0 : (double)M * to) + (b_ok ? 0.0 : (double)N * to), (double)M * N, 1};
   const Plan plan = make_plan(q, [&](int b) { return (double)((M + b - 1) / b) * ((N + b - 1) / b); });
   Int8Args p{A, B, scale_a, scale_b, C, Y, M, N, K, lda, ldb, ldc, ldy, 0};
   Workspace ws(workspace);

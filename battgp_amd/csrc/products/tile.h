@@ -15,12 +15,18 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
+typedef double v2d __attribute__((ext_vector_type(2)));
 typedef double v4d __attribute__((ext_vector_type(4)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef int v4i __attribute__((ext_vector_type(4)));
 typedef short v4s __attribute__((ext_vector_type(4)));
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+
+typedef uint32_t chunk_t __attribute__((ext_vector_type(4)));  // 16 bytes, what every load and LDS access moves
+__device__ __forceinline__ chunk_t chunk_of(uint32_t a, uint32_t b, uint32_t c, uint32_t d) { return chunk_t{a, b, c, d}; }
 
 struct bf16_t { uint16_t v; };
 struct f16_t { uint16_t v; };
@@ -34,20 +40,16 @@ struct __attribute__((packed, aligned(A))) Chunk { uint32_t a, b, c, d; };
 template <class T> struct Num;
 template <> struct Num<double> {
   using acc = v4d;
-  static __device__ __forceinline__ acc mma(const uint4& a, const uint4& b, acc c) {
-    double x[2], y[2];
-    __builtin_memcpy(x, &a, 16);
-    __builtin_memcpy(y, &b, 16);
+  static __device__ __forceinline__ acc mma(const chunk_t& a, const chunk_t& b, acc c) {
+    const v2d x = __builtin_bit_cast(v2d, a), y = __builtin_bit_cast(v2d, b);
     c = __builtin_amdgcn_mfma_f64_16x16x4f64(x[0], y[0], c, 0, 0, 0);
     return __builtin_amdgcn_mfma_f64_16x16x4f64(x[1], y[1], c, 0, 0, 0);
   }
 };
 template <> struct Num<float> {
   using acc = v4f;
-  static __device__ __forceinline__ acc mma(const uint4& a, const uint4& b, acc c) {
-    float x[4], y[4];
-    __builtin_memcpy(x, &a, 16);
-    __builtin_memcpy(y, &b, 16);
+  static __device__ __forceinline__ acc mma(const chunk_t& a, const chunk_t& b, acc c) {
+    const v4f x = __builtin_bit_cast(v4f, a), y = __builtin_bit_cast(v4f, b);
 #pragma unroll
     for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], y[j], c, 0, 0, 0);
     return c;
@@ -55,28 +57,22 @@ template <> struct Num<float> {
 };
 template <> struct Num<bf16_t> {
   using acc = v4f;
-  static __device__ __forceinline__ acc mma(const uint4& a, const uint4& b, acc c) {
-    v8bf x, y;
-    __builtin_memcpy(&x, &a, 16);
-    __builtin_memcpy(&y, &b, 16);
+  static __device__ __forceinline__ acc mma(const chunk_t& a, const chunk_t& b, acc c) {
+    const v8bf x = __builtin_bit_cast(v8bf, a), y = __builtin_bit_cast(v8bf, b);
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, c, 0, 0, 0);
   }
 };
 template <> struct Num<f16_t> {
   using acc = v4f;
-  static __device__ __forceinline__ acc mma(const uint4& a, const uint4& b, acc c) {
-    v8h x, y;
-    __builtin_memcpy(&x, &a, 16);
-    __builtin_memcpy(&y, &b, 16);
+  static __device__ __forceinline__ acc mma(const chunk_t& a, const chunk_t& b, acc c) {
+    const v8h x = __builtin_bit_cast(v8h, a), y = __builtin_bit_cast(v8h, b);
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, c, 0, 0, 0);
   }
 };
 template <> struct Num<int8_t> {
   using acc = v4i;
-  static __device__ __forceinline__ acc mma(const uint4& a, const uint4& b, acc c) {
-    v4i x, y;
-    __builtin_memcpy(&x, &a, 16);
-    __builtin_memcpy(&y, &b, 16);
+  static __device__ __forceinline__ acc mma(const chunk_t& a, const chunk_t& b, acc c) {
+    const v4i x = __builtin_bit_cast(v4i, a), y = __builtin_bit_cast(v4i, b);
     return __builtin_amdgcn_mfma_i32_16x16x64_i8(x, y, c, 0, 0, 0);
   }
 };
@@ -102,11 +98,13 @@ template <> __device__ __forceinline__ f16_t round_to<f16_t, float>(float v) {
   return r;
 }
 
-// element (r, k) = p[r ld + k] (along k) or p[k ld + r] (along rows); rows: how many from p on may be read
+// element (r, k) = p[r ld + k] (along k) or p[k ld + r] (along rows); rows: how many from p on may be read; wide: the
+// matrix's rows (in memory) are 16 bytes long at least
 template <class T> struct Operand {
   const T* p;
   int64_t ld;
   int64_t rows;
+  bool wide;
 };
 
 template <class T> constexpr int CHE = 16 / (int)sizeof(T);        // elements in a chunk
@@ -120,22 +118,44 @@ template <class T, bool ALONG_K> __device__ __forceinline__ int swizzle(int row,
   return chunk;
 }
 
-// up to CHE elements (n of them exist, the others are 0)
-template <class T, bool VEC> __device__ __forceinline__ uint4 load_chunk(const T* p, int64_t n) {
-  uint4 v = make_uint4(0, 0, 0, 0);
-  if (n >= CHE<T>) {
-    if (VEC) return *reinterpret_cast<const uint4*>(p);
-    const Chunk<sizeof(T)> c = *reinterpret_cast<const Chunk<sizeof(T)>*>(p);
-    return make_uint4(c.a, c.b, c.c, c.d);
-  }
-  if (n > 0) {
-    T e[CHE<T>] = {};
+// a chunk at any alignment
+template <class T> __device__ __forceinline__ chunk_t load_any(const T* p) {
+  const Chunk<sizeof(T)> c = *reinterpret_cast<const Chunk<sizeof(T)>*>(p);
+  return chunk_of(c.a, c.b, c.c, c.d);
+}
+
+// the first n elements of a chunk, then zeros, one by one
+template <class T> __device__ __forceinline__ chunk_t load_few(const T* p, int64_t n) {
+  T e[CHE<T>] = {};
 #pragma unroll
-    for (int j = 0; j < CHE<T>; ++j)
-      if (j < n) e[j] = p[j];
-    __builtin_memcpy(&v, e, 16);
-  }
+  for (int j = 0; j < CHE<T>; ++j)
+    if (j < n) e[j] = p[j];
+  chunk_t v;
+  __builtin_memcpy(&v, e, 16);
   return v;
+}
+
+// The same without a branch, where the chunk that ends at p + n (0 < n < CHE) lies in the same row: it is loaded whole, and
+// later (`settle`: not before it is needed, so that many loads are in flight) moved down.  n <= 0: zeros, and `home`
+// is read instead.
+template <class T> __device__ __forceinline__ int kept(int64_t n) { return n >= CHE<T> ? CHE<T> : n > 0 ? (int)n : 0; }
+template <class T> __device__ __forceinline__ chunk_t load_edge(const T* p, int64_t n, const T* home) {
+  const int keep = kept<T>(n);
+  return load_any(keep ? p - (CHE<T> - keep) : home);
+}
+template <class T> __device__ __forceinline__ chunk_t settle(const chunk_t& c, int64_t n) {
+  const int keep = kept<T>(n);
+  uint64_t lo = (uint64_t)c.y << 32 | c.x, hi = (uint64_t)c.w << 32 | c.z;
+  int bits = (CHE<T> - keep) * 8 * (int)sizeof(T);
+  if (bits >= 64) {
+    lo = hi;
+    hi = 0;
+    bits -= 64;
+  }
+  lo = lo >> (bits & 63) | hi << 1 << (63 - (bits & 63));
+  hi >>= bits & 63;
+  if (!keep) lo = hi = 0;
+  return chunk_of((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
 }
 
 // a value that all lanes hold, in scalar registers
@@ -145,41 +165,79 @@ __device__ __forceinline__ int64_t scalar64(int64_t v) {
 }
 
 // one operand's share of a stage: ROWS x 128 bytes, fetched into registers by all NT threads, then stored to LDS
-template <class T, int ROWS, bool ALONG_K, bool VEC, int NT> struct Stage {
+template <class T, int ROWS, bool ALONG_K, int NT> struct Stage {
   static constexpr int CHUNKS = ROWS * 8, NL = CHUNKS / NT;
   static constexpr int CPR = ALONG_K ? 8 : ROWS / CHE<T>;  // chunks per LDS row
   static_assert(CHUNKS % NT == 0, "every thread loads the same number of chunks");
-  uint4 r[NL];
+  chunk_t r[NL];
 
-  __device__ __forceinline__ void fetch(const Operand<T>& o, int64_t k0, int64_t klen) {
-    if (k0 + KSTAGE<T> <= klen && o.rows >= ROWS) fetch_part<true>(o, k0, klen);  // without a branch per chunk
-    else fetch_part<false>(o, k0, klen);
-  }
-  template <bool WHOLE> __device__ __forceinline__ void fetch_part(const Operand<T>& o, int64_t k0, int64_t klen) {
+  // A stage of which all k exist.  EDGE: not all rows do; along k the last one is repeated (it only reaches elements of D
+  // that are not stored), along rows what does not exist is 0.
+  template <bool EDGE> __device__ __forceinline__ void fetch(const Operand<T>& o, int64_t k0) {
+    if (EDGE && !o.wide) return;
+    const int last = EDGE && o.rows < ROWS ? (int)o.rows - 1 : ROWS - 1;
 #pragma unroll
     for (int l = 0; l < NL; ++l) {
       const int i = threadIdx.x + l * NT, row = i / CPR, c = swizzle<T, ALONG_K>(row, i % CPR, CPR);
       if (ALONG_K) {
-        const int64_t k = k0 + c * CHE<T>;
-        r[l] = load_chunk<T, VEC>(o.p + row * o.ld + k, WHOLE ? CHE<T> : row < o.rows ? klen - k : 0);
+        r[l] = load_any(o.p + (EDGE && row > last ? last : row) * o.ld + k0 + c * CHE<T>);
       } else {
-        const int64_t k = k0 + row;
-        r[l] = load_chunk<T, VEC>(o.p + k * o.ld + c * CHE<T>, WHOLE ? CHE<T> : k < klen ? o.rows - c * CHE<T> : 0);
+        const T* p = o.p + (k0 + row) * o.ld + c * CHE<T>;
+        r[l] = EDGE ? load_edge(p, o.rows - c * CHE<T>, o.rows >= CHE<T> ? o.p : o.p + o.rows - CHE<T>) : load_any(p);
       }
     }
   }
-  __device__ __forceinline__ void store(char* lds) const {
+  template <bool EDGE> __device__ __forceinline__ void store(char* lds, const Operand<T>& o, int64_t k0) const {
+    if (EDGE && !o.wide) {
+      store_narrow(lds, o, k0, k0 + KSTAGE<T>);
+      return;
+    }
 #pragma unroll
-    for (int l = 0; l < NL; ++l) *reinterpret_cast<uint4*>(lds + (threadIdx.x + l * NT) * 16) = r[l];
+    for (int l = 0; l < NL; ++l) {
+      const int i = threadIdx.x + l * NT, row = i / CPR, c = swizzle<T, ALONG_K>(row, i % CPR, CPR);
+      *reinterpret_cast<chunk_t*>(lds + i * 16) = EDGE && !ALONG_K ? settle<T>(r[l], o.rows - c * CHE<T>) : r[l];
+    }
+  }
+
+  // the stage in which k ends
+  __device__ __forceinline__ void fetch_store_end(char* lds, const Operand<T>& o, int64_t k0, int64_t klen) {
+    if (!o.wide) {
+      store_narrow(lds, o, k0, klen);
+      return;
+    }
+    const int last = o.rows < ROWS ? (int)o.rows - 1 : ROWS - 1;
+    const T* home = ALONG_K || o.rows >= CHE<T> ? o.p : o.p + o.rows - CHE<T>;
+    if (ALONG_K && klen < CHE<T>) home -= CHE<T> - klen;  // a part of k that is not the first
+    auto exist = [&](int row, int c) { return ALONG_K ? klen - k0 - c * CHE<T> : k0 + row < klen ? o.rows - c * CHE<T> : 0; };
+#pragma unroll
+    for (int l = 0; l < NL; ++l) {
+      const int i = threadIdx.x + l * NT, row = i / CPR, c = swizzle<T, ALONG_K>(row, i % CPR, CPR);
+      r[l] = load_edge(ALONG_K ? o.p + (row < last ? row : last) * o.ld + k0 + c * CHE<T> : o.p + (k0 + row) * o.ld + c * CHE<T>, exist(row, c), home);
+    }
+#pragma unroll
+    for (int l = 0; l < NL; ++l) {
+      const int i = threadIdx.x + l * NT, row = i / CPR, c = swizzle<T, ALONG_K>(row, i % CPR, CPR);
+      *reinterpret_cast<chunk_t*>(lds + i * 16) = settle<T>(r[l], exist(row, c));
+    }
+  }
+
+  // rows of less than 16 bytes, element by element
+  static __device__ __forceinline__ void store_narrow(char* lds, const Operand<T>& o, int64_t k0, int64_t klen) {
+#pragma unroll 1
+    for (int i = threadIdx.x; i < CHUNKS; i += NT) {
+      const int row = i / CPR, c = swizzle<T, ALONG_K>(row, i % CPR, CPR);
+      const int64_t n = ALONG_K ? (row < o.rows ? klen - k0 - c * CHE<T> : 0) : (k0 + row < klen ? o.rows - c * CHE<T> : 0);
+      *reinterpret_cast<chunk_t*>(lds + i * 16) = load_few(ALONG_K ? o.p + row * o.ld + k0 + c * CHE<T> : o.p + (k0 + row) * o.ld + c * CHE<T>, n);
+    }
   }
 };
 
 // the 16 bytes of row r0 + lane % 16 that lane / 16 holds of half s of a stage
-template <class T, int ROWS, bool ALONG_K> __device__ __forceinline__ uint4 fragment(const char* lds, int r0, int s) {
+template <class T, int ROWS, bool ALONG_K> __device__ __forceinline__ chunk_t fragment(const char* lds, int r0, int s) {
   const int lane = threadIdx.x & 63, q = s * 4 + (lane >> 4), r = lane & 15;
-  uint4 v;
+  chunk_t v;
   if constexpr (ALONG_K) {
-    v = *reinterpret_cast<const uint4*>(lds + (r0 + r) * 128 + swizzle<T, true>(r0 + r, q, 8) * 16);
+    v = *reinterpret_cast<const chunk_t*>(lds + (r0 + r) * 128 + swizzle<T, true>(r0 + r, q, 8) * 16);
   } else {
     constexpr int CPR = ROWS / CHE<T>, LROW = CPR * 16;
     if constexpr (sizeof(T) == 2) {
@@ -204,9 +262,62 @@ template <class T, int ROWS, bool ALONG_K> __device__ __forceinline__ uint4 frag
   return v;
 }
 
+// Hands the wave's part of D out in units of E neighbours of a row, through LDS: a matrix instruction leaves 4 neighbours in
+// a lane, whose stores would touch 16 rows at 8 to 32 bytes each.  f(i, j, sums): X row i, W rows j .. j + E - 1; only
+// i < rows.  Each wave has a region of LDS to itself, whose operations happen in order: no barrier.  Rows are
+// handed out in a loop of few instructions: unrolled over the accumulators the same work was bound by fetching
+// its code (8192 x 2048 bf16 results: 13 us instead of 4).
+template <class T, int C, int E, int REGION, int FA, int FB, class ACC, class F>
+__device__ __forceinline__ void hand_out(const ACC (&acc)[FB][FA], char* mine, int x0, int w0, int64_t rows, F&& f) {
+  using S = typename std::remove_reference<decltype(acc[0][0][0] + acc[0][0][0])>::type;
+  constexpr int LROW = C * (int)sizeof(S), FIT = REGION / LROW / 16;                       // 16-row blocks in the region
+  constexpr int AT_ONCE = FIT >= FA ? FA : FIT >= 8 ? 8 : FIT >= 4 ? 4 : FIT >= 2 ? 2 : FIT;
+  static_assert(AT_ONCE >= 1 && FA % AT_ONCE == 0, "a wave's region holds whole blocks");
+  constexpr int UNITS = LROW / 16;  // 16-byte pieces of a row, swizzled by the row
+  const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+  auto place = [&](int row, int col) {
+    const int byte = col * (int)sizeof(S);
+    return mine + row * LROW + (((byte >> 4) ^ row) & (UNITS - 1)) * 16 + (byte & 15);
+  };
+#pragma unroll
+  for (int first = 0; first < FA; first += AT_ONCE) {
+    if (x0 + first * 16 >= rows) return;
+#pragma unroll
+    for (int a = 0; a < AT_ONCE; ++a)
+#pragma unroll
+      for (int b = 0; b < FB; ++b) {
+        if (sizeof(T) == 8) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) *reinterpret_cast<S*>(place(a * 16 + r, b * 16 + q + 4 * e)) = acc[b][first + a][e];
+        } else {
+          *reinterpret_cast<ACC*>(place(a * 16 + r, b * 16 + q * 4)) = acc[b][first + a];
+        }
+      }
+    __builtin_amdgcn_wave_barrier();
+    constexpr int PER_ROW = C / E;
+#pragma unroll 2
+    for (int u = lane; u < AT_ONCE * 16 * PER_ROW; u += 64) {
+      const int row = u / PER_ROW, j = u % PER_ROW * E;
+      S v[E];
+      if constexpr (E * sizeof(S) < 16) {
+        __builtin_memcpy(v, place(row, j), E * sizeof(S));
+      } else {
+#pragma unroll
+        for (int c = 0; c < (int)(E * sizeof(S) / 16); ++c) {
+          const chunk_t one = *reinterpret_cast<const chunk_t*>(place(row, j + c * 16 / (int)sizeof(S)));
+          __builtin_memcpy(reinterpret_cast<char*>(v) + c * 16, &one, 16);
+        }
+      }
+      const int i = x0 + first * 16 + row;
+      if (i < rows) f(i, w0 + j, v);
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
 // The workgroup's tile: WX x WW waves, each (BM / WX) x (BN / WW).  acc[b][a] is the 16 x 16 block of X rows 16 a and
 // W rows 16 b of the wave's part.
-template <class T, int BM, int BN, int WX, int WW, bool XK, bool WK, bool VEC> struct Tile {
+template <class T, int BM, int BN, int WX, int WW, bool XK, bool WK> struct Tile {
   static constexpr int NT = 64 * WX * WW, FA = BM / WX / 16, FB = BN / WW / 16;
   static constexpr int LDS_BYTES = 2 * (BM + BN) * 128;
   using acc_t = typename Num<T>::acc;
@@ -221,56 +332,62 @@ template <class T, int BM, int BN, int WX, int WW, bool XK, bool WK, bool VEC> s
 #pragma unroll
       for (int a = 0; a < FA; ++a) acc[b][a] = acc_t{};
     if (klen <= 0) return;
-    Stage<T, BM, XK, VEC, NT> sx;
-    Stage<T, BN, WK, VEC, NT> sw;
-    sx.fetch(x, 0, klen);
-    sw.fetch(w, 0, klen);
-    sx.store(lds);
-    sw.store(lds + BM * 128);
+    if (x.rows >= BM && w.rows >= BN && x.wide && w.wide) loop<false>(x, w, klen, lds);
+    else loop<true>(x, w, klen, lds);
+  }
+
+  // two buffers: while a stage is multiplied the next is fetched into registers.  If k ends inside a stage, that one
+  // comes first.
+  template <bool EDGE> __device__ __forceinline__ void loop(const Operand<T>& x, const Operand<T>& w, int64_t klen, char* lds) {
+    constexpr int BUF = (BM + BN) * 128;
+    Stage<T, BM, XK, NT> sx;
+    Stage<T, BN, WK, NT> sw;
+    const int whole = (int)(klen / KSTAGE<T>), stages = whole + (klen % KSTAGE<T> != 0);
+    if (stages > whole) {
+      sx.fetch_store_end(lds, x, (int64_t)whole * KSTAGE<T>, klen);
+      sw.fetch_store_end(lds + BM * 128, w, (int64_t)whole * KSTAGE<T>, klen);
+    } else {
+      sx.template fetch<EDGE>(x, 0);
+      sw.template fetch<EDGE>(w, 0);
+      sx.template store<EDGE>(lds, x, 0);
+      sw.template store<EDGE>(lds + BM * 128, w, 0);
+    }
+    int64_t k0 = stages > whole ? 0 : KSTAGE<T>;  // the next stage's
     __syncthreads();
-    int buf = 0;
-    for (int64_t k0 = 0; k0 < klen; k0 += KSTAGE<T>) {
-      const bool more = k0 + KSTAGE<T> < klen;
+    for (int s = 0; s < stages; ++s) {
+      const char *lx = lds + (s & 1) * BUF, *lw = lx + BM * 128;
+      char* next = lds + (~s & 1) * BUF;
+      const bool more = s + 1 < stages;
       if (more) {
-        sx.fetch(x, k0 + KSTAGE<T>, klen);
-        sw.fetch(w, k0 + KSTAGE<T>, klen);
+        sx.template fetch<EDGE>(x, k0);
+        sw.template fetch<EDGE>(w, k0);
       }
-      const char *lx = lds + buf * (BM + BN) * 128, *lw = lx + BM * 128;
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        uint4 fx[FA], fw[FB];
+      for (int h = 0; h < 2; ++h) {
+        chunk_t fx[FA], fw[FB];
 #pragma unroll
-        for (int a = 0; a < FA; ++a) fx[a] = fragment<T, BM, XK>(lx, x0() + a * 16, s);
+        for (int a = 0; a < FA; ++a) fx[a] = fragment<T, BM, XK>(lx, x0() + a * 16, h);
 #pragma unroll
-        for (int b = 0; b < FB; ++b) fw[b] = fragment<T, BN, WK>(lw, w0() + b * 16, s);
+        for (int b = 0; b < FB; ++b) fw[b] = fragment<T, BN, WK>(lw, w0() + b * 16, h);
 #pragma unroll
         for (int b = 0; b < FB; ++b)
 #pragma unroll
           for (int a = 0; a < FA; ++a) acc[b][a] = Num<T>::mma(fw[b], fx[a], acc[b][a]);
       }
-      buf ^= 1;
       if (more) {
-        sx.store(lds + buf * (BM + BN) * 128);
-        sw.store(lds + buf * (BM + BN) * 128 + BM * 128);
+        sx.template store<EDGE>(next, x, k0);
+        sw.template store<EDGE>(next + BM * 128, w, k0);
+        k0 += KSTAGE<T>;
       }
       __syncthreads();
     }
   }
 
-  // f(i, j, values, first, step): X row i, W rows j + first + step * e for e < 4
-  template <class F> __device__ __forceinline__ void each(F&& f) const {
-    const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
-#pragma unroll
-    for (int a = 0; a < FA; ++a)
-#pragma unroll
-      for (int b = 0; b < FB; ++b) {
-        if (sizeof(T) == 8) f(x0() + a * 16 + r, w0() + b * 16 + q, 4, acc[b][a]);
-        else f(x0() + a * 16 + r, w0() + b * 16 + q * 4, 1, acc[b][a]);
-      }
+  template <int E, class F> __device__ __forceinline__ void out(char* lds, int64_t rows, F&& f) const {
+    constexpr int C = BN / WW, REGION = LDS_BYTES / (WX * WW);
+    hand_out<T, C, E, REGION, FA, FB>(acc, lds + (threadIdx.x >> 6) * REGION, x0(), w0(), rows, f);
   }
 };
-
-__device__ __attribute__((aligned(16))) const uint4 zero_chunk = {0, 0, 0, 0};
 
 // The same tile for operands in whole aligned 16-byte chunks, as a pipeline: two buffers of a stage each, filled by loads
 // that write LDS themselves (global_load_lds, 16 bytes a lane: no registers, no LDS stores, one 32-bit offset per lane
@@ -316,9 +433,10 @@ template <class T, int BM, int BN, int WX, int WW, bool XK, bool WK> struct Pipe
       }
     }
     __device__ __forceinline__ void issue(uint32_t lds) {
+      const int64_t from = scalar64(reinterpret_cast<int64_t>(p));
 #pragma unroll
       for (int l = 0; l < L; ++l)
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds + l * NW * 1024), "v"(at[l]), "s"(p) : "memory");
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds + l * NW * 1024), "v"(at[l]), "s"(from) : "memory");
       p += step;
     }
   };
@@ -343,19 +461,17 @@ template <class T, int BM, int BN, int WX, int WW, bool XK, bool WK> struct Pipe
       sw.issue(base + buf * BUF + BM * 128);
     };
     if (tail) {
-      Stage<T, BM, XK, true, NT> tx;
-      Stage<T, BN, WK, true, NT> tw;
-      tx.fetch(x, whole, klen);
-      tw.fetch(w, whole, klen);
-      tx.store(lds);
-      tw.store(lds + BM * 128);
+      Stage<T, BM, XK, NT> tx;
+      Stage<T, BN, WK, NT> tw;
+      tx.fetch_store_end(lds, x, whole, klen);
+      tw.fetch_store_end(lds + BM * 128, w, whole, klen);
     } else {
       issue(0);
     }
     if (stages > 1) issue(1);
     if (stages > 1 && !tail) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(XL + WL) : "memory");
     else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    uint4 fx[2][FA], fw[2][FB];
+    chunk_t fx[2][FA], fw[2][FB];
     auto read = [&](int buf, int half) {
       const char* at = lds + buf * BUF;
 #pragma unroll
@@ -405,15 +521,9 @@ template <class T, int BM, int BN, int WX, int WW, bool XK, bool WK> struct Pipe
     }
   }
 
-  template <class F> __device__ __forceinline__ void each(F&& f) const {
-    const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
-#pragma unroll
-    for (int a = 0; a < FA; ++a)
-#pragma unroll
-      for (int b = 0; b < FB; ++b) {
-        if (sizeof(T) == 8) f(x0() + a * 16 + r, w0() + b * 16 + q, 4, acc[b][a]);
-        else f(x0() + a * 16 + r, w0() + b * 16 + q * 4, 1, acc[b][a]);
-      }
+  template <int E, class F> __device__ __forceinline__ void out(char* lds, int64_t rows, F&& f) const {
+    constexpr int C = BN / WW, REGION = LDS_BYTES / NW;
+    hand_out<T, C, E, REGION, FA, FB>(acc, lds + wave() * REGION, x0(), w0(), rows, f);
   }
 };
 
@@ -439,30 +549,45 @@ template <class T, int FA, int FB, bool XK, bool WK> struct DirectTile {
       ld = o.ld;
       p = ALONG_K ? o.p + row * o.ld + k : o.p + row + k * o.ld;
     }
-    __device__ __forceinline__ uint4 load(int64_t k) const {
+    __device__ __forceinline__ chunk_t load(int64_t k) const {
       if constexpr (ALONG_K) {
-        return load_chunk<T, false>(p + k, CHE<T>);
+        return load_any(p + k);
       } else {
         T e[CHE<T>];
 #pragma unroll
         for (int j = 0; j < CHE<T>; ++j) e[j] = p[(k + j) * ld];
-        uint4 v;
+        chunk_t v;
         __builtin_memcpy(&v, e, 16);
         return v;
       }
     }
-    __device__ __forceinline__ uint4 load_end(int64_t k, int64_t klen) const {
-      const int64_t left = klen - k - ((threadIdx.x & 63) >> 4) * CHE<T>;
+    // where k ends: loaded now, settled when it is multiplied
+    __device__ __forceinline__ chunk_t load_end(int64_t k, int64_t klen) const {
+      const int first = ((threadIdx.x & 63) >> 4) * CHE<T>;
+      const int64_t left = klen - k - first;
       if constexpr (ALONG_K) {
-        return load_chunk<T, false>(p + k, left);
+        return load_edge(p + k, left, p - first);
       } else {
         T e[CHE<T>] = {};
 #pragma unroll
-        for (int j = 0; j < CHE<T>; ++j)
-          if (j < left) e[j] = p[(k + j) * ld];
-        uint4 v;
+        for (int j = 0; j < CHE<T>; ++j) e[j] = p[((j < left ? k + j : -first)) * ld];  // past the end: row 0, settled to 0
+        chunk_t v;
         __builtin_memcpy(&v, e, 16);
         return v;
+      }
+    }
+    __device__ __forceinline__ chunk_t settle_end(const chunk_t& v, int64_t k, int64_t klen) const {
+      const int64_t left = klen - k - ((threadIdx.x & 63) >> 4) * CHE<T>;
+      if constexpr (ALONG_K) {
+        return settle<T>(v, left);
+      } else {
+        T e[CHE<T>];
+        __builtin_memcpy(e, &v, 16);
+#pragma unroll
+        for (int j = 0; j < CHE<T>; ++j) e[j] = j < left ? e[j] : (T)0;
+        chunk_t r;
+        __builtin_memcpy(&r, e, 16);
+        return r;
       }
     }
   };
@@ -472,7 +597,7 @@ template <class T, int FA, int FB, bool XK, bool WK> struct DirectTile {
     for (int b = 0; b < FB; ++b)
 #pragma unroll
       for (int a = 0; a < FA; ++a) acc[b][a] = acc_t{};
-    const int wave = threadIdx.x >> 6;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int64_t share = ((klen + KE - 1) / KE + NW - 1) / NW * KE, end = (wave + 1) * share < klen ? (wave + 1) * share : klen;
     int64_t k = wave * share;
     if (k < end) {
@@ -482,8 +607,8 @@ template <class T, int FA, int FB, bool XK, bool WK> struct DirectTile {
       for (int a = 0; a < FA; ++a) sx[a].start(x, a * 16);
 #pragma unroll
       for (int b = 0; b < FB; ++b) sw[b].start(w, b * 16);
+      chunk_t fx[2 * FLIGHT][FA], fw[2 * FLIGHT][FB];
       for (; k + FLIGHT * KE <= end; k += FLIGHT * KE) {
-        uint4 fx[2 * FLIGHT][FA], fw[2 * FLIGHT][FB];
 #pragma unroll
         for (int s = 0; s < 2 * FLIGHT; ++s) {
 #pragma unroll
@@ -498,17 +623,26 @@ template <class T, int FA, int FB, bool XK, bool WK> struct DirectTile {
 #pragma unroll
             for (int a = 0; a < FA; ++a) acc[b][a] = Num<T>::mma(fw[s][b], fx[s][a], acc[b][a]);
       }
-      for (; k < end; k += KE / 2) {
-        uint4 fx[FA], fw[FB];
 #pragma unroll
-        for (int b = 0; b < FB; ++b) fw[b] = sw[b].load_end(k, end);
+      for (int s = 0; s < 2 * FLIGHT; ++s)
+        if (k + s * (KE / 2) < end) {
 #pragma unroll
-        for (int a = 0; a < FA; ++a) fx[a] = sx[a].load_end(k, end);
+          for (int b = 0; b < FB; ++b) fw[s][b] = sw[b].load_end(k + s * (KE / 2), end);
 #pragma unroll
-        for (int b = 0; b < FB; ++b)
+          for (int a = 0; a < FA; ++a) fx[s][a] = sx[a].load_end(k + s * (KE / 2), end);
+        }
 #pragma unroll
-          for (int a = 0; a < FA; ++a) acc[b][a] = Num<T>::mma(fw[b], fx[a], acc[b][a]);
-      }
+      for (int s = 0; s < 2 * FLIGHT; ++s)
+        if (k + s * (KE / 2) < end) {
+#pragma unroll
+          for (int b = 0; b < FB; ++b) fw[s][b] = sw[b].settle_end(fw[s][b], k + s * (KE / 2), end);
+#pragma unroll
+          for (int a = 0; a < FA; ++a) fx[s][a] = sx[a].settle_end(fx[s][a], k + s * (KE / 2), end);
+#pragma unroll
+          for (int b = 0; b < FB; ++b)
+#pragma unroll
+            for (int a = 0; a < FA; ++a) acc[b][a] = Num<T>::mma(fw[s][b], fx[s][a], acc[b][a]);
+        }
     }
     acc_t* part = reinterpret_cast<acc_t*>(lds) + (threadIdx.x & 63);
 #pragma unroll
@@ -520,16 +654,31 @@ template <class T, int FA, int FB, bool XK, bool WK> struct DirectTile {
   }
   const acc_t* sums;
 
-  // every wave adds up and hands out its share of the 16 x 16 blocks
-  template <class F> __device__ __forceinline__ void each(F&& f) const {
+  // every wave adds up its share of the 16 x 16 blocks and hands it out
+  template <int E, class F> __device__ __forceinline__ void out(char* lds, int64_t rows, F&& f) const {
+    using S = typename std::remove_reference<decltype(acc[0][0][0] + acc[0][0][0])>::type;
     const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
     for (int i = threadIdx.x >> 6; i < FA * FB; i += NW) {
       acc_t v = sums[i * 64];
 #pragma unroll
       for (int w = 1; w < NW; ++w) v += sums[(w * FA * FB + i) * 64];
-      const int a = i % FA, b = i / FA;
-      if (sizeof(T) == 8) f(a * 16 + r, b * 16 + q, 4, v);
-      else f(a * 16 + r, b * 16 + q * 4, 1, v);
+      const int a = i % FA * 16 + r, b = i / FA * 16;
+      if (a < rows) {
+        // a lane's 4 sums: neighbours, or (fp64) every fourth column
+        if (sizeof(T) == 8) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const S one = v[e];
+            f.single(a, b + q + 4 * e, one);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const S one = v[e];
+            f.single(a, b + q * 4 + e, one);
+          }
+        }
+      }
     }
   }
 };
@@ -538,6 +687,31 @@ template <class T, int FA, int FB, bool XK, bool WK> struct DirectTile {
 inline bool pipe_fits(int64_t ld, int size, bool along_k, int rows) {
   return (along_k ? rows : 128 / size) * ld * size < (int64_t)1 << 32;
 }
+
+// D's rows as they are: E = 16 bytes of them at a time
+template <class O> struct PlainRows {
+  O* d;
+  int64_t ld, cols;
+  static constexpr int E = 16 / (int)sizeof(O);
+  template <class S> __device__ __forceinline__ void single(int i, int j, S v) const {
+    if (j < cols) d[i * ld + j] = round_to<O>(v);
+  }
+  template <class S> __device__ __forceinline__ void operator()(int i, int j, const S* v) const {
+    O e[E];
+#pragma unroll
+    for (int c = 0; c < E; ++c) e[c] = round_to<O>(v[c]);
+    O* to = d + i * ld + j;
+    if (j + E <= cols) {
+      Chunk<sizeof(O)> u;
+      __builtin_memcpy(&u, e, 16);
+      *reinterpret_cast<Chunk<sizeof(O)>*>(to) = u;
+    } else {
+#pragma unroll 1
+      for (int c = 0; c < E; ++c)
+        if (j + c < cols) to[c] = round_to<O>(v[c]);
+    }
+  }
+};
 
 // D[j .. j + 3 step] = values where they are inside n columns
 template <class T, class A> __device__ __forceinline__ void store_row(T* row, int64_t j, int step, const A& v, int64_t n) {
