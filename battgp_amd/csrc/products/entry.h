@@ -65,13 +65,19 @@ __device__ __forceinline__ int place_runs(int total) {
   const int run = (total + XCDS - 1) / XCDS, at = blockIdx.x / XCDS, i = blockIdx.x % XCDS * run + at;
   return at < run && i < total ? i : -1;
 }
+// Tiles of uneven length, the longest first: dealt to the XCDs 8 at a time, so that each has its share of the long ones.
+constexpr int DEALT = 8;
+__device__ __forceinline__ int deal(int i) {
+  constexpr int XCDS = 8;
+  const int at = i / XCDS;
+  return (at / DEALT * XCDS + i % XCDS) * DEALT + at % DEALT;
+}
 // inside a run 8 row tiles are gone through before the next column tile, so that workgroups that run together share rows
 // of both operands
 struct TileAt {
   int m, n;
 };
-__device__ __forceinline__ TileAt tile_at(int i, int tiles_m, int tiles_n) {
-  constexpr int DEEP = 8;
+template <int DEEP = 8> __device__ __forceinline__ TileAt tile_at(int i, int tiles_m, int tiles_n) {
   const int strip = i / (DEEP * tiles_n), in = i - strip * DEEP * tiles_n, deep = tiles_m - strip * DEEP < DEEP ? tiles_m - strip * DEEP : DEEP;
   return TileAt{strip * DEEP + in % deep, in / deep};
 }

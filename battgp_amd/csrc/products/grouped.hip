@@ -192,12 +192,30 @@ template <class T, class P> __device__ __forceinline__ void dw_tile(const Groupe
   }
 }
 
+// The group with the n-th most rows (up to 64 groups; more are taken as they come).  A tile's time is its group's rows:
+// with 2880 of 8192 rows in one of 16 groups the long tiles at the end of an XCD's run made it 207 us.
+__device__ __forceinline__ int group_by_length(const GroupedArgs& p, int n) {
+  if (p.G > 64) return n;
+  const int lane = threadIdx.x & 63;
+  int rows = -1;
+  if (lane < p.G) {
+    const int64_t a = clamp64(p.off[lane], 0, p.T), b = clamp64(p.off[lane + 1], a, p.T);
+    rows = (int)(b - a < INT32_MAX ? b - a : INT32_MAX);
+  }
+  int before = 0;  // groups that are longer, or as long and earlier
+  for (int j = 0; j < p.G; ++j) {
+    const int other = __builtin_amdgcn_readlane(rows, j);
+    before += other > rows || (other == rows && j < lane);
+  }
+  return __ffsll((unsigned long long)__ballot(lane < p.G && before == n)) - 1;
+}
+
 template <class T, class P, int BM, int BN> __device__ __forceinline__ void dw_workgroup(const GroupedArgs& p, char* lds) {
   const int tiles_k = (int)((p.K + BN - 1) / BN), tiles = p.tiles_n * tiles_k;
-  const int i = place_runs(tiles * p.G);
-  if (i < 0) return;
-  const TileAt at = tile_at(i % tiles, p.tiles_n, tiles_k);
-  dw_tile<T, P>(p, i / tiles, (int64_t)at.m * BM, (int64_t)at.n * BN, lds);
+  const int i = deal(blockIdx.x);
+  if (i >= tiles * p.G) return;
+  const TileAt at = tile_at<4>(i % tiles, p.tiles_n, tiles_k);
+  dw_tile<T, P>(p, group_by_length(p, i / tiles), (int64_t)at.m * BM, (int64_t)at.n * BN, lds);
 }
 
 template <class T, int BM, int BN> __global__ __launch_bounds__(tile_threads(BM, sizeof(T)), 2) void grouped_dw_kernel(GroupedArgs p) {
@@ -216,10 +234,11 @@ template <class T> __global__ __launch_bounds__(512, 2) void grouped_dw_pipe256_
   using P = PipeTile<T, 256, 256, 2, 4, false, false>;
   __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
   const int tiles_k = (int)((p.K + 255) / 256), tiles = p.tiles_n * tiles_k;
-  const Place place = place_256(tiles * p.G);
+  Place place = place_256(tiles * p.G);
   if (place.tile < 0) return;
-  const int g = place.tile / tiles;
-  const TileAt at = tile_at(place.tile % tiles, p.tiles_n, tiles_k);
+  if (place.parts == 1 && (int)blockIdx.x < tiles * p.G / CUS * CUS) place.tile = deal(blockIdx.x);
+  const int g = group_by_length(p, place.tile / tiles);
+  const TileAt at = tile_at<4>(place.tile % tiles, p.tiles_n, tiles_k);
   int64_t n0 = (int64_t)at.m * 256, k0 = (int64_t)at.n * 256;
   if (place.parts == 1) {
     dw_tile<T, P>(p, g, n0, k0, lds);
@@ -345,7 +364,7 @@ template <class T, int CUT> int run_dw(const GroupedArgs& p0, hipStream_t st) {
   constexpr int B = tile_of(CUT);
   GroupedArgs p = p0;
   p.tiles_n = (int)((p.N + B - 1) / B);
-  const int64_t tiles = (int64_t)p.G * p.tiles_n * ((p.K + B - 1) / B) + (B == 256 ? CUS : 7);
+  const int64_t tiles = (int64_t)p.G * p.tiles_n * ((p.K + B - 1) / B) + (B == 256 ? CUS : 8 * DEALT - 1);
   if (tiles > MAX_WORKGROUPS / 2) return bgp_products_fail(-1, "%s: %lld tiles are more than one launch holds", what, (long long)tiles);
   const dim3 grid((unsigned)tiles, p.split);
   if constexpr (CUT <= DIRECT32) return launch(what, grouped_dw_direct_kernel<T, B / 16>, grid, dim3(256), st, p);
@@ -401,7 +420,7 @@ extern "C" int64_t bgp_grouped_gemm(int device, void* stream, int dtype, int64_t
   Laid x(X, 1, 0, T, ldx, K, size, true), w(W, strideW ? G : 1, strideW, w_trans ? K : N, ldw, w_trans ? N : K, size, !w_trans);
   const bool wide = K * size >= 16 && (!w_trans || N * size >= 16);
   const Question q{size, wide && (!w_trans || size >= 4), x.ok && w.ok, pipe_fits(padded_row(x.extent, size), size, true, 256) && pipe_fits(padded_row(w.extent, size), size, !w_trans, 256),
-                   !w.along_k && !w.ok, (double)K, (double)(x.bytes(size) + w.bytes(size)), (double)T * N, G > 0 ? 16 : 1};
+                   (double)K, (double)(x.bytes(size) + w.bytes(size)), (double)T * N, G > 0 ? 16 : 1};
   const Plan plan = make_plan(q, [&](int b) { return expected_tiles(T, G, b) * ((N + b - 1) / b); });
   Workspace ws(workspace);
   PackJob jobs[2];
@@ -441,7 +460,7 @@ extern "C" int64_t bgp_grouped_gemm_dw(int device, void* stream, int dtype, int6
   // a group's rows are its length of k: their mean, and as much again for the longest of uneven ones
   const double used = (double)(G < T ? G : T > 0 ? T : 1);
   const Question q{size, size >= 4, x.ok && y.ok, pipe_fits(padded_row(N, size), size, false, 256) && pipe_fits(padded_row(K, size), size, false, 256),
-                   !x.ok || !y.ok, ceil(T / used), (double)(x.bytes(size) + y.bytes(size)), (double)G * N * K, 16};
+                   ceil(T / used), (double)(x.bytes(size) + y.bytes(size)), (double)G * N * K, 16};
   const Plan plan = make_plan(q, [&](int b) { return (double)G * ((N + b - 1) / b) * ((K + b - 1) / b); });
   Workspace ws(workspace);
   PackJob jobs[2];

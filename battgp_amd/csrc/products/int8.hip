@@ -437,7 +437,7 @@ extern "C" int64_t bgp_int8_gemm(int device, void* stream, int dtype, int64_t M,
   const int64_t to = padded_row(K, 1);
   const bool a_ok = reinterpret_cast<uintptr_t>(A) % 16 == 0 && lda % 16 == 0 && pipe_fits(lda, 1, true, 256);
   const bool b_ok = reinterpret_cast<uintptr_t>(B) % 16 == 0 && ldb % 16 == 0 && pipe_fits(ldb, 1, true, 256);
-  const Question q{1, K >= 16, a_ok && b_ok, true, false, (double)K, (a_ok ? 0.0 : (double)M * to) + (b_ok ? 0.0 : (double)N * to), (double)M * N, 1};
+  const Question q{1, K >= 16, a_ok && b_ok, true, (double)K, (a_ok ? 0.0 : (double)M * to) + (b_ok ? 0.0 : (double)N * to), (double)M * N, 1};
   const Plan plan = make_plan(q, [&](int b) { return (double)((M + b - 1) / b) * ((N + b - 1) / b); });
   Int8Args p{A, B, scale_a, scale_b, C, Y, M, N, K, lda, ldb, ldc, ldy, 0};
   Workspace ws(workspace);

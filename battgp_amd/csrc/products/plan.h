@@ -16,7 +16,7 @@ constexpr int kind_of(int size) { return size == 1 ? 0 : size == 2 ? 1 : size ==
 // from stage to stage of a tile that has its CU to itself.  {int8, 16 bits, fp32, fp64}, by Cut.  In TFLOP/s of the whole
 // chip the first row of e.g. PIPE128 is 2138, 925, 148 and 71, of DIRECT32 271, 190, 65 and 41; PLAIN* were measured
 // on operands that are not aligned, since the others are pipelined.
-constexpr float STAGE_US[4][CUTS] = {{0.115f, 0.247f, 0.43f, 1.05f, 0.187f, 0.50f, 1.68f},
+constexpr float STAGE_US[4][CUTS] = {{0.115f, 0.247f, 0.40f, 0.95f, 0.187f, 0.50f, 1.68f},
                                      {0.075f, 0.177f, 0.39f, 0.87f, 0.228f, 0.58f, 1.78f},
                                      {0.090f, 0.260f, 0.61f, 2.20f, 0.476f, 1.82f, 9e9f},
                                      {0.075f, 0.200f, 0.60f, 2.20f, 0.470f, 1.90f, 9e9f}};
@@ -26,8 +26,6 @@ constexpr float ALONE_US[4][CUTS] = {{0.12f, 0.22f, 0.52f, 1.0f, 0.30f, 0.62f, 1
                                      {0.10f, 0.23f, 0.88f, 2.5f, 0.59f, 1.95f, 9e9f}};
 constexpr float LAUNCH_US = 3.0f, PACK_US = 2.0f, COPY_BYTES_US = 3.5e6f;
 constexpr int CUS = 256;
-// an operand along rows that is not aligned: PLAIN128 takes 99 us instead of 59 with 16-bit types
-constexpr float ROWS_UNALIGNED = 1.6f;
 
 struct Plan {
   int cut = PLAIN64, split = 1;
@@ -39,7 +37,6 @@ struct Question {
   int size;                // of an element
   bool direct, pipe;       // which cuts the operands allow as they are
   bool packable;           // the pipelined ones after unaligned operands have been copied into aligned rows
-  bool rows_unaligned;     // an operand along rows is not aligned
   double k, pack_bytes;    // length of k; bytes of the operands that would be copied
   double outputs;          // elements of D
   int most_split;          // 1: k is not cut
@@ -62,7 +59,6 @@ template <class F> Plan make_plan(const Question& q, F&& tiles) {
       const double each = ceil(unit * split / CUS), deep = ceil(stages / split);
       double stage = each * STAGE_US[kind][cut];
       if (stage < ALONE_US[kind][cut]) stage = ALONE_US[kind][cut];
-      if (!pipe && cut > DIRECT32 && q.size == 2 && q.rows_unaligned) stage *= ROWS_UNALIGNED;
       double us = LAUNCH_US + deep * stage;
       if (split > 1) us += LAUNCH_US + (split + 1) * q.outputs * (q.size == 8 ? 8 : 4) / COPY_BYTES_US;
       if (pack) us += PACK_US + 2 * q.pack_bytes / COPY_BYTES_US;
