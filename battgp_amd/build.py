@@ -32,6 +32,11 @@ PRODUCTS_HEADERS = [os.path.join(PRODUCTS, h) for h in ("tile.h", "entry.h", "pl
 PRODUCTS_FLAGS = FLAGS + ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
+# _products_torch.so: what battgp_amd/products.py calls when nothing about a call is out of the ordinary (host code only)
+TORCH_CALLS = os.path.join(PRODUCTS, "torch_calls.cpp")
+LIB_TORCH_CALLS = os.path.join(HERE, "_products_torch.so")
+
+
 def _hipcc() -> str:
     for cand in (shutil.which("hipcc"), "/opt/rocm/bin/hipcc"):
         if cand and os.path.exists(cand):
@@ -60,7 +65,29 @@ def build_products(force: bool = False, verbose: bool = True) -> str:
     deps = [os.path.join(PRODUCTS, s) for s in PRODUCTS_SOURCES] + PRODUCTS_HEADERS + [os.path.abspath(__file__)]
     if force or not os.path.exists(LIB_PRODUCTS) or any(os.path.getmtime(d) > os.path.getmtime(LIB_PRODUCTS) for d in deps):
         _compile(PRODUCTS, PRODUCTS_SOURCES, PRODUCTS_FLAGS, ".o", LIB_PRODUCTS, verbose)
+    deps = [TORCH_CALLS, PRODUCTS_HEADERS[-1], os.path.abspath(__file__)]
+    if force or not os.path.exists(LIB_TORCH_CALLS) or any(os.path.getmtime(d) > os.path.getmtime(LIB_TORCH_CALLS) for d in deps):
+        _build_torch_calls(verbose)
     return LIB_PRODUCTS
+
+
+def _build_torch_calls(verbose):
+    import sysconfig
+
+    import torch
+
+    root = os.path.dirname(torch.__file__)
+    rocm = os.path.dirname(os.path.dirname(_hipcc()))
+    cmd = [
+        shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+        f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{sysconfig.get_paths()['include']}",
+        "-isystem", os.path.join(root, "include"), "-isystem", os.path.join(root, "include", "torch", "csrc", "api", "include"),
+        "-isystem", os.path.join(rocm, "include"), TORCH_CALLS, "-o", LIB_TORCH_CALLS, f"-L{os.path.join(root, 'lib')}", f"-L{HERE}",
+        "-l:libbattgp_products.so", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN",
+    ]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.check_call(cmd)
 
 
 def _compile(folder, sources, flags, suffix, lib, verbose):

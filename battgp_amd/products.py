@@ -4,7 +4,9 @@ products grouped by expert with ragged sizes, their gradients, and products in 8
 torch tensors on the GPU in and out, in fp64, fp32, bf16 and fp16.  Every function enqueues its kernels on the current
 torch stream of the tensors' device and returns without waiting for them; nothing is kept between calls, so the calls can
 be captured into a graph and come from several threads.  The kernels run in libbattgp_products.so
-(``include/battgp_products.h``); there is no fallback.  Like the engine's ``lml_grad``, gradients are calls of their own:
+(``include/battgp_products.h``); there is no fallback.  An ordinary call goes there by way of ``_products_torch``
+(``csrc/products/torch_calls.cpp``); whatever that does not take - an ``out``, a part of the gradients, a wrong argument - goes
+through the checks below.  Like the engine's ``lml_grad``, gradients are calls of their own:
 no function records an autograd graph, and inputs that ask for one are refused.
 """
 
@@ -15,33 +17,38 @@ import torch
 from . import _lib
 from .engine import EngineError
 
+_lib.load_products()  # first: the module below is linked against it
+try:
+    from . import _products_torch as _calls
+except ImportError as exc:
+    raise ImportError(f"battgp_amd/_products_torch.so can not be loaded ({exc}): build it with `python -m battgp_amd.build`") from exc
+
 DTYPES = {torch.float64: _lib.F64, torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 INT8_MAX_K = _lib.INT8_MAX_K
 MAX_GROUPS = _lib.MAX_GROUPS
 
 
 FIRST_DEVICE = 0  # torch's index of the first device there is a kernel for; the CPU's is below it
+_Tensor, _strided, _int64, _int8 = torch.Tensor, torch.strided, torch.int64, torch.int8  # looked up once: a call is a few us
 
 
-def _check(rc: int) -> None:
-    if rc != 0:
-        raise EngineError(_lib.load_products().bgp_products_last_error().decode())
-
-
-def _call(entry, like: torch.Tensor, *args) -> None:
+def _call(name: str, like: torch.Tensor, *args) -> None:
     """A C entry that may ask for a workspace: torch's allocator gives it, on the stream that the call uses."""
+    lib = _lib.load_products()
+    entry = getattr(lib, name)
     rc = entry(*args, None, 0)
     if rc > 0:
         work = like.new_empty(rc, dtype=torch.uint8)
         rc = entry(*args, work.data_ptr(), rc)
-    _check(rc)
+    if rc != 0:
+        raise EngineError(lib.bgp_products_last_error().decode())
 
 
 def _gpu_tensor(name: str, t, dim: int, device: int | None = None) -> int:
     """the index of the device that ``t`` is on (checks are written for the call that passes: they cost a call its time)"""
-    if not isinstance(t, torch.Tensor):
+    if not isinstance(t, _Tensor):
         raise TypeError(f"{name} is not a torch tensor")
-    if t.layout is not torch.strided:
+    if t.layout is not _strided:
         raise ValueError(f"{name} is not a dense tensor")
     if t.dim() != dim:
         raise ValueError(f"{name} has {t.dim()} dimensions, {dim} are wanted")
@@ -111,13 +118,13 @@ def _stream(device: int) -> int:
 
 def _offsets(offsets, groups: int, device: int) -> None:
     _gpu_tensor("offsets", offsets, 1, device)
-    if offsets.dtype is not torch.int64:
+    if offsets.dtype is not _int64:
         raise ValueError(f"offsets are {offsets.dtype}, int64 is wanted")
-    if offsets.shape[0] != groups + 1:
-        raise ValueError(f"{offsets.shape[0]} offsets for {groups} groups, {groups + 1} are wanted")
+    if offsets.numel() != groups + 1:
+        raise ValueError(f"{offsets.numel()} offsets for {groups} groups, {groups + 1} are wanted")
     if groups > MAX_GROUPS:
         raise ValueError(f"{groups} groups, at most {MAX_GROUPS} are possible")
-    if groups and offsets.stride(0) != 1:
+    if not offsets.is_contiguous():
         raise ValueError("offsets are not contiguous")
 
 
@@ -131,7 +138,7 @@ def _grouped(device, dtype, x, w, offsets, out, t, n, k, g):
         y = _output(out, "out", (t, n), x.dtype, device, (x, w, offsets))
         ldy = _rows("out", y, t, n)
     _call(
-        _lib.load_products().bgp_grouped_gemm, x, device, _stream(device), dtype, t, n, k, g, x.data_ptr(), ldx, w.data_ptr(), sw, ldw, trans,
+        "bgp_grouped_gemm", x, device, _stream(device), dtype, t, n, k, g, x.data_ptr(), ldx, w.data_ptr(), sw, ldw, trans,
         offsets.data_ptr(), y.data_ptr(), ldy, out is None,
     )
     return y
@@ -145,6 +152,10 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, out:
     [G + 1]`` int64 on the device, ascending, within ``[0, T]`` - they are never read on the host.  Groups may be empty.
     Rows in no group are 0 in a new output and left as they are in a given ``out``.  Sums are held in fp32 (fp64 for
     fp64) and rounded once."""
+    if out is None:
+        y = _calls.grouped(x, w, offsets)
+        if y is not None:
+            return y
     device = _gpu_tensor("x", x, 2)
     _gpu_tensor("w", w, 3, device)
     dtype = _float_type("x", x.dtype)
@@ -162,6 +173,10 @@ def grouped_matmul_grad(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, offs
     """Gradients of :func:`grouped_matmul` for ``dy [T, N]``: ``(dx [T, K], dw [G, N, K])``, ``None`` for one that is not
     needed.  ``dx`` is 0 in rows of no group, ``dw`` is 0 for an empty group; both are new and contiguous, and for shared
     weights (``expand``) ``dw`` still holds each group's own share."""
+    if need_dx and need_dw:
+        both = _calls.grouped_grad(dy, x, w, offsets)
+        if both is not None:
+            return both
     device = _gpu_tensor("x", x, 2)
     _gpu_tensor("dy", dy, 2, device)
     _gpu_tensor("w", w, 3, device)
@@ -180,7 +195,7 @@ def grouped_matmul_grad(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, offs
     if need_dw:
         dw = x.new_empty((g, n, k))
         _call(
-            _lib.load_products().bgp_grouped_gemm_dw, x, device, _stream(device), dtype, t, n, k, g, dy.data_ptr(), lddy, x.data_ptr(), ldx,
+            "bgp_grouped_gemm_dw", x, device, _stream(device), dtype, t, n, k, g, dy.data_ptr(), lddy, x.data_ptr(), ldx,
             offsets.data_ptr(), dw.data_ptr(), n * (k or 1), k or 1,
         )
     return dx, dw
@@ -197,6 +212,9 @@ def quantize_rows(x: torch.Tensor, pow2: bool = False, residual: bool = False):
     ``max |row| <= 127 p``; at least the smallest normal number.  ``q`` is rounded to the nearest, ties to even.
     ``rest = x - scale * q``, exact with ``pow2``: quantising it again gives the next slice of the row.  A row with an
     infinity or a NaN has that for its scale, and codes 0."""
+    made = _calls.quantize(x, pow2, residual)
+    if made is not None:
+        return made
     device = _gpu_tensor("x", x, 2)
     dtype = _float_type("x", x.dtype)
     m, k = x.shape
@@ -204,11 +222,20 @@ def quantize_rows(x: torch.Tensor, pow2: bool = False, residual: bool = False):
     q = x.new_empty((m, k), dtype=torch.int8)
     scale = x.new_empty(m, dtype=_scale_type(x.dtype))
     rest = x.new_empty((m, k)) if residual else None
-    _check(_lib.load_products().bgp_quantize_rows(
+    lib = _lib.load_products()
+    rc = lib.bgp_quantize_rows(
         device, _stream(device), dtype, m, k, x.data_ptr(), ldx, q.data_ptr(), k or 1, scale.data_ptr(), bool(pow2), rest.data_ptr() if residual else None,
         k or 1,
-    ))
+    )
+    if rc != 0:
+        raise EngineError(lib.bgp_products_last_error().decode())
     return (q, scale, rest) if residual else (q, scale)
+
+
+def _scale(name: str, s, rows: int, dtype, device: int) -> None:
+    _gpu_tensor(name, s, 1, device)
+    if s.dtype is not dtype or s.numel() != rows or not s.is_contiguous():
+        raise ValueError(f"{name}: {rows} contiguous values of {dtype} are wanted for this result")
 
 
 def int8_matmul(
@@ -220,10 +247,14 @@ def int8_matmul(
     ``a [M, K]`` and ``b [N, K]`` int8 with contiguous rows, ``K <= 131071`` (the sum is exact in 32 bits);
     scales fp64 for a fp64 result, else fp32; ``c`` and ``out`` of the result's type, ``out`` may be ``c`` itself.  The
     scaling and the sum with ``c`` are computed in fp64 and rounded once."""
+    if out is None:
+        y = _calls.int8(a, b, a_scale, b_scale, c, DTYPES.get(dtype, -1))
+        if y is not None:
+            return y
     device = _gpu_tensor("a", a, 2)
     _gpu_tensor("b", b, 2, device)
     code = _float_type("dtype", dtype)
-    if a.dtype is not torch.int8 or b.dtype is not torch.int8:
+    if a.dtype is not _int8 or b.dtype is not _int8:
         raise ValueError(f"a is {a.dtype}, b is {b.dtype}: int8 is wanted")
     m, k = a.shape
     n, bk = b.shape
@@ -231,10 +262,9 @@ def int8_matmul(
         raise ValueError(f"a has {k} columns, b has {bk}")
     if k > INT8_MAX_K:
         raise ValueError(f"{k} columns: a sum over more than {INT8_MAX_K} can pass 32 bits")
-    for name, s, rows in (("a_scale", a_scale, m), ("b_scale", b_scale, n)):
-        _gpu_tensor(name, s, 1, device)
-        if s.dtype is not _scale_type(dtype) or s.shape[0] != rows or (rows > 1 and s.stride(0) != 1):
-            raise ValueError(f"{name}: {rows} contiguous values of {_scale_type(dtype)} are wanted for a result in {dtype}")
+    stype = _scale_type(dtype)
+    _scale("a_scale", a_scale, m, stype, device)
+    _scale("b_scale", b_scale, n, stype, device)
     cp, ldc = None, 0
     if c is not None:
         _gpu_tensor("c", c, 2, device)
@@ -251,7 +281,7 @@ def int8_matmul(
         y = _output(out, "out", (m, n), dtype, device, inputs)
         ldy = _rows("out", y, m, n)
     _call(
-        _lib.load_products().bgp_int8_gemm, a, device, _stream(device), code, m, n, k, a.data_ptr(), lda, b.data_ptr(), ldb, a_scale.data_ptr(),
+        "bgp_int8_gemm", a, device, _stream(device), code, m, n, k, a.data_ptr(), lda, b.data_ptr(), ldb, a_scale.data_ptr(),
         b_scale.data_ptr(), cp, ldc, y.data_ptr(), ldy,
     )
     return y
