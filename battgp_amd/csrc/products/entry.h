@@ -95,6 +95,11 @@ struct PackJob {
 int launch_pack(const char* what, int size, const PackJob* jobs, int count, hipStream_t st);
 constexpr int64_t padded_row(int64_t extent, int size) { return (extent * size + 127) / 128 * 128 / size; }
 
+// whether rows start off the 4-byte words
+inline bool off_words(const void* p, int64_t ld, int64_t stride, int size) {
+  return (reinterpret_cast<uintptr_t>(p) | (uintptr_t)(ld * size) | (uintptr_t)(stride * size)) % 4 != 0;
+}
+
 // Takes pieces of the workspace, or only adds up what they come to.
 class Workspace {
   char* at_;

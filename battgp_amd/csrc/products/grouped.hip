@@ -168,8 +168,8 @@ template <class T, bool WK> __global__ __launch_bounds__(512, 2) void grouped_ro
 }
 
 // small ones, straight from memory
-template <class T, int F, bool WK> __global__ __launch_bounds__(256) void grouped_rows_direct_kernel(GroupedArgs p) {
-  using P = DirectTile<T, F, F, true, WK>;
+template <class T, int F, bool WK, bool ODD> __global__ __launch_bounds__(256) void grouped_rows_direct_kernel(GroupedArgs p) {
+  using P = DirectTile<T, F, F, true, WK, ODD>;
   __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
   rows_workgroup<T, P, 16 * F, 16 * F, WK>(p, lds);
 }
@@ -193,29 +193,45 @@ template <class T, class P> __device__ __forceinline__ void dw_tile(const Groupe
 }
 
 // The group with the n-th most rows (up to 64 groups; more are taken as they come).  A tile's time is its group's rows:
-// with 2880 of 8192 rows in one of 16 groups the long tiles at the end of an XCD's run made it 207 us.
+// with 2880 of 8192 rows in one of 16 groups the long tiles at the end of an XCD's run made it 207 us.  Where groups are
+// short on average the order matters less than the 0.5 us that finding it takes.
 __device__ __forceinline__ int group_by_length(const GroupedArgs& p, int n) {
-  if (p.G > 64) return n;
+  if (p.G > 64 || p.T < 256 * (int64_t)p.G) return n;
   const int lane = threadIdx.x & 63;
-  int rows = -1;
+  int key = -1;  // rows (2^25 and more are alike), then the earlier group
   if (lane < p.G) {
-    const int64_t a = clamp64(p.off[lane], 0, p.T), b = clamp64(p.off[lane + 1], a, p.T);
-    rows = (int)(b - a < INT32_MAX ? b - a : INT32_MAX);
+    const int64_t a = clamp64(p.off[lane], 0, p.T), rows = clamp64(p.off[lane + 1], a, p.T) - a;
+    key = (int)(rows < 33554431 ? rows : 33554431) << 6 | (63 - lane);
   }
-  int before = 0;  // groups that are longer, or as long and earlier
-  for (int j = 0; j < p.G; ++j) {
-    const int other = __builtin_amdgcn_readlane(rows, j);
-    before += other > rows || (other == rows && j < lane);
-  }
+  int before = 0;
+  for (int j = 0; j < p.G; ++j) before += __builtin_amdgcn_readlane(key, j) > key;
   return __ffsll((unsigned long long)__ballot(lane < p.G && before == n)) - 1;
+}
+
+// A group without rows: its zeros, where they lie in one piece, as one of `parts` shares of it.  True if that was it.
+template <class T> __device__ __forceinline__ bool dw_empty(const GroupedArgs& p, int g, int part, int parts) {
+  const int64_t a = clamp64(p.off[g], 0, p.T), total = p.N * p.K;
+  if (clamp64(p.off[g + 1], a, p.T) > a || p.split > 1 || p.ldw != p.K) return false;
+  const int64_t share = ((total + parts - 1) / parts + 63) / 64 * 64, from = part * share, to = from + share < total ? from + share : total;
+  T* d = static_cast<T*>(const_cast<void*>(p.w)) + g * p.sw;
+  const int64_t lead = from + (16 - reinterpret_cast<uintptr_t>(d + from) % 16) % 16 / sizeof(T);  // the first whole 16 bytes
+  for (int64_t i = lead + (int64_t)threadIdx.x * CHE<T>; i + CHE<T> <= to; i += (int64_t)blockDim.x * CHE<T>) *reinterpret_cast<chunk_t*>(d + i) = chunk_of(0, 0, 0, 0);
+  if (threadIdx.x < CHE<T>) {
+    const int64_t i = from + threadIdx.x, j = (to - lead) / CHE<T> * CHE<T> + lead + threadIdx.x;
+    if (i < lead && i < to) d[i] = T{};
+    if (lead <= to && j < to) d[j] = T{};
+  }
+  return true;
 }
 
 template <class T, class P, int BM, int BN> __device__ __forceinline__ void dw_workgroup(const GroupedArgs& p, char* lds) {
   const int tiles_k = (int)((p.K + BN - 1) / BN), tiles = p.tiles_n * tiles_k;
   const int i = deal(blockIdx.x);
   if (i >= tiles * p.G) return;
+  const int g = group_by_length(p, i / tiles);
+  if (dw_empty<T>(p, g, i % tiles, tiles)) return;
   const TileAt at = tile_at<4>(i % tiles, p.tiles_n, tiles_k);
-  dw_tile<T, P>(p, group_by_length(p, i / tiles), (int64_t)at.m * BM, (int64_t)at.n * BN, lds);
+  dw_tile<T, P>(p, g, (int64_t)at.m * BM, (int64_t)at.n * BN, lds);
 }
 
 template <class T, int BM, int BN> __global__ __launch_bounds__(tile_threads(BM, sizeof(T)), 2) void grouped_dw_kernel(GroupedArgs p) {
@@ -238,6 +254,11 @@ template <class T> __global__ __launch_bounds__(512, 2) void grouped_dw_pipe256_
   if (place.tile < 0) return;
   if (place.parts == 1 && (int)blockIdx.x < tiles * p.G / CUS * CUS) place.tile = deal(blockIdx.x);
   const int g = group_by_length(p, place.tile / tiles);
+  if (dw_empty<T>(p, g, place.tile % tiles * 4 + place.part, tiles * 4)) {  // in quarters: all four of a whole tile
+    if (place.parts < 4)
+      for (int q = place.parts; q < 4; q += place.parts) dw_empty<T>(p, g, place.tile % tiles * 4 + q + place.part, tiles * 4);
+    return;
+  }
   const TileAt at = tile_at<4>(place.tile % tiles, p.tiles_n, tiles_k);
   int64_t n0 = (int64_t)at.m * 256, k0 = (int64_t)at.n * 256;
   if (place.parts == 1) {
@@ -252,7 +273,7 @@ template <class T> __global__ __launch_bounds__(512, 2) void grouped_dw_pipe256_
 }
 
 template <class T, int F> __global__ __launch_bounds__(256) void grouped_dw_direct_kernel(GroupedArgs p) {
-  using P = DirectTile<T, F, F, false, false>;
+  using P = DirectTile<T, F, F, false, false, false>;
   __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
   dw_workgroup<T, P, 16 * F, 16 * F>(p, lds);
 }
@@ -335,10 +356,18 @@ template <class T, bool WK, int CUT> int run_rows(const GroupedArgs& p0, hipStre
   const int64_t tiles = (p.T / B + p.G + (p.rest ? 2 : 0)) * p.tiles_n + (B == 256 ? CUS : 7);
   if (tiles > MAX_WORKGROUPS / 2) return bgp_products_fail(-1, "%s: %lld tiles are more than one launch holds", what, (long long)tiles);
   const dim3 grid((unsigned)tiles, p.split);
-  if constexpr (CUT <= DIRECT32) return launch(what, grouped_rows_direct_kernel<T, B / 16, WK>, grid, dim3(256), st, p);
-  else if constexpr (CUT <= PLAIN128) return launch(what, grouped_rows_kernel<T, B, B, WK>, grid, dim3(tile_threads(B, sizeof(T))), st, p);
-  else if constexpr (CUT == PIPE256) return launch(what, grouped_rows_pipe256_kernel<T, WK>, grid, dim3(512), st, p);
-  else return launch(what, grouped_rows_pipe_kernel<T, B, B, WK>, grid, dim3(tile_threads(B, sizeof(T))), st, p);
+  if constexpr (CUT <= DIRECT32) {
+    if constexpr (sizeof(T) < 4)
+      if (off_words(p.x, p.ldx, 0, sizeof(T)) || off_words(p.w, p.ldw, p.sw, sizeof(T)))
+        return launch(what, grouped_rows_direct_kernel<T, B / 16, WK, true>, grid, dim3(256), st, p);
+    return launch(what, grouped_rows_direct_kernel<T, B / 16, WK, false>, grid, dim3(256), st, p);
+  } else if constexpr (CUT <= PLAIN128) {
+    return launch(what, grouped_rows_kernel<T, B, B, WK>, grid, dim3(tile_threads(B, sizeof(T))), st, p);
+  } else if constexpr (CUT == PIPE256) {
+    return launch(what, grouped_rows_pipe256_kernel<T, WK>, grid, dim3(512), st, p);
+  } else {
+    return launch(what, grouped_rows_pipe_kernel<T, B, B, WK>, grid, dim3(tile_threads(B, sizeof(T))), st, p);
+  }
 }
 
 template <class T, bool WK> int rows_by_cut(const GroupedArgs& p, int cut, hipStream_t st) {

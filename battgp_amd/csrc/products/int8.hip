@@ -217,12 +217,13 @@ template <class T, bool POW2, int TPR, int U, bool LONG> __global__ __launch_bou
 
 template <class T, bool POW2> int quantize_by_length(const QuantArgs& p, hipStream_t st) {
   const char* what = "bgp_quantize_rows";
-  // a wave per row up to 2048 elements, a workgroup of 4 waves up to 8192, of 16 beyond
-  const int rows = p.K <= 2048 ? 4 : 1;
-  const int64_t groups = (p.M + rows - 1) / rows;
+  // a wave per row up to 2048 elements where there are rows enough for every CU, else a workgroup of 4 waves up to 8192, of
+  // 16 beyond
+  const bool wave = p.K <= 2048 && p.M >= 4 * CUS;
+  const int64_t groups = wave ? (p.M + 3) / 4 : p.M;
   if (groups > MAX_WORKGROUPS / 4) return bgp_products_fail(-1, "%s: %lld rows are more than one launch holds", what, (long long)p.M);
   const dim3 grid((unsigned)groups);
-  if (p.K <= 2048) return launch(what, quantize_rows_kernel<T, POW2, 64, 4, false>, grid, dim3(256), st, p);
+  if (wave) return launch(what, quantize_rows_kernel<T, POW2, 64, 4, false>, grid, dim3(256), st, p);
   if (p.K <= 8192) return launch(what, quantize_rows_kernel<T, POW2, 256, 4, false>, grid, dim3(256), st, p);
   return launch(what, quantize_rows_kernel<T, POW2, 1024, 4, true>, grid, dim3(1024), st, p);
 }
@@ -330,8 +331,8 @@ template <class T, int BM, int BN> __global__ __launch_bounds__(tile_threads(BM,
 }
 
 // small ones, straight from memory
-template <class T, int F> __global__ __launch_bounds__(256) void int8_gemm_direct_kernel(Int8Args p) {
-  using P = DirectTile<int8_t, F, F, true, true>;
+template <class T, int F, bool ODD> __global__ __launch_bounds__(256) void int8_gemm_direct_kernel(Int8Args p) {
+  using P = DirectTile<int8_t, F, F, true, true, ODD>;
   __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
   int8_workgroup<T, P, 16 * F, 16 * F>(p, lds);
 }
@@ -344,10 +345,17 @@ template <class T, int CUT> int run_int8(const Int8Args& p0, hipStream_t st) {
   const int64_t tiles = (p.M + B - 1) / B * p.tiles_n + (B == 256 ? CUS : 7);
   if (tiles > MAX_WORKGROUPS / 2) return bgp_products_fail(-1, "%s: %lld tiles are more than one launch holds", what, (long long)tiles);
   const dim3 grid((unsigned)tiles);
-  if constexpr (CUT <= DIRECT32) return launch(what, int8_gemm_direct_kernel<T, B / 16>, grid, dim3(256), st, p);
-  else if constexpr (CUT <= PLAIN128) return launch(what, int8_gemm_kernel<T, B, B>, grid, dim3(256), st, p);
-  else if constexpr (CUT == PIPE256) return launch(what, int8_gemm_pipe256_kernel<T>, grid, dim3(512), st, p);
-  else return launch(what, int8_gemm_pipe_kernel<T, B, B>, grid, dim3(tile_threads(B, 1)), st, p);
+  if constexpr (CUT <= DIRECT32) {
+    if (off_words(p.a, p.lda, 0, 1) || off_words(p.b, p.ldb, 0, 1))
+      return launch(what, int8_gemm_direct_kernel<T, B / 16, true>, grid, dim3(256), st, p);
+    return launch(what, int8_gemm_direct_kernel<T, B / 16, false>, grid, dim3(256), st, p);
+  } else if constexpr (CUT <= PLAIN128) {
+    return launch(what, int8_gemm_kernel<T, B, B>, grid, dim3(256), st, p);
+  } else if constexpr (CUT == PIPE256) {
+    return launch(what, int8_gemm_pipe256_kernel<T>, grid, dim3(512), st, p);
+  } else {
+    return launch(what, int8_gemm_pipe_kernel<T, B, B>, grid, dim3(tile_threads(B, 1)), st, p);
+  }
 }
 
 template <class T> int run_int8_cut(const Int8Args& p, int cut, hipStream_t st) {

@@ -118,11 +118,35 @@ template <class T, bool ALONG_K> __device__ __forceinline__ int swizzle(int row,
   return chunk;
 }
 
-// a chunk at any alignment
-template <class T> __device__ __forceinline__ chunk_t load_any(const T* p) {
-  const Chunk<sizeof(T)> c = *reinterpret_cast<const Chunk<sizeof(T)>*>(p);
-  return chunk_of(c.a, c.b, c.c, c.d);
-}
+// A chunk at any alignment, as it is loaded and as it is used.  Loads of 16 bytes are as fast at any multiple of 4 but take
+// up to three times as long off it, which a tile straight from memory waits for (a product of 707 x 144 x 6467 8-bit
+// integers: 35 us, of 6464: 12).  ODD: such a chunk is loaded from the word that its first element lies in, with
+// the word behind, and moved down when it is used (21 us; but 23 for the 6464).  Words that hold no element of it are
+// not touched.
+template <class T, bool ODD = false> struct Piece {
+  chunk_t c;
+  static __device__ __forceinline__ Piece load(const T* p) {
+    const Chunk<sizeof(T)> c = *reinterpret_cast<const Chunk<sizeof(T)>*>(p);
+    return Piece{chunk_of(c.a, c.b, c.c, c.d)};
+  }
+  __device__ __forceinline__ chunk_t value() const { return c; }
+};
+template <class T> struct Piece<T, true> {
+  chunk_t c;
+  uint32_t next, off;
+  static __device__ __forceinline__ Piece load(const T* p) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+    const uint32_t off = (uint32_t)at & 3;
+    const char* word = reinterpret_cast<const char*>(at - off);
+    const Chunk<4> c = *reinterpret_cast<const Chunk<4>*>(word);
+    return Piece{chunk_of(c.a, c.b, c.c, c.d), *reinterpret_cast<const uint32_t*>(word + (off ? 16 : 12)), off};
+  }
+  __device__ __forceinline__ chunk_t value() const {
+    return chunk_of(__builtin_amdgcn_alignbyte(c.y, c.x, off), __builtin_amdgcn_alignbyte(c.z, c.y, off), __builtin_amdgcn_alignbyte(c.w, c.z, off),
+                    __builtin_amdgcn_alignbyte(next, c.w, off));
+  }
+};
+template <class T> __device__ __forceinline__ chunk_t load_any(const T* p) { return Piece<T>::load(p).value(); }
 
 // the first n elements of a chunk, then zeros, one by one
 template <class T> __device__ __forceinline__ chunk_t load_few(const T* p, int64_t n) {
@@ -139,12 +163,13 @@ template <class T> __device__ __forceinline__ chunk_t load_few(const T* p, int64
 // later (`settle`: not before it is needed, so that many loads are in flight) moved down.  n <= 0: zeros, and `home`
 // is read instead.
 template <class T> __device__ __forceinline__ int kept(int64_t n) { return n >= CHE<T> ? CHE<T> : n > 0 ? (int)n : 0; }
-template <class T> __device__ __forceinline__ chunk_t load_edge(const T* p, int64_t n, const T* home) {
+template <class T, bool ODD = false> __device__ __forceinline__ Piece<T, ODD> load_edge(const T* p, int64_t n, const T* home) {
   const int keep = kept<T>(n);
-  return load_any(keep ? p - (CHE<T> - keep) : home);
+  return Piece<T, ODD>::load(keep ? p - (CHE<T> - keep) : home);
 }
-template <class T> __device__ __forceinline__ chunk_t settle(const chunk_t& c, int64_t n) {
+template <class T, bool ODD> __device__ __forceinline__ chunk_t settle(const Piece<T, ODD>& piece, int64_t n) {
   const int keep = kept<T>(n);
+  const chunk_t c = piece.value();
   uint64_t lo = (uint64_t)c.y << 32 | c.x, hi = (uint64_t)c.w << 32 | c.z;
   int bits = (CHE<T> - keep) * 8 * (int)sizeof(T);
   if (bits >= 64) {
@@ -169,7 +194,7 @@ template <class T, int ROWS, bool ALONG_K, int NT> struct Stage {
   static constexpr int CHUNKS = ROWS * 8, NL = CHUNKS / NT;
   static constexpr int CPR = ALONG_K ? 8 : ROWS / CHE<T>;  // chunks per LDS row
   static_assert(CHUNKS % NT == 0, "every thread loads the same number of chunks");
-  chunk_t r[NL];
+  Piece<T> r[NL];
 
   // A stage of which all k exist.  EDGE: not all rows do; along k the last one is repeated (it only reaches elements of D
   // that are not stored), along rows what does not exist is 0.
@@ -180,10 +205,10 @@ template <class T, int ROWS, bool ALONG_K, int NT> struct Stage {
     for (int l = 0; l < NL; ++l) {
       const int i = threadIdx.x + l * NT, row = i / CPR, c = swizzle<T, ALONG_K>(row, i % CPR, CPR);
       if (ALONG_K) {
-        r[l] = load_any(o.p + (EDGE && row > last ? last : row) * o.ld + k0 + c * CHE<T>);
+        r[l] = Piece<T>::load(o.p + (EDGE && row > last ? last : row) * o.ld + k0 + c * CHE<T>);
       } else {
         const T* p = o.p + (k0 + row) * o.ld + c * CHE<T>;
-        r[l] = EDGE ? load_edge(p, o.rows - c * CHE<T>, o.rows >= CHE<T> ? o.p : o.p + o.rows - CHE<T>) : load_any(p);
+        r[l] = EDGE ? load_edge(p, o.rows - c * CHE<T>, o.rows >= CHE<T> ? o.p : o.p + o.rows - CHE<T>) : Piece<T>::load(p);
       }
     }
   }
@@ -195,7 +220,7 @@ template <class T, int ROWS, bool ALONG_K, int NT> struct Stage {
 #pragma unroll
     for (int l = 0; l < NL; ++l) {
       const int i = threadIdx.x + l * NT, row = i / CPR, c = swizzle<T, ALONG_K>(row, i % CPR, CPR);
-      *reinterpret_cast<chunk_t*>(lds + i * 16) = EDGE && !ALONG_K ? settle<T>(r[l], o.rows - c * CHE<T>) : r[l];
+      *reinterpret_cast<chunk_t*>(lds + i * 16) = EDGE && !ALONG_K ? settle(r[l], o.rows - c * CHE<T>) : r[l].value();
     }
   }
 
@@ -217,7 +242,7 @@ template <class T, int ROWS, bool ALONG_K, int NT> struct Stage {
 #pragma unroll
     for (int l = 0; l < NL; ++l) {
       const int i = threadIdx.x + l * NT, row = i / CPR, c = swizzle<T, ALONG_K>(row, i % CPR, CPR);
-      *reinterpret_cast<chunk_t*>(lds + i * 16) = settle<T>(r[l], exist(row, c));
+      *reinterpret_cast<chunk_t*>(lds + i * 16) = settle(r[l], exist(row, c));
     }
   }
 
@@ -528,10 +553,10 @@ template <class T, int BM, int BN, int WX, int WW, bool XK, bool WK> struct Pipe
 };
 
 // The tile for small problems, where a wait for every stage costs more than what is multiplied: 16 FA x 16 FB elements of D
-// by 4 waves that split k between them and add up in LDS at the end.  Fragments come straight from memory, several
-// in flight, without a barrier; operands of any alignment.  Along rows the elements are gathered one by one, which
+// by 4 waves that split k between them (8 were no faster) and add up in LDS at the end.  Fragments come straight from memory, several
+// in flight, without a barrier; operands of any alignment (ODD: not of 4 bytes).  Along rows the elements are gathered one by one, which
 // suits 32- and 64-bit types (16 lanes read 64 or 128 consecutive bytes).
-template <class T, int FA, int FB, bool XK, bool WK> struct DirectTile {
+template <class T, int FA, int FB, bool XK, bool WK, bool ODD> struct DirectTile {
   static constexpr int NW = 4, BM = 16 * FA, BN = 16 * FB;
   static constexpr int KE = KSTAGE<T>, FLIGHT = FA * FB == 1 ? 4 : 2;  // stages of 128 bytes of k whose loads are in flight
   using acc_t = typename Num<T>::acc;
@@ -549,46 +574,45 @@ template <class T, int FA, int FB, bool XK, bool WK> struct DirectTile {
       ld = o.ld;
       p = ALONG_K ? o.p + row * o.ld + k : o.p + row + k * o.ld;
     }
-    __device__ __forceinline__ chunk_t load(int64_t k) const {
+    __device__ __forceinline__ Piece<T, ODD> load(int64_t k) const {
       if constexpr (ALONG_K) {
-        return load_any(p + k);
+        return Piece<T, ODD>::load(p + k);
       } else {
         T e[CHE<T>];
 #pragma unroll
         for (int j = 0; j < CHE<T>; ++j) e[j] = p[(k + j) * ld];
-        chunk_t v;
-        __builtin_memcpy(&v, e, 16);
-        return v;
+        return gathered(e);
       }
     }
     // where k ends: loaded now, settled when it is multiplied
-    __device__ __forceinline__ chunk_t load_end(int64_t k, int64_t klen) const {
+    __device__ __forceinline__ Piece<T, ODD> load_end(int64_t k, int64_t klen) const {
       const int first = ((threadIdx.x & 63) >> 4) * CHE<T>;
       const int64_t left = klen - k - first;
       if constexpr (ALONG_K) {
-        return load_edge(p + k, left, p - first);
-      } else {
-        T e[CHE<T>] = {};
-#pragma unroll
-        for (int j = 0; j < CHE<T>; ++j) e[j] = p[((j < left ? k + j : -first)) * ld];  // past the end: row 0, settled to 0
-        chunk_t v;
-        __builtin_memcpy(&v, e, 16);
-        return v;
-      }
-    }
-    __device__ __forceinline__ chunk_t settle_end(const chunk_t& v, int64_t k, int64_t klen) const {
-      const int64_t left = klen - k - ((threadIdx.x & 63) >> 4) * CHE<T>;
-      if constexpr (ALONG_K) {
-        return settle<T>(v, left);
+        return load_edge<T, ODD>(p + k, left, p - first);
       } else {
         T e[CHE<T>];
-        __builtin_memcpy(e, &v, 16);
+#pragma unroll
+        for (int j = 0; j < CHE<T>; ++j) e[j] = p[(j < left ? k + j : -first) * ld];  // past the end: row 0, settled to 0
+        return gathered(e);
+      }
+    }
+    __device__ __forceinline__ chunk_t settle_end(const Piece<T, ODD>& v, int64_t k, int64_t klen) const {
+      const int64_t left = klen - k - ((threadIdx.x & 63) >> 4) * CHE<T>;
+      if constexpr (ALONG_K) {
+        return settle(v, left);
+      } else {
+        T e[CHE<T>];
+        __builtin_memcpy(e, &v.c, 16);
 #pragma unroll
         for (int j = 0; j < CHE<T>; ++j) e[j] = j < left ? e[j] : (T)0;
-        chunk_t r;
-        __builtin_memcpy(&r, e, 16);
-        return r;
+        return gathered(e).c;
       }
+    }
+    static __device__ __forceinline__ Piece<T, ODD> gathered(const T (&e)[CHE<T>]) {
+      Piece<T, ODD> v;
+      __builtin_memcpy(&v.c, e, 16);
+      return v;
     }
   };
 
@@ -607,7 +631,7 @@ template <class T, int FA, int FB, bool XK, bool WK> struct DirectTile {
       for (int a = 0; a < FA; ++a) sx[a].start(x, a * 16);
 #pragma unroll
       for (int b = 0; b < FB; ++b) sw[b].start(w, b * 16);
-      chunk_t fx[2 * FLIGHT][FA], fw[2 * FLIGHT][FB];
+      Piece<T, ODD> fx[2 * FLIGHT][FA], fw[2 * FLIGHT][FB];
       for (; k + FLIGHT * KE <= end; k += FLIGHT * KE) {
 #pragma unroll
         for (int s = 0; s < 2 * FLIGHT; ++s) {
@@ -621,7 +645,7 @@ template <class T, int FA, int FB, bool XK, bool WK> struct DirectTile {
 #pragma unroll
           for (int b = 0; b < FB; ++b)
 #pragma unroll
-            for (int a = 0; a < FA; ++a) acc[b][a] = Num<T>::mma(fw[s][b], fx[s][a], acc[b][a]);
+            for (int a = 0; a < FA; ++a) acc[b][a] = Num<T>::mma(fw[s][b].value(), fx[s][a].value(), acc[b][a]);
       }
 #pragma unroll
       for (int s = 0; s < 2 * FLIGHT; ++s)
@@ -635,13 +659,11 @@ template <class T, int FA, int FB, bool XK, bool WK> struct DirectTile {
       for (int s = 0; s < 2 * FLIGHT; ++s)
         if (k + s * (KE / 2) < end) {
 #pragma unroll
-          for (int b = 0; b < FB; ++b) fw[s][b] = sw[b].settle_end(fw[s][b], k + s * (KE / 2), end);
+          for (int b = 0; b < FB; ++b) {
+            const chunk_t w = sw[b].settle_end(fw[s][b], k + s * (KE / 2), end);
 #pragma unroll
-          for (int a = 0; a < FA; ++a) fx[s][a] = sx[a].settle_end(fx[s][a], k + s * (KE / 2), end);
-#pragma unroll
-          for (int b = 0; b < FB; ++b)
-#pragma unroll
-            for (int a = 0; a < FA; ++a) acc[b][a] = Num<T>::mma(fw[s][b], fx[s][a], acc[b][a]);
+            for (int a = 0; a < FA; ++a) acc[b][a] = Num<T>::mma(w, sx[a].settle_end(fx[s][a], k + s * (KE / 2), end), acc[b][a]);
+          }
         }
     }
     acc_t* part = reinterpret_cast<acc_t*>(lds) + (threadIdx.x & 63);
