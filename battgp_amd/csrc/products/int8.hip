@@ -76,9 +76,32 @@ template <class T> __device__ __forceinline__ typename Quant<T>::B magnitude(typ
   return bits_as<B>(v) & (~(B)0 >> 1);
 }
 
-// A row by TPR threads, 8 elements to a unit, U units a thread: the row stays in registers between the search for its
-// scale and the codes, so x is read once.  LONG: rows of more than 8 U TPR elements, read twice (the second time out
-// of the caches).
+// the largest of the 64 lanes' values: inside rows of 16 lanes, then across them; it ends up in lane 63
+template <int CTRL, int ROWS> __device__ __forceinline__ uint32_t dpp(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false); }
+template <int CTRL, int ROWS> __device__ __forceinline__ uint64_t dpp(uint64_t v) {
+  return (uint64_t)dpp<CTRL, ROWS>((uint32_t)(v >> 32)) << 32 | dpp<CTRL, ROWS>((uint32_t)v);
+}
+template <int CTRL, int ROWS, class B> __device__ __forceinline__ B max_step(B v) {
+  const B o = dpp<CTRL, ROWS>(v);
+  return o > v ? o : v;
+}
+template <class B> __device__ __forceinline__ B wave_max(B v) {
+  v = max_step<0x111, 0xf>(v);
+  v = max_step<0x112, 0xf>(v);
+  v = max_step<0x114, 0xf>(v);
+  v = max_step<0x118, 0xf>(v);
+  v = max_step<0x142, 0xa>(v);
+  v = max_step<0x143, 0xc>(v);
+  const uint32_t lo = __builtin_amdgcn_readlane((int)v, 63);
+  if constexpr (sizeof(B) == 4) return lo;
+  else return (B)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), 63) << 32 | lo;
+}
+
+// A row by TPR threads, U units of 8 elements each: the row stays in registers between the search for its scale and the
+// codes, so x is read once.  With one unit the code is short, and fetching code is what short kernels wait for (16384 x 1024
+// bf16 numbers: 25 us with four units a thread, 15 with one; 16 rows: 7.8 and 3.8); large matrices of long rows have
+// fewer waves to start with four (8192 x 8192: 44 us against 51).  LONG: rows of more than 8 U TPR elements, read twice
+// (the second time out of the caches).
 template <class T, bool POW2, int TPR, int U, bool LONG> __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void quantize_rows_kernel(QuantArgs p) {
   using F = typename Quant<T>::F;
   using B = typename Quant<T>::B;
@@ -114,20 +137,16 @@ template <class T, bool POW2, int TPR, int U, bool LONG> __global__ __launch_bou
   };
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    load((int64_t)(u * TPR + lane) * 8, v[u]);
+    load((u * TPR + lane) * 8, v[u]);
     look(v[u]);
   }
   if (LONG)
-    for (int64_t k = (int64_t)(U * TPR + lane) * 8; k < K; k += TPR * 8) {
+    for (int64_t k = (U * TPR + lane) * 8; k < K; k += TPR * 8) {
       F f[8];
       load(k, f);
       look(f);
     }
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) {
-    const B o = __shfl_xor(top, d);
-    top = o > top ? o : top;
-  }
+  top = wave_max(top);
   if (WPR > 1) {
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
     __syncthreads();
@@ -206,26 +225,30 @@ template <class T, bool POW2, int TPR, int U, bool LONG> __global__ __launch_bou
     }
   };
 #pragma unroll
-  for (int u = 0; u < U; ++u) put((int64_t)(u * TPR + lane) * 8, v[u]);
+  for (int u = 0; u < U; ++u) put((u * TPR + lane) * 8, v[u]);
   if (LONG)
-    for (int64_t k = (int64_t)(U * TPR + lane) * 8; k < K; k += TPR * 8) {
+    for (int64_t k = (U * TPR + lane) * 8; k < K; k += TPR * 8) {
       F f[8];
       load(k, f);
       put(k, f);
     }
 }
 
+template <class T, bool POW2, int TPR, int U, bool LONG> int run_quantize(const QuantArgs& p, hipStream_t st) {
+  constexpr int NT = TPR > 256 ? TPR : 256, RPW = NT / TPR;
+  const int64_t groups = (p.M + RPW - 1) / RPW;
+  if (groups > MAX_WORKGROUPS / 4) return bgp_products_fail(-1, "bgp_quantize_rows: %lld rows are more than one launch holds", (long long)p.M);
+  return launch("bgp_quantize_rows", quantize_rows_kernel<T, POW2, TPR, U, LONG>, dim3((unsigned)groups), dim3(NT), st, p);
+}
+
 template <class T, bool POW2> int quantize_by_length(const QuantArgs& p, hipStream_t st) {
-  const char* what = "bgp_quantize_rows";
-  // a wave per row up to 2048 elements where there are rows enough for every CU, else a workgroup of 4 waves up to 8192, of
-  // 16 beyond
-  const bool wave = p.K <= 2048 && p.M >= 4 * CUS;
-  const int64_t groups = wave ? (p.M + 3) / 4 : p.M;
-  if (groups > MAX_WORKGROUPS / 4) return bgp_products_fail(-1, "%s: %lld rows are more than one launch holds", what, (long long)p.M);
-  const dim3 grid((unsigned)groups);
-  if (wave) return launch(what, quantize_rows_kernel<T, POW2, 64, 4, false>, grid, dim3(256), st, p);
-  if (p.K <= 8192) return launch(what, quantize_rows_kernel<T, POW2, 256, 4, false>, grid, dim3(256), st, p);
-  return launch(what, quantize_rows_kernel<T, POW2, 1024, 4, true>, grid, dim3(1024), st, p);
+  if (p.K <= 512) return run_quantize<T, POW2, 64, 1, false>(p, st);
+  if (p.K <= 1024) return run_quantize<T, POW2, 128, 1, false>(p, st);
+  if (p.K <= 2048) return run_quantize<T, POW2, 256, 1, false>(p, st);
+  if (p.K <= 4096) return run_quantize<T, POW2, 512, 1, false>(p, st);
+  if (p.K <= 8192 && p.M >= 8 * CUS) return run_quantize<T, POW2, 256, 4, false>(p, st);
+  if (p.K <= 8192) return run_quantize<T, POW2, 1024, 1, false>(p, st);
+  return run_quantize<T, POW2, 1024, 1, true>(p, st);
 }
 
 template <class T> int quantize_by_type(const QuantArgs& p, int pow2, hipStream_t st) {
