@@ -449,7 +449,7 @@ extern "C" int64_t bgp_grouped_gemm(int device, void* stream, int dtype, int64_t
   Laid x(X, 1, 0, T, ldx, K, size, true), w(W, strideW ? G : 1, strideW, w_trans ? K : N, ldw, w_trans ? N : K, size, !w_trans);
   const bool wide = K * size >= 16 && (!w_trans || N * size >= 16);
   const Question q{size, wide && (!w_trans || size >= 4), x.ok && w.ok, pipe_fits(padded_row(x.extent, size), size, true, 256) && pipe_fits(padded_row(w.extent, size), size, !w_trans, 256),
-                   (double)K, (double)(x.bytes(size) + w.bytes(size)), (double)T * N, G > 0 ? 16 : 1};
+                   (double)K, (double)(x.bytes(size) + w.bytes(size)), (double)T * N, size, G > 0 ? 16 : 1};
   const Plan plan = make_plan(q, [&](int b) { return expected_tiles(T, G, b) * ((N + b - 1) / b); });
   Workspace ws(workspace);
   PackJob jobs[2];
@@ -489,7 +489,7 @@ extern "C" int64_t bgp_grouped_gemm_dw(int device, void* stream, int dtype, int6
   // a group's rows are its length of k: their mean, and as much again for the longest of uneven ones
   const double used = (double)(G < T ? G : T > 0 ? T : 1);
   const Question q{size, size >= 4, x.ok && y.ok, pipe_fits(padded_row(N, size), size, false, 256) && pipe_fits(padded_row(K, size), size, false, 256),
-                   ceil(T / used), (double)(x.bytes(size) + y.bytes(size)), (double)G * N * K, 16};
+                   ceil(T / used), (double)(x.bytes(size) + y.bytes(size)), (double)G * N * K, size, 16};
   const Plan plan = make_plan(q, [&](int b) { return (double)G * ((N + b - 1) / b) * ((K + b - 1) / b); });
   Workspace ws(workspace);
   PackJob jobs[2];

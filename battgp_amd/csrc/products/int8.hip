@@ -266,29 +266,39 @@ struct Int8Args {
 // N neighbours of a row, at the alignment of one
 template <class T, int N> struct __attribute__((packed, aligned(sizeof(T)))) Few { T e[N]; };
 
-// scaled sums to D's rows, 16 bytes at a time
+// scaled sums to D's rows, 16 bytes at a time; C is fetched for AHEAD units before the first is stored (the compiler may
+// not do that: C can be D)
 template <class T, bool ADD> struct ScaledRows {
   using S = typename ScaleOf<T>::type;
-  static constexpr int E = 16 / (int)sizeof(T);
+  static constexpr int E = 16 / (int)sizeof(T), AHEAD = ADD && sizeof(T) >= 4 ? 4 : 2;
   T* y;
   const T* c;
   const S *sa, *sb;
   int64_t ldy, ldc, cols;
+  struct Other {
+    Few<T, ADD ? E : 1> add;
+  };
+  __device__ __forceinline__ Other other(int i, int j) const {
+    Other o;
+    if constexpr (ADD)
+      if (j + E <= cols) o.add = *reinterpret_cast<const Few<T, E>*>(c + i * ldc + j);
+    return o;
+  }
   __device__ __forceinline__ void single(int i, int j, int v) const {
     if (j >= cols) return;
     const double r = (double)v * ((double)sa[i] * (double)sb[j]);
     y[i * ldy + j] = narrow<T>(ADD ? r + widen(c[i * ldc + j]) : r);
   }
-  __device__ __forceinline__ void operator()(int i, int j, const int* v) const {
+  __device__ __forceinline__ void operator()(int i, int j, const int* v, const Other& t) const {
     if (j + E <= cols) {
       const Few<S, E> s = *reinterpret_cast<const Few<S, E>*>(sb + j);
       const double si = (double)sa[i];
-      Few<T, E> add, o;
-      if (ADD) add = *reinterpret_cast<const Few<T, E>*>(c + i * ldc + j);
+      Few<T, E> o;
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        const double r = (double)v[e] * (si * (double)s.e[e]);
-        o.e[e] = narrow<T>(ADD ? r + widen(add.e[e]) : r);
+        double r = (double)v[e] * (si * (double)s.e[e]);
+        if constexpr (ADD) r += widen(t.add.e[e]);
+        o.e[e] = narrow<T>(r);
       }
       *reinterpret_cast<Few<T, E>*>(y + i * ldy + j) = o;
     } else {
@@ -468,7 +478,8 @@ extern "C" int64_t bgp_int8_gemm(int device, void* stream, int dtype, int64_t M,
   const int64_t to = padded_row(K, 1);
   const bool a_ok = reinterpret_cast<uintptr_t>(A) % 16 == 0 && lda % 16 == 0 && pipe_fits(lda, 1, true, 256);
   const bool b_ok = reinterpret_cast<uintptr_t>(B) % 16 == 0 && ldb % 16 == 0 && pipe_fits(ldb, 1, true, 256);
-  const Question q{1, K >= 16, a_ok && b_ok, true, (double)K, (a_ok ? 0.0 : (double)M * to) + (b_ok ? 0.0 : (double)N * to), (double)M * N, 1};
+  const Question q{1, K >= 16, a_ok && b_ok, true, (double)K, (a_ok ? 0.0 : (double)M * to) + (b_ok ? 0.0 : (double)N * to), (double)M * N,
+                   (dtype == BGP_F64 ? 8 : dtype == BGP_F32 ? 4 : 2) * (C ? 2 : 1), 1};
   const Plan plan = make_plan(q, [&](int b) { return (double)((M + b - 1) / b) * ((N + b - 1) / b); });
   Int8Args p{A, B, scale_a, scale_b, C, Y, M, N, K, lda, ldb, ldc, ldy, 0};
   Workspace ws(workspace);

@@ -25,6 +25,7 @@ constexpr float ALONE_US[4][CUTS] = {{0.12f, 0.22f, 0.52f, 1.0f, 0.30f, 0.62f, 1
                                      {0.12f, 0.27f, 0.85f, 2.5f, 0.61f, 2.06f, 9e9f},
                                      {0.10f, 0.23f, 0.88f, 2.5f, 0.59f, 1.95f, 9e9f}};
 constexpr float LAUNCH_US = 3.0f, PACK_US = 2.0f, COPY_BYTES_US = 3.5e6f;
+constexpr float OUT_BYTES_US = 20e3f;  // a CU's results to memory and back, with more than 4 waves at it
 constexpr int CUS = 256;
 
 struct Plan {
@@ -39,6 +40,7 @@ struct Question {
   bool packable;           // the pipelined ones after unaligned operands have been copied into aligned rows
   double k, pack_bytes;    // length of k; bytes of the operands that would be copied
   double outputs;          // elements of D
+  int out_bytes;           // written (and read, if D is added to) for each
   int most_split;          // 1: k is not cut
 };
 
@@ -59,7 +61,8 @@ template <class F> Plan make_plan(const Question& q, F&& tiles) {
       const double each = ceil(unit * split / CUS), deep = ceil(stages / split);
       double stage = each * STAGE_US[kind][cut];
       if (stage < ALONE_US[kind][cut]) stage = ALONE_US[kind][cut];
-      double us = LAUNCH_US + deep * stage;
+      const double tile_bytes = each * tile_of(cut) * tile_of(cut) * (split > 1 ? (q.size == 8 ? 8 : 4) : q.out_bytes);
+      double us = LAUNCH_US + deep * stage + tile_bytes / (each > 1 || cut == PIPE256 ? OUT_BYTES_US : OUT_BYTES_US / 2);
       if (split > 1) us += LAUNCH_US + (split + 1) * q.outputs * (q.size == 8 ? 8 : 4) / COPY_BYTES_US;
       if (pack) us += PACK_US + 2 * q.pack_bytes / COPY_BYTES_US;
       if (us < least) {

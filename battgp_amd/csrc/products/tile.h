@@ -319,22 +319,33 @@ __device__ __forceinline__ void hand_out(const ACC (&acc)[FB][FA], char* mine, i
         }
       }
     __builtin_amdgcn_wave_barrier();
-    constexpr int PER_ROW = C / E;
-#pragma unroll 2
-    for (int u = lane; u < AT_ONCE * 16 * PER_ROW; u += 64) {
-      const int row = u / PER_ROW, j = u % PER_ROW * E;
-      S v[E];
-      if constexpr (E * sizeof(S) < 16) {
-        __builtin_memcpy(v, place(row, j), E * sizeof(S));
-      } else {
+    constexpr int PER_ROW = C / E, ALL = AT_ONCE * 16 * PER_ROW / 64;
+    constexpr int AHEAD = std::remove_reference<F>::type::AHEAD < ALL ? std::remove_reference<F>::type::AHEAD : ALL;
+    static_assert(ALL % AHEAD == 0, "whole rounds");
+#pragma unroll 1
+    for (int u0 = lane; u0 < 64 * ALL; u0 += 64 * AHEAD) {
+      typename std::remove_reference<F>::type::Other other[AHEAD];  // what a unit takes from memory, before any is stored
 #pragma unroll
-        for (int c = 0; c < (int)(E * sizeof(S) / 16); ++c) {
-          const chunk_t one = *reinterpret_cast<const chunk_t*>(place(row, j + c * 16 / (int)sizeof(S)));
-          __builtin_memcpy(reinterpret_cast<char*>(v) + c * 16, &one, 16);
-        }
+      for (int n = 0; n < AHEAD; ++n) {
+        const int u = u0 + 64 * n, i = x0 + first * 16 + u / PER_ROW;
+        other[n] = f.other(i < rows ? i : (int)rows - 1, w0 + u % PER_ROW * E);
       }
-      const int i = x0 + first * 16 + row;
-      if (i < rows) f(i, w0 + j, v);
+#pragma unroll
+      for (int n = 0; n < AHEAD; ++n) {
+        const int u = u0 + 64 * n, row = u / PER_ROW, j = u % PER_ROW * E;
+        S v[E];
+        if constexpr (E * sizeof(S) < 16) {
+          __builtin_memcpy(v, place(row, j), E * sizeof(S));
+        } else {
+#pragma unroll
+          for (int c = 0; c < (int)(E * sizeof(S) / 16); ++c) {
+            const chunk_t one = *reinterpret_cast<const chunk_t*>(place(row, j + c * 16 / (int)sizeof(S)));
+            __builtin_memcpy(reinterpret_cast<char*>(v) + c * 16, &one, 16);
+          }
+        }
+        const int i = x0 + first * 16 + row;
+        if (i < rows) f(i, w0 + j, v, other[n]);
+      }
     }
     __builtin_amdgcn_wave_barrier();
   }
@@ -714,11 +725,13 @@ inline bool pipe_fits(int64_t ld, int size, bool along_k, int rows) {
 template <class O> struct PlainRows {
   O* d;
   int64_t ld, cols;
-  static constexpr int E = 16 / (int)sizeof(O);
+  static constexpr int E = 16 / (int)sizeof(O), AHEAD = 2;
+  struct Other {};
+  __device__ __forceinline__ Other other(int, int) const { return {}; }
   template <class S> __device__ __forceinline__ void single(int i, int j, S v) const {
     if (j < cols) d[i * ld + j] = round_to<O>(v);
   }
-  template <class S> __device__ __forceinline__ void operator()(int i, int j, const S* v) const {
+  template <class S> __device__ __forceinline__ void operator()(int i, int j, const S* v, const Other&) const {
     O e[E];
 #pragma unroll
     for (int c = 0; c < E; ++c) e[c] = round_to<O>(v[c]);
