@@ -26,14 +26,18 @@ class DeviceScope {
     if (before_ >= 0) (void)hipSetDevice(before_);
   }
   int check(const char* what) const {
-    return err_ == hipSuccess ? 0 : bgp_products_fail(-2, "%s: %s", what, hipGetErrorString(err_));
+    if (err_ == hipSuccess) return 0;
+    (void)hipGetLastError();
+    return bgp_products_fail(-2, "%s: %s", what, hipGetErrorString(err_));
   }
 };
 
 template <class... A> int launch(const char* what, void (*kernel)(A...), dim3 grid, dim3 block, hipStream_t stream, A... args) {
   void* ptrs[] = {(void*)&args...};
   const hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, block, ptrs, 0, stream);
-  return e == hipSuccess ? 0 : bgp_products_fail(-2, "%s: launch failed: %s", what, hipGetErrorString(e));
+  if (e == hipSuccess) return 0;
+  (void)hipGetLastError();  // reported here: not by whoever asks next
+  return bgp_products_fail(-2, "%s: launch failed: %s", what, hipGetErrorString(e));
 }
 
 // Waves of a tile in LDS: 2 x 4 of 128 x 64 on 256 x 256; 2 x 2 below, but 2 x 4 of 64 x 32 for fp64 on 128 x 128, whose

@@ -29,6 +29,7 @@ struct GroupedArgs {
   const int64_t* off;
   int64_t T, N, K, ldx, ldw, sw, ldy;
   int G, rest, tiles_n;
+  int most_m;  // row tiles that the launch was sized for: offsets that do not ascend can ask for more
   int split;   // k is cut in this many parts,
   void* part;  // whose sums go here: [split][rows of D][columns of D], fp32 (fp64)
 };
@@ -81,13 +82,14 @@ __device__ __forceinline__ int count_row_tiles(const GroupedArgs& p, int BM, Bou
   const int lane = threadIdx.x & 63, groups = p.rest ? p.G + 2 : p.G;
   *first = lane_bounds(p, BM, lane);
   int tiles = __builtin_amdgcn_readlane(first->sum, 63);
-  for (int base = 64; base < groups; base += 64) tiles += __builtin_amdgcn_readlane(lane_bounds(p, BM, base + lane).sum, 63);
-  return tiles;
+  for (int base = 64; base < groups && tiles < p.most_m; base += 64) tiles += __builtin_amdgcn_readlane(lane_bounds(p, BM, base + lane).sum, 63);
+  return tiles < p.most_m ? tiles : p.most_m;
 }
 
+// the want-th of them
 __device__ __forceinline__ RowTile find_row_tile(const GroupedArgs& p, int BM, Bounds r, int want) {
-  const int lane = threadIdx.x & 63;
-  for (int base = 0;;) {
+  const int lane = threadIdx.x & 63, groups = p.rest ? p.G + 2 : p.G;
+  for (int base = 0; base < groups;) {
     const unsigned long long past = __ballot(r.sum > want);
     if (past) {
       const int j = __ffsll(past) - 1;
@@ -99,13 +101,14 @@ __device__ __forceinline__ RowTile find_row_tile(const GroupedArgs& p, int BM, B
     base += 64;
     r = lane_bounds(p, BM, base + lane);
   }
+  return RowTile{-1, 0, 0};
 }
 
 // Y[rows of g, :] = X[rows of g, :] W_g^T;  WK: W_g[n, k] = w[g sw + n ldw + k], else w[g sw + k ldw + n]
 template <class T, class P, bool WK> __device__ __forceinline__ void rows_tile(const GroupedArgs& p, const RowTile& t, int64_t n0, char* lds) {
   using A = typename Sum<T>::type;
   const bool some = t.g < p.G;
-  if (p.split > 1 && !some) return;
+  if (t.g < 0 || (p.split > 1 && !some)) return;
   const Part k = some ? part_of(p.K, KSTAGE<T>, p.split, blockIdx.y) : Part{0, 0};
   const Operand<T> x{static_cast<const T*>(p.x) + t.row0 * p.ldx + k.from, p.ldx, t.rows, p.K >= CHE<T>};
   const Operand<T> w{static_cast<const T*>(p.w) + (some ? t.g * p.sw + (WK ? n0 * p.ldw + k.from : n0 + k.from * p.ldw) : 0), p.ldw, p.N - n0,
@@ -353,8 +356,9 @@ template <class T, bool WK, int CUT> int run_rows(const GroupedArgs& p0, hipStre
   GroupedArgs p = p0;
   p.tiles_n = (int)((p.N + B - 1) / B);
   // row tiles there can be at most: a group adds less than one to its share of the rows
-  const int64_t tiles = (p.T / B + p.G + (p.rest ? 2 : 0)) * p.tiles_n + (B == 256 ? CUS : 7);
+  const int64_t most_m = p.T / B + p.G + (p.rest ? 2 : 0), tiles = most_m * p.tiles_n + (B == 256 ? CUS : 7);
   if (tiles > MAX_WORKGROUPS / 2) return bgp_products_fail(-1, "%s: %lld tiles are more than one launch holds", what, (long long)tiles);
+  p.most_m = (int)most_m;
   const dim3 grid((unsigned)tiles, p.split);
   if constexpr (CUT <= DIRECT32) {
     if constexpr (sizeof(T) < 4)
@@ -466,7 +470,7 @@ extern "C" int64_t bgp_grouped_gemm(int device, void* stream, int dtype, int64_t
   const hipStream_t st = static_cast<hipStream_t>(stream);
   if (count)
     if (int rc = launch_pack(what, size, jobs, count, st)) return rc;
-  const GroupedArgs p{x.p, w.p, Y, offsets, T, N, K, x.ld, w.ld, w.stride, ldy, (int)G, zero_rest != 0, 0, plan.split, part};
+  const GroupedArgs p{x.p, w.p, Y, offsets, T, N, K, x.ld, w.ld, w.stride, ldy, (int)G, zero_rest != 0, 0, 0, plan.split, part};
   switch (dtype) {
     case BGP_F64: return run_rows_plan<double>(p, w_trans, plan, st);
     case BGP_F32: return run_rows_plan<float>(p, w_trans, plan, st);
@@ -505,7 +509,7 @@ extern "C" int64_t bgp_grouped_gemm_dw(int device, void* stream, int dtype, int6
   const hipStream_t st = static_cast<hipStream_t>(stream);
   if (count)
     if (int rc = launch_pack(what, size, jobs, count, st)) return rc;
-  const GroupedArgs p{x.p, dW, const_cast<void*>(y.p), offsets, T, N, K, x.ld, ldw, strideW, y.ld, (int)G, 0, 0, plan.split, part};
+  const GroupedArgs p{x.p, dW, const_cast<void*>(y.p), offsets, T, N, K, x.ld, ldw, strideW, y.ld, (int)G, 0, 0, 0, plan.split, part};
   switch (dtype) {
     case BGP_F64: return run_dw_plan<double>(p, plan, st);
     case BGP_F32: return run_dw_plan<float>(p, plan, st);

@@ -22,7 +22,7 @@ const Tensor* gpu_tensor(PyObject* o, int dim, int device = -1) {
   if (!THPVariable_Check(o)) return nullptr;
   const Tensor& t = THPVariable_Unpack(o);
   if (t.layout() != at::kStrided || !t.is_cuda() || t.dim() != dim || (device >= 0 && t.get_device() != device)) return nullptr;
-  if (t.requires_grad() && c10::GradMode::is_enabled()) return nullptr;
+  if (t.is_neg() || (t.requires_grad() && c10::GradMode::is_enabled())) return nullptr;
   return &t;
 }
 

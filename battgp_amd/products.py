@@ -48,8 +48,8 @@ def _gpu_tensor(name: str, t, dim: int, device: int | None = None) -> int:
     """the index of the device that ``t`` is on (checks are written for the call that passes: they cost a call its time)"""
     if not isinstance(t, _Tensor):
         raise TypeError(f"{name} is not a torch tensor")
-    if t.layout is not _strided:
-        raise ValueError(f"{name} is not a dense tensor")
+    if t.layout is not _strided or t.is_neg():
+        raise ValueError(f"{name} is not a dense tensor that holds its own values")
     if t.dim() != dim:
         raise ValueError(f"{name} has {t.dim()} dimensions, {dim} are wanted")
     at = t.get_device()

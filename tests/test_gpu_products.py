@@ -444,3 +444,191 @@ def test_offsets_past_32_bits(products):
     a[-1] = 3
     z = products.int8_matmul(a, a[-2:], torch.ones(a.shape[0], device="cuda"), torch.ones(2, device="cuda"))
     assert z[-1].tolist() == [0.0, float(torch.tensor(9360.0).bfloat16())] and not z[:-1].any()
+
+
+# ---- sizes and strides that take the other ways through the library ----
+
+def gpu_whole(shape, seed, dtype, most=4):
+    return torch.randint(-most, most + 1, shape, device="cuda", generator=torch.Generator(device="cuda").manual_seed(seed)).to(dtype)
+
+
+def gpu_grouped_ref(x, w, off):
+    """in 64 bits on the GPU, one group at a time"""
+    y = torch.zeros(x.shape[0], w.shape[1], dtype=torch.float64, device="cuda")
+    for g, (a, b) in enumerate(rows_of(off)):
+        if b > a:
+            y[a:b] = x[a:b].double() @ w[g].double().T
+    return y
+
+
+def in_rows_of(t, ld, at=0):
+    """t[.., m, n] inside rows of ld elements, from column `at` on, NaN (99) around it"""
+    buf = torch.full((*t.shape[:-1], ld), 99 if t.dtype == torch.int8 else float("nan"), dtype=t.dtype, device="cuda")
+    buf[..., at:at + t.shape[-1]] = t
+    return buf[..., at:at + t.shape[-1]]
+
+
+CUTS = [  # rows of the groups, n, k: many tiles, a last round of few, long k with few tiles, long groups with few tiles
+    ([1500, 3, 0, 700, 2600], 1500, 70),
+    ([4000, 260, 1], 4300, 200),
+    ([9000], 2100, 24),
+    ([3], 96, 4100),
+    ([17, 0, 30], 130, 2600),
+    ([6000, 0, 2500], 70, 90),
+    ([20000], 33, 40),
+]
+
+
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("counts, n, k", CUTS, ids=lambda v: str(v).replace(" ", ""))
+@pytest.mark.parametrize("layout", ["contiguous", "aligned rows", "words", "odd"])
+def test_larger_products_and_layouts(products, dtype, counts, n, k, layout):
+    """exact whole numbers again: |x|, |w|, |dy| <= 2, so that sums of 20000 products stay below 2^24"""
+    off = np.concatenate(([0], np.cumsum(counts))).tolist()
+    t, g = off[-1], len(counts)
+    x, w, dy = gpu_whole((t, k), 1, dtype, 2), gpu_whole((g, n, k), 2, dtype, 2), gpu_whole((t, n), 3, dtype, 2)
+    yr, dxr = gpu_grouped_ref(x, w, off), gpu_grouped_ref(dy, w.transpose(1, 2), off)
+    dwr = torch.stack([dy[a:b].double().T @ x[a:b].double() for a, b in rows_of(off)])
+    if layout != "contiguous":
+        size = dtype.itemsize
+        unit = {"aligned rows": 16, "words": max(4, size), "odd": size}[layout] // size
+        at = {"aligned rows": 0, "words": unit, "odd": 1}[layout]
+        x, w, dy = (in_rows_of(m, (m.shape[-1] + at) // unit * unit + 2 * unit, at) for m in (x, w, dy))
+    od = torch.tensor(off, device="cuda")
+    assert torch.equal(products.grouped_matmul(x, w, od), yr.to(dtype))
+    dx, dw = products.grouped_matmul_grad(dy, x, w, od)
+    assert torch.equal(dx, dxr.to(dtype))
+    if dtype == torch.float16:  # sums past 65504 are infinities in both
+        assert torch.equal(dw, dwr.float().to(dtype))
+    else:
+        assert torch.equal(dw, dwr.to(dtype))
+    wt = w.transpose(1, 2).contiguous().transpose(1, 2)
+    assert torch.equal(products.grouped_matmul(x, wt, od), yr.to(dtype))
+    dx, _ = products.grouped_matmul_grad(dy, x, wt, od)
+    assert torch.equal(dx, dxr.to(dtype))
+
+
+@pytest.mark.parametrize("m, n, k", [(3000, 5000, 300), (2600, 2700, 33), (1, 300, 9000), (70, 50, 8000), (9000, 20, 100)])
+@pytest.mark.parametrize("layout", ["contiguous", "aligned rows", "words", "odd"])
+def test_larger_int8_products_and_layouts(products, m, n, k, layout):
+    gen = torch.Generator(device="cuda").manual_seed(m)
+    a, b = (torch.randint(-128, 128, s, device="cuda", generator=gen, dtype=torch.int8) for s in ((m, k), (n, k)))
+    ref = a.double() @ b.double().T  # below 2^53: exact
+    if layout != "contiguous":
+        unit, at = {"aligned rows": (16, 0), "words": (4, 4), "odd": (1, 1)}[layout]
+        a, b = (in_rows_of(t, (k + at) // unit * unit + 2 * unit, at) for t in (a, b))
+    one = torch.ones(max(m, n), device="cuda", dtype=torch.float64)
+    assert torch.equal(products.int8_matmul(a, b, one[:m], one[:n], dtype=torch.float64), ref)
+    half = torch.full((max(m, n),), 0.5, device="cuda")
+    got = products.int8_matmul(a, b, half[:m], half[:n], dtype=torch.bfloat16)
+    # a quarter of a whole number below 2^53: its rounding to bf16 by way of fp32 could round twice; by way of whole steps not
+    step = torch.exp2(torch.floor(torch.log2((ref / 4).abs().clamp_min(1e-30))) - 7)
+    assert torch.equal(got.double(), torch.where(ref == 0, ref, torch.round(ref / 4 / step) * step))
+
+
+def test_offsets_that_do_not_ascend_stay_inside(products):
+    """what they select is up to the call, but nothing outside the output is written and the call ends"""
+    x, w = gpu_whole((300, 64), 1, torch.float32), gpu_whole((5, 70, 64), 2, torch.float32)
+    for off in ([0, 300, 0, 300, 0, 300], [300, 200, 100, 50, 20, 0], [-9, 2 ** 60, -2 ** 60, 7, 3, 2 ** 40]):
+        out, rim = guarded((300, 70), torch.float32)
+        od = torch.tensor(off, device="cuda")
+        products.grouped_matmul(x, w, od, out=out)
+        products.grouped_matmul_grad(out, x, w, od)
+        torch.cuda.synchronize()
+        rim()
+    many = torch.tensor([0, 300] * 2000 + [0], device="cuda")
+    products.grouped_matmul(x, w[:1].expand(4000, 70, 64), many)
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_numbers_below_the_normal_ones(products, dtype):
+    fi = torch.finfo(dtype)
+    least = fi.smallest_normal * fi.eps  # the smallest number above 0
+    x = torch.tensor([[least, 3 * least, -5 * least, fi.smallest_normal] + [0.0] * 12], dtype=torch.float64)
+    w = torch.eye(16, dtype=torch.float64)[None] * 64.0
+    y = products.grouped_matmul(x.to(dtype).cuda(), w.to(dtype).cuda(), torch.tensor([0, 1], device="cuda"))
+    assert torch.equal(y.cpu().double(), x * 64.0)
+
+
+def test_infinities_stay_in_their_rows(products):
+    for dtype in ALL:
+        x, w = whole((40, 100), 1).to(dtype).cuda(), whole((2, 50, 100), 2).to(dtype).cuda()
+        off = torch.tensor([0, 25, 40], device="cuda")
+        clean = products.grouped_matmul(x, w, off)
+        x[7, 3], w[1, 9, 99] = float("inf"), float("-inf")
+        y = products.grouped_matmul(x, w, off)
+        hit = torch.zeros(40, 50, dtype=torch.bool, device="cuda")
+        hit[7] = True
+        hit[25:, 9] = True
+        assert torch.equal(y[~hit], clean[~hit]) and not y[hit].isfinite().any()
+
+
+def test_rest_in_the_place_of_the_input(products):
+    """the C entry lets the rest overwrite what was quantised: in rows that are kept in registers and in longer ones"""
+    import ctypes as C
+
+    from battgp_amd import _lib
+
+    lib = _lib.load_products()
+    st = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    for k in (50, 3000, 8000, 30000):
+        x = torch.randn(5, k, device="cuda", dtype=torch.float64)
+        q, s, r = products.quantize_rows(x, pow2=True, residual=True)
+        q2, s2 = torch.empty_like(q), torch.empty_like(s)
+        assert lib.bgp_quantize_rows(0, st, _lib.F64, 5, k, x.data_ptr(), k, q2.data_ptr(), k, s2.data_ptr(), 1, x.data_ptr(), k) == 0
+        torch.cuda.synchronize()
+        assert torch.equal(x, r) and torch.equal(q2, q) and torch.equal(s2, s)
+
+
+def test_workspaces_are_asked_for_and_fewer_bytes_refused(products):
+    import ctypes as C
+
+    from battgp_amd import _lib
+
+    lib = _lib.load_products()
+    st = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    t, n, k = 2, 64, 8192  # few tiles and a long k along rows: k is cut
+    x, w, off = gpu_whole((t, k), 1, torch.bfloat16, 1), gpu_whole((1, k, n), 2, torch.bfloat16, 1), torch.tensor([0, t], device="cuda")
+    y = torch.full((t, n), 7.0, dtype=torch.bfloat16, device="cuda")
+    args = (0, st, _lib.BF16, t, n, k, 1, x.data_ptr(), k, w.data_ptr(), n * k, n, 1, off.data_ptr(), y.data_ptr(), n, 0)
+    need = lib.bgp_grouped_gemm(*args, None, 0)
+    assert need > 0
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+    assert lib.bgp_grouped_gemm(*args, ws.data_ptr(), need - 1) == need
+    torch.cuda.synchronize()
+    assert (y == 7.0).all()  # nothing was enqueued
+    assert lib.bgp_grouped_gemm(*args, ws.data_ptr(), need) == 0
+    assert torch.equal(y, (x.double() @ w[0].double()).to(torch.bfloat16))
+
+
+def test_graph_replays_with_workspaces(products):
+    """two graphs that cut k and copy operands, replayed in turn with eager work between"""
+    off = torch.tensor([0, 3], device="cuda")
+    w = gpu_whole((1, 4100, 96), 2, torch.bfloat16, 1).transpose(1, 2)
+    a, b = (torch.randint(-99, 99, s, device="cuda", dtype=torch.int8) for s in ((2100, 2047), (2200, 2047)))
+    one = torch.ones(2200, device="cuda")
+    x = gpu_whole((3, 4100), 3, torch.bfloat16, 1)
+
+    def first():
+        return products.grouped_matmul(x, w, off)
+
+    def second():
+        return products.int8_matmul(a, b, one[:2100], one, dtype=torch.float32)
+
+    first(), second()
+    torch.cuda.synchronize()
+    graphs = []
+    for f in (first, second):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = f()
+        graphs.append((g, out))
+    for i in range(4):
+        x.copy_(gpu_whole((3, 4100), 10 + i, torch.bfloat16, 1))
+        a.copy_(torch.randint(-99, 99, a.shape, device="cuda", dtype=torch.int8))
+        for g, _ in graphs:
+            g.replay()
+        eager = (first(), second())
+        torch.cuda.synchronize()
+        assert torch.equal(graphs[0][1], eager[0]) and torch.equal(graphs[1][1], eager[1])
