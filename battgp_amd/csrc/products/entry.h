@@ -6,8 +6,8 @@
 #include "../../../include/battgp_products.h"
 #include "plan.h"
 
-// workgroups of 256 threads in one launch: the threads of a launch are counted in 32 bits
-constexpr int64_t MAX_WORKGROUPS = (1 << 24) - 1;
+// the threads of a launch are counted in 32 bits
+constexpr int64_t max_workgroups(int threads) { return ((int64_t)1 << 32) / threads - 1; }
 
 int bgp_products_fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
 
@@ -117,4 +117,7 @@ class Workspace {
     return p;
   }
   int64_t used() const { return used_; }
+  // whether `bytes` of it, as the caller gave them, do not hold what was taken
+  bool short_of(int64_t bytes) const { return used_ > 0 && (!at_ || bytes < used_); }
+  bool aligned() const { return reinterpret_cast<uintptr_t>(at_) % 16 == 0; }
 };

@@ -333,7 +333,7 @@ struct Laid {
   bool along_k, ok;
   Laid(const void* at, int64_t batches, int64_t stride_, int64_t per_, int64_t ld_, int64_t extent_, int size, bool along)
       : p(at), stride(stride_), ld(ld_), rows(batches * per_), per(per_), extent(extent_), along_k(along), ok(aligned(at, ld_, stride_, size, along, extent_)) {}
-  int64_t bytes(int size) const { return ok ? 0 : rows * padded_row(extent, size) * size; }
+  double bytes(int size) const { return ok ? 0 : (double)rows * padded_row(extent, size) * size; }
   void move(Workspace& ws, int size, PackJob* jobs, int* count) {
     if (ok) return;
     const int64_t to = padded_row(extent, size);
@@ -357,7 +357,6 @@ template <class T, bool WK, int CUT> int run_rows(const GroupedArgs& p0, hipStre
   p.tiles_n = (int)((p.N + B - 1) / B);
   // row tiles there can be at most: a group adds less than one to its share of the rows
   const int64_t most_m = p.T / B + p.G + (p.rest ? 2 : 0), tiles = most_m * p.tiles_n + (B == 256 ? CUS : 7);
-  if (tiles > MAX_WORKGROUPS / 2) return bgp_products_fail(-1, "%s: %lld tiles are more than one launch holds", what, (long long)tiles);
   p.most_m = (int)most_m;
   const dim3 grid((unsigned)tiles, p.split);
   if constexpr (CUT <= DIRECT32) {
@@ -398,7 +397,6 @@ template <class T, int CUT> int run_dw(const GroupedArgs& p0, hipStream_t st) {
   GroupedArgs p = p0;
   p.tiles_n = (int)((p.N + B - 1) / B);
   const int64_t tiles = (int64_t)p.G * p.tiles_n * ((p.K + B - 1) / B) + (B == 256 ? CUS : 8 * DEALT - 1);
-  if (tiles > MAX_WORKGROUPS / 2) return bgp_products_fail(-1, "%s: %lld tiles are more than one launch holds", what, (long long)tiles);
   const dim3 grid((unsigned)tiles, p.split);
   if constexpr (CUT <= DIRECT32) return launch(what, grouped_dw_direct_kernel<T, B / 16>, grid, dim3(256), st, p);
   else if constexpr (CUT <= PLAIN128) return launch(what, grouped_dw_kernel<T, B, B>, grid, dim3(tile_threads(B, sizeof(T))), st, p);
@@ -453,8 +451,10 @@ extern "C" int64_t bgp_grouped_gemm(int device, void* stream, int dtype, int64_t
   Laid x(X, 1, 0, T, ldx, K, size, true), w(W, strideW ? G : 1, strideW, w_trans ? K : N, ldw, w_trans ? N : K, size, !w_trans);
   const bool wide = K * size >= 16 && (!w_trans || N * size >= 16);
   const Question q{size, wide && (!w_trans || size >= 4), x.ok && w.ok, pipe_fits(padded_row(x.extent, size), size, true, 256) && pipe_fits(padded_row(w.extent, size), size, !w_trans, 256),
-                   (double)K, (double)(x.bytes(size) + w.bytes(size)), (double)T * N, size, G > 0 ? 16 : 1};
-  const Plan plan = make_plan(q, [&](int b) { return expected_tiles(T, G, b) * ((N + b - 1) / b); });
+                   (double)K, (x.bytes(size) + w.bytes(size)), (double)T * N, size, G > 0 ? 16 : 1};
+  const Plan plan = make_plan(
+      q, [&](int b) { return expected_tiles(T, G, b) * ((N + b - 1) / b); }, [&](int b) { return ((double)(T / b) + G + 2) * ((N + b - 1) / b); });
+  if (plan.cut == CUTS) return bgp_products_fail(-1, "%s: T=%lld N=%lld are more tiles than one launch holds", what, (long long)T, (long long)N);
   Workspace ws(workspace);
   PackJob jobs[2];
   int count = 0;
@@ -464,7 +464,8 @@ extern "C" int64_t bgp_grouped_gemm(int device, void* stream, int dtype, int64_t
     if (strideW == 0) w.stride = 0;
   }
   void* part = plan.split > 1 ? ws.take(plan.split * T * N * (size == 8 ? 8 : 4)) : nullptr;
-  if (ws.used() > 0 && (!workspace || workspace_bytes < ws.used())) return ws.used();
+  if (ws.short_of(workspace_bytes)) return ws.used();
+  if (!ws.aligned()) return bgp_products_fail(-1, "%s: the workspace is not aligned to 16 bytes", what);
   DeviceScope scope(device);
   if (int rc = scope.check(what)) return rc;
   const hipStream_t st = static_cast<hipStream_t>(stream);
@@ -493,8 +494,11 @@ extern "C" int64_t bgp_grouped_gemm_dw(int device, void* stream, int dtype, int6
   // a group's rows are its length of k: their mean, and as much again for the longest of uneven ones
   const double used = (double)(G < T ? G : T > 0 ? T : 1);
   const Question q{size, size >= 4, x.ok && y.ok, pipe_fits(padded_row(N, size), size, false, 256) && pipe_fits(padded_row(K, size), size, false, 256),
-                   ceil(T / used), (double)(x.bytes(size) + y.bytes(size)), (double)G * N * K, size, 16};
-  const Plan plan = make_plan(q, [&](int b) { return (double)G * ((N + b - 1) / b) * ((K + b - 1) / b); });
+                   ceil(T / used), (x.bytes(size) + y.bytes(size)), (double)G * N * K, size, 16};
+  const auto tiles = [&](int b) { return (double)G * ((N + b - 1) / b) * ((K + b - 1) / b); };
+  const Plan plan = make_plan(q, tiles, tiles);
+  if (plan.cut == CUTS)
+    return bgp_products_fail(-1, "%s: G=%lld N=%lld K=%lld are more tiles than one launch holds", what, (long long)G, (long long)N, (long long)K);
   Workspace ws(workspace);
   PackJob jobs[2];
   int count = 0;
@@ -503,7 +507,8 @@ extern "C" int64_t bgp_grouped_gemm_dw(int device, void* stream, int dtype, int6
     x.move(ws, size, jobs, &count);
   }
   void* part = plan.split > 1 ? ws.take(plan.split * G * N * K * (size == 8 ? 8 : 4)) : nullptr;
-  if (ws.used() > 0 && (!workspace || workspace_bytes < ws.used())) return ws.used();
+  if (ws.short_of(workspace_bytes)) return ws.used();
+  if (!ws.aligned()) return bgp_products_fail(-1, "%s: the workspace is not aligned to 16 bytes", what);
   DeviceScope scope(device);
   if (int rc = scope.check(what)) return rc;
   const hipStream_t st = static_cast<hipStream_t>(stream);

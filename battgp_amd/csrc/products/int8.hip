@@ -236,9 +236,17 @@ template <class T, bool POW2, int TPR, int U, bool LONG> __global__ __launch_bou
 
 template <class T, bool POW2, int TPR, int U, bool LONG> int run_quantize(const QuantArgs& p, hipStream_t st) {
   constexpr int NT = TPR > 256 ? TPR : 256, RPW = NT / TPR;
-  const int64_t groups = (p.M + RPW - 1) / RPW;
-  if (groups > MAX_WORKGROUPS / 4) return bgp_products_fail(-1, "bgp_quantize_rows: %lld rows are more than one launch holds", (long long)p.M);
-  return launch("bgp_quantize_rows", quantize_rows_kernel<T, POW2, TPR, U, LONG>, dim3((unsigned)groups), dim3(NT), st, p);
+  constexpr int64_t MOST = max_workgroups(NT) * RPW;
+  for (int64_t from = 0; from < p.M; from += MOST) {
+    QuantArgs q = p;
+    q.M = p.M - from < MOST ? p.M - from : MOST;
+    q.x = static_cast<const T*>(p.x) + from * p.ldx;
+    q.q = p.q + from * p.ldq;
+    q.scale = static_cast<typename Quant<T>::F*>(p.scale) + from;
+    q.rest = p.rest ? static_cast<T*>(p.rest) + from * p.ldr : nullptr;
+    if (int rc = launch("bgp_quantize_rows", quantize_rows_kernel<T, POW2, TPR, U, LONG>, dim3((unsigned)((q.M + RPW - 1) / RPW)), dim3(NT), st, q)) return rc;
+  }
+  return 0;
 }
 
 template <class T, bool POW2> int quantize_by_length(const QuantArgs& p, hipStream_t st) {
@@ -376,7 +384,6 @@ template <class T, int CUT> int run_int8(const Int8Args& p0, hipStream_t st) {
   Int8Args p = p0;
   p.tiles_n = (int)((p.N + B - 1) / B);
   const int64_t tiles = (p.M + B - 1) / B * p.tiles_n + (B == 256 ? CUS : 7);
-  if (tiles > MAX_WORKGROUPS / 2) return bgp_products_fail(-1, "%s: %lld tiles are more than one launch holds", what, (long long)tiles);
   const dim3 grid((unsigned)tiles);
   if constexpr (CUT <= DIRECT32) {
     if (off_words(p.a, p.lda, 0, 1) || off_words(p.b, p.ldb, 0, 1))
@@ -473,14 +480,16 @@ extern "C" int64_t bgp_int8_gemm(int device, void* stream, int dtype, int64_t M,
     return bgp_products_fail(-1, "%s: bad sizes M=%lld N=%lld K=%lld (K <= %d: a longer sum can pass 32 bits)", what, (long long)M, (long long)N, (long long)K, BGP_INT8_MAX_K);
   if (M == 0 || N == 0) return 0;
   if (!Y || !scale_a || !scale_b || (K > 0 && (!A || !B))) return bgp_products_fail(-1, "%s: null pointer", what);
-  if (lda < K || ldb < K || ldy < N || (C && ldc < N))
+  if (lda < K || ldb < K || ldy < N || (C && ldc < N) || (C == Y && ldc != ldy))
     return bgp_products_fail(-1, "%s: bad strides lda=%lld ldb=%lld ldc=%lld ldy=%lld", what, (long long)lda, (long long)ldb, (long long)ldc, (long long)ldy);
   const int64_t to = padded_row(K, 1);
   const bool a_ok = reinterpret_cast<uintptr_t>(A) % 16 == 0 && lda % 16 == 0 && pipe_fits(lda, 1, true, 256);
   const bool b_ok = reinterpret_cast<uintptr_t>(B) % 16 == 0 && ldb % 16 == 0 && pipe_fits(ldb, 1, true, 256);
   const Question q{1, K >= 16, a_ok && b_ok, true, (double)K, (a_ok ? 0.0 : (double)M * to) + (b_ok ? 0.0 : (double)N * to), (double)M * N,
                    (dtype == BGP_F64 ? 8 : dtype == BGP_F32 ? 4 : 2) * (C ? 2 : 1), 1};
-  const Plan plan = make_plan(q, [&](int b) { return (double)((M + b - 1) / b) * ((N + b - 1) / b); });
+  const auto tiles = [&](int b) { return (double)((M + b - 1) / b) * ((N + b - 1) / b); };
+  const Plan plan = make_plan(q, tiles, tiles);
+  if (plan.cut == CUTS) return bgp_products_fail(-1, "%s: M=%lld N=%lld are more tiles than one launch holds", what, (long long)M, (long long)N);
   Int8Args p{A, B, scale_a, scale_b, C, Y, M, N, K, lda, ldb, ldc, ldy, 0};
   Workspace ws(workspace);
   PackJob jobs[2];
@@ -495,7 +504,8 @@ extern "C" int64_t bgp_int8_gemm(int device, void* stream, int dtype, int64_t M,
     p.ldb = to;
     jobs[count++] = PackJob{B, const_cast<int8_t*>(p.b), N, N, 0, ldb, K, to};
   }
-  if (ws.used() > 0 && (!workspace || workspace_bytes < ws.used())) return ws.used();
+  if (ws.short_of(workspace_bytes)) return ws.used();
+  if (!ws.aligned()) return bgp_products_fail(-1, "%s: the workspace is not aligned to 16 bytes", what);
   DeviceScope scope(device);
   if (int rc = scope.check(what)) return rc;
   const hipStream_t st = static_cast<hipStream_t>(stream);

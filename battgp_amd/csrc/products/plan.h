@@ -27,9 +27,10 @@ constexpr float ALONE_US[4][CUTS] = {{0.12f, 0.22f, 0.52f, 1.0f, 0.30f, 0.62f, 1
 constexpr float LAUNCH_US = 3.0f, PACK_US = 2.0f, COPY_BYTES_US = 3.5e6f;
 constexpr float OUT_BYTES_US = 20e3f;  // a CU's results to memory and back, with more than 4 waves at it
 constexpr int CUS = 256;
+constexpr int64_t MOST_TILES = (1 << 23) - 1 - CUS;  // the threads of a launch (512 to a workgroup) are counted in 32 bits
 
 struct Plan {
-  int cut = PLAIN64, split = 1;
+  int cut = CUTS, split = 1;  // CUTS: more tiles than one launch holds, however it is cut
   bool pack = false;
 };
 
@@ -44,8 +45,8 @@ struct Question {
   int most_split;          // 1: k is not cut
 };
 
-// tiles: double(int b)
-template <class F> Plan make_plan(const Question& q, F&& tiles) {
+// double(int b), of tiles: how many are expected, and how many there may be at most
+template <class F, class M> Plan make_plan(const Question& q, F&& tiles, M&& most) {
   Plan best;
   double least = 1e30;
   const int kind = kind_of(q.size);
@@ -55,6 +56,7 @@ template <class F> Plan make_plan(const Question& q, F&& tiles) {
     const bool pipe = cut >= PIPE64, pack = pipe && !q.pipe;
     if (pack && !q.packable) continue;
     if ((cut == PLAIN64 || cut == PLAIN128) && q.pipe) continue;
+    if (most(tile_of(cut)) > MOST_TILES) continue;
     const double unit = tiles(tile_of(cut));
     for (int split = 1; split <= (cut <= DIRECT32 ? 1 : q.most_split); split *= 2) {
       if (split > 1 && stages < 4.0 * split) break;

@@ -632,3 +632,27 @@ def test_graph_replays_with_workspaces(products):
         eager = (first(), second())
         torch.cuda.synchronize()
         assert torch.equal(graphs[0][1], eager[0]) and torch.equal(graphs[1][1], eager[1])
+
+
+def test_rows_of_more_than_one_launch_are_quantised(products):
+    """67 million rows of one number: the code is 127 or -127, the scale the number's 127th part.  (The quotient in 64 bits
+    is not rounded across an fp32 midpoint m: a / 127 - m is a whole multiple of m's last place / 254, or 0.)"""
+    m = 4 * ((1 << 24) - 1) + 5
+    x = torch.randint(-64, 65, (m, 1), device="cuda", generator=torch.Generator("cuda").manual_seed(5), dtype=torch.int8).to(torch.bfloat16)
+    q, scale = products.quantize_rows(x)
+    assert torch.equal(q[:, 0], torch.sign(x[:, 0]).to(torch.int8) * 127)
+    want = (x[:, 0].double().abs() / 127).float().clamp_min(torch.finfo(torch.float32).tiny)
+    assert torch.equal(scale, want)
+
+
+def test_more_row_tiles_than_the_smallest_cut_could_launch(products):
+    t, n, k = 150_000_001, 8, 8
+    x = torch.randint(-4, 5, (t, k), device="cuda", generator=torch.Generator("cuda").manual_seed(6), dtype=torch.int8).to(torch.bfloat16)
+    w = whole((2, n, k), 7, dtype=torch.bfloat16).cuda()
+    cut = 75_000_005
+    y = products.grouped_matmul(x, w, torch.tensor([0, cut, t - 3], device="cuda"))
+    for a, b, g in ((0, cut, 0), (cut, t - 3, 1)):
+        for i in range(a, b, 25_000_000):
+            j = min(i + 25_000_000, b)  # sums of 8 products up to 16: exact in bf16 (128 < 256)
+            assert torch.equal(y[i:j], (x[i:j].float() @ w[g].float().T).to(torch.bfloat16))
+    assert not y[t - 3:].any()

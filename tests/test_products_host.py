@@ -96,6 +96,64 @@ def test_nothing_to_do_is_no_error(name, base, change):
     assert getattr(_lib.load_products(), name)(*{**base, **change}.values()) == 0
 
 
+MANY = 1 << 40
+
+
+@pytest.mark.parametrize("name, base, change", [
+    ("bgp_grouped_gemm", GEMM, dict(T=MANY)),
+    ("bgp_grouped_gemm", GEMM, dict(T=MANY, X=C.c_void_p(4098), ldx=5)),  # operands that would be copied first
+    ("bgp_grouped_gemm", GEMM, dict(N=MANY, ldy=MANY, sW=4 * MANY)),
+    ("bgp_grouped_gemm_dw", DW, dict(N=1 << 20, K=1 << 20, lddy=1 << 20, ldx=1 << 20, ldw=1 << 20, sW=MANY)),
+    ("bgp_grouped_gemm_dw", DW, dict(G=65535, N=1 << 12, K=1 << 12, lddy=1 << 12, ldx=1 << 12, ldw=1 << 12, sW=1 << 24)),
+    ("bgp_int8_gemm", INT8, dict(M=MANY)),
+    ("bgp_int8_gemm", INT8, dict(M=MANY, N=MANY, ldy=MANY)),
+])
+def test_more_tiles_than_a_launch_holds_are_refused_before_anything_is_enqueued(name, base, change):
+    lib = _lib.load_products()
+    assert getattr(lib, name)(*{**base, **change}.values()) == -1
+    assert "launch" in lib.bgp_products_last_error().decode()
+
+
+def test_many_tiles_that_a_launch_holds_are_taken():
+    """2e8 rows of 16 numbers to 16: too many tiles of 16 rows, which the sizes would ask for, but not of 64 or 128"""
+    lib = _lib.load_products()
+    rc = lib.bgp_grouped_gemm(*{**GEMM, "T": 200_000_000, "N": 16, "K": 16, "ldx": 16, "ldw": 16, "ldy": 16, "sW": 256, "device": 4095}.values())
+    assert rc == -2  # it got as far as the device
+
+
+@pytest.mark.parametrize("name, base, change", [
+    # operands off the 16-byte chunks and long enough to be copied
+    ("bgp_grouped_gemm", GEMM, dict(dtype=2, T=8192, N=2049, K=2049, X=C.c_void_p(4098), ldx=2049, ldw=2049, sW=2049 * 2049, ldy=2049)),
+    ("bgp_int8_gemm", INT8, dict(M=4097, N=4097, K=4097, A=C.c_void_p(4097), lda=4097, ldb=4097, ldy=4097)),
+])
+def test_workspaces_off_their_alignment_are_refused(name, base, change):
+    lib = _lib.load_products()
+    args = {**base, **change}
+    need = getattr(lib, name)(*args.values())
+    assert need > 0 and getattr(lib, name)(*{**args, "ws": P, "wsb": need - 1}.values()) == need
+    assert getattr(lib, name)(*{**args, "ws": C.c_void_p(4104), "wsb": need}.values()) == -1
+    assert "workspace" in lib.bgp_products_last_error().decode()
+
+
+def test_added_in_place_with_another_leading_dimension_is_refused():
+    lib = _lib.load_products()
+    assert lib.bgp_int8_gemm(*{**INT8, "C": P, "ldc": 5}.values()) == -1
+    assert "strides" in lib.bgp_products_last_error().decode()
+
+
+@pytest.mark.parametrize("call", [
+    lambda t: products.grouped_matmul(t, torch.ones(1, 4, 3), torch.tensor([0, 6])),
+    lambda t: products.quantize_rows(t),
+])
+def test_lazily_negated_tensors_are_refused(recorder, call):
+    """the imaginary part of a conjugate: its memory holds the opposite of its values"""
+    t = torch.complex(torch.ones(6, 3), torch.ones(6, 3)).conj().imag
+    assert t.is_neg()
+    with pytest.raises(ValueError, match="own values"):
+        call(t)
+    assert not recorder.calls
+
+
 class Recorder:
     """Stands for the library on the CPU: keeps the last call's arguments by the header's names."""
 
