@@ -34,6 +34,15 @@ struct Plan {
   bool pack = false;
 };
 
+// Rounds of a chip full of tiles.  The last round of 256 x 256 tiles is cut into parts where its tiles are few (entry.h,
+// place_256): by their stages a quarter takes 0.35 and a half 0.6 of a whole one (16 groups of 512 rows, 2048 x 2048 in bf16, 320
+// tiles expected: 62 us against 68 in tiles of 128, which two whole rounds would say to take).
+inline double rounds_of(int cut, double units) {
+  if (cut != PIPE256) return ceil(units / CUS);
+  const double whole = floor(units / CUS), left = (units - whole * CUS) / CUS;
+  return whole + (left == 0 ? 0 : left <= 0.25 ? 0.35 : left <= 0.5 ? 0.6 : 1);
+}
+
 // What the model is asked: D in tiles of b x b has tiles(b) of them; k bytes of k each.
 struct Question {
   int size;                // of an element
@@ -60,7 +69,7 @@ template <class F, class M> Plan make_plan(const Question& q, F&& tiles, M&& mos
     const double unit = tiles(tile_of(cut));
     for (int split = 1; split <= (cut <= DIRECT32 ? 1 : q.most_split); split *= 2) {
       if (split > 1 && stages < 4.0 * split) break;
-      const double each = ceil(unit * split / CUS), deep = ceil(stages / split);
+      const double each = rounds_of(cut, unit * split), deep = ceil(stages / split);
       double stage = each * STAGE_US[kind][cut];
       if (stage < ALONE_US[kind][cut]) stage = ALONE_US[kind][cut];
       const double tile_bytes = each * tile_of(cut) * tile_of(cut) * (split > 1 ? (q.size == 8 ? 8 : 4) : q.out_bytes);
