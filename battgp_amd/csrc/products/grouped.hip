@@ -145,8 +145,8 @@ template <class T, int BM, int BN, bool WK> __global__ __launch_bounds__(tile_th
 }
 
 // operands in whole chunks, pipelined
-template <class T, int BM, int BN, bool WK> __global__ __launch_bounds__(tile_threads(BM, sizeof(T)), 2) void grouped_rows_pipe_kernel(GroupedArgs p) {
-  using P = PipeTile<T, BM, BN, 2, waves_w(BM, sizeof(T)), true, WK>;
+template <class T, int BM, int BN, bool WK, int SETS> __global__ __launch_bounds__(SETS * tile_threads(BM, sizeof(T)), 2) void grouped_rows_pipe_kernel(GroupedArgs p) {
+  using P = PipeTile<T, BM, BN, 2, waves_w(BM, sizeof(T)), true, WK, SETS>;
   __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
   rows_workgroup<T, P, BM, BN, WK>(p, lds);
 }
@@ -248,8 +248,8 @@ template <class T, int BM, int BN> __global__ __launch_bounds__(tile_threads(BM,
   dw_workgroup<T, P, BM, BN>(p, lds);
 }
 
-template <class T, int BM, int BN> __global__ __launch_bounds__(tile_threads(BM, sizeof(T)), 2) void grouped_dw_pipe_kernel(GroupedArgs p) {
-  using P = PipeTile<T, BM, BN, 2, waves_w(BM, sizeof(T)), false, false>;
+template <class T, int BM, int BN, int SETS> __global__ __launch_bounds__(SETS * tile_threads(BM, sizeof(T)), 2) void grouped_dw_pipe_kernel(GroupedArgs p) {
+  using P = PipeTile<T, BM, BN, 2, waves_w(BM, sizeof(T)), false, false, SETS>;
   __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
   dw_workgroup<T, P, BM, BN>(p, lds);
 }
@@ -357,7 +357,7 @@ template <class T> int join(const char* what, const JoinArgs& j, hipStream_t st)
 
 template <class T, bool WK, int CUT> int run_rows(const GroupedArgs& p0, hipStream_t st) {
   const char* what = "bgp_grouped_gemm";
-  constexpr int B = tile_of(CUT);
+  constexpr int B = tile_of(CUT), SETS = CUT == TWIN64 ? 2 : 1;
   GroupedArgs p = p0;
   p.tiles_n = (int)((p.N + B - 1) / B);
   // row tiles there can be at most: a group adds less than one to its share of the rows
@@ -374,7 +374,7 @@ template <class T, bool WK, int CUT> int run_rows(const GroupedArgs& p0, hipStre
   } else if constexpr (CUT == PIPE256) {
     return launch(what, grouped_rows_pipe256_kernel<T, WK>, grid, dim3(512), st, p);
   } else {
-    return launch(what, grouped_rows_pipe_kernel<T, B, B, WK>, grid, dim3(tile_threads(B, sizeof(T))), st, p);
+    return launch(what, grouped_rows_pipe_kernel<T, B, B, WK, SETS>, grid, dim3(SETS * tile_threads(B, sizeof(T))), st, p);
   }
 }
 
@@ -385,8 +385,10 @@ template <class T, bool WK> int rows_by_cut(const GroupedArgs& p, int cut, hipSt
   }
   if (cut == PLAIN64) return run_rows<T, WK, PLAIN64>(p, st);
   if (cut == PLAIN128) return run_rows<T, WK, PLAIN128>(p, st);
-  if constexpr (sizeof(T) == 2)
+  if constexpr (sizeof(T) == 2) {
     if (cut == PIPE256) return run_rows<T, WK, PIPE256>(p, st);
+    if (cut == TWIN64) return run_rows<T, WK, TWIN64>(p, st);
+  }
   return cut == PIPE64 ? run_rows<T, WK, PIPE64>(p, st) : run_rows<T, WK, PIPE128>(p, st);
 }
 
@@ -398,7 +400,7 @@ template <class T> int run_rows_plan(const GroupedArgs& p, bool trans, const Pla
 
 template <class T, int CUT> int run_dw(const GroupedArgs& p0, hipStream_t st) {
   const char* what = "bgp_grouped_gemm_dw";
-  constexpr int B = tile_of(CUT);
+  constexpr int B = tile_of(CUT), SETS = CUT == TWIN64 ? 2 : 1;
   GroupedArgs p = p0;
   p.tiles_n = (int)((p.N + B - 1) / B);
   const int64_t tiles = (int64_t)p.G * p.tiles_n * ((p.K + B - 1) / B) + (B == 256 ? CUS : 8 * DEALT - 1);
@@ -406,7 +408,7 @@ template <class T, int CUT> int run_dw(const GroupedArgs& p0, hipStream_t st) {
   if constexpr (CUT <= DIRECT32) return launch(what, grouped_dw_direct_kernel<T, B / 16>, grid, dim3(256), st, p);
   else if constexpr (CUT <= PLAIN128) return launch(what, grouped_dw_kernel<T, B, B>, grid, dim3(tile_threads(B, sizeof(T))), st, p);
   else if constexpr (CUT == PIPE256) return launch(what, grouped_dw_pipe256_kernel<T>, grid, dim3(512), st, p);
-  else return launch(what, grouped_dw_pipe_kernel<T, B, B>, grid, dim3(tile_threads(B, sizeof(T))), st, p);
+  else return launch(what, grouped_dw_pipe_kernel<T, B, B, SETS>, grid, dim3(SETS * tile_threads(B, sizeof(T))), st, p);
 }
 
 template <class T> int dw_by_cut(const GroupedArgs& p, int cut, hipStream_t st) {
@@ -416,8 +418,10 @@ template <class T> int dw_by_cut(const GroupedArgs& p, int cut, hipStream_t st) 
   }
   if (cut == PLAIN64) return run_dw<T, PLAIN64>(p, st);
   if (cut == PLAIN128) return run_dw<T, PLAIN128>(p, st);
-  if constexpr (sizeof(T) == 2)
+  if constexpr (sizeof(T) == 2) {
     if (cut == PIPE256) return run_dw<T, PIPE256>(p, st);
+    if (cut == TWIN64) return run_dw<T, TWIN64>(p, st);
+  }
   return cut == PIPE64 ? run_dw<T, PIPE64>(p, st) : run_dw<T, PIPE128>(p, st);
 }
 
@@ -427,8 +431,10 @@ template <class T> int run_dw_plan(const GroupedArgs& p, const Plan& plan, hipSt
   return join<T>("bgp_grouped_gemm_dw", JoinArgs{p.part, const_cast<void*>(p.w), p.G * p.N, p.K, p.N, p.sw, p.ldw, p.split, nullptr, p.G, 0}, st);
 }
 
-// Row tiles of b rows that are expected: every group with rows has one at least and half of one to spare.
+// Row tiles of b rows that are expected: every group with rows has one at least and half of one to spare, a single one is
+// taken to hold all rows.
 double expected_tiles(int64_t T, int64_t G, int b) {
+  if (G == 1) return ceil((double)T / b);
   const double used = (double)(G < T ? G : T), even = (double)T / b + 0.5 * used;
   return even > used ? even : used;
 }

@@ -369,8 +369,8 @@ template <class T, int BM, int BN> __global__ __launch_bounds__(256, 2) void int
 }
 
 // operands in whole chunks, pipelined
-template <class T, int BM, int BN> __global__ __launch_bounds__(tile_threads(BM, 1), 2) void int8_gemm_pipe_kernel(Int8Args p) {
-  using P = PipeTile<int8_t, BM, BN, 2, waves_w(BM, 1), true, true>;
+template <class T, int BM, int BN, int SETS> __global__ __launch_bounds__(SETS * tile_threads(BM, 1), 2) void int8_gemm_pipe_kernel(Int8Args p) {
+  using P = PipeTile<int8_t, BM, BN, 2, waves_w(BM, 1), true, true, SETS>;
   __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
   int8_workgroup<T, P, BM, BN>(p, lds);
 }
@@ -384,7 +384,7 @@ template <class T, int F, bool ODD> __global__ __launch_bounds__(256) void int8_
 
 template <class T, int CUT> int run_int8(const Int8Args& p0, hipStream_t st) {
   const char* what = "bgp_int8_gemm";
-  constexpr int B = tile_of(CUT);
+  constexpr int B = tile_of(CUT), SETS = CUT == TWIN64 ? 2 : 1;
   Int8Args p = p0;
   p.tiles_n = (int)((p.N + B - 1) / B);
   const int64_t tiles = (p.M + B - 1) / B * p.tiles_n + (B == 256 ? CUS : 7);
@@ -398,7 +398,7 @@ template <class T, int CUT> int run_int8(const Int8Args& p0, hipStream_t st) {
   } else if constexpr (CUT == PIPE256) {
     return launch(what, int8_gemm_pipe256_kernel<T>, grid, dim3(512), st, p);
   } else {
-    return launch(what, int8_gemm_pipe_kernel<T, B, B>, grid, dim3(tile_threads(B, 1)), st, p);
+    return launch(what, int8_gemm_pipe_kernel<T, B, B, SETS>, grid, dim3(SETS * tile_threads(B, 1)), st, p);
   }
 }
 
@@ -410,6 +410,7 @@ template <class T> int run_int8_cut(const Int8Args& p, int cut, hipStream_t st) 
     case PLAIN128: return run_int8<T, PLAIN128>(p, st);
     case PIPE64: return run_int8<T, PIPE64>(p, st);
     case PIPE128: return run_int8<T, PIPE128>(p, st);
+    case TWIN64: return run_int8<T, TWIN64>(p, st);
     default: return run_int8<T, PIPE256>(p, st);
   }
 }

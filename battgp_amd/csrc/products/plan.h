@@ -5,10 +5,10 @@
 #include <stdint.h>
 
 // Straight from memory in tiles of 16 or 32, through registers (any operands) or pipelined (16-byte aligned rows) in tiles
-// of 64, 128 or 256.
-enum Cut { DIRECT16, DIRECT32, PLAIN64, PLAIN128, PIPE64, PIPE128, PIPE256, CUTS };
+// of 64, 128 or 256, or of 64 with k halved between two sets of waves.
+enum Cut { DIRECT16, DIRECT32, PLAIN64, PLAIN128, PIPE64, PIPE128, PIPE256, TWIN64, CUTS };
 constexpr int tile_of(int cut) {
-  return cut == DIRECT16 ? 16 : cut == DIRECT32 ? 32 : cut == PLAIN64 || cut == PIPE64 ? 64 : cut == PIPE256 ? 256 : 128;
+  return cut == DIRECT16 ? 16 : cut == DIRECT32 ? 32 : cut == PLAIN64 || cut == PIPE64 || cut == TWIN64 ? 64 : cut == PIPE256 ? 256 : 128;
 }
 constexpr int kind_of(int size) { return size == 1 ? 0 : size == 2 ? 1 : size == 4 ? 2 : 3; }
 
@@ -16,14 +16,15 @@ constexpr int kind_of(int size) { return size == 1 ? 0 : size == 2 ? 1 : size ==
 // from stage to stage of a tile that has its CU to itself.  {int8, 16 bits, fp32, fp64}, by Cut.  In TFLOP/s of the whole
 // chip the first row of e.g. PIPE128 is 2138, 925, 148 and 71, of DIRECT32 271, 190, 65 and 41; PLAIN* were measured
 // on operands that are not aligned, since the others are pipelined.
-constexpr float STAGE_US[4][CUTS] = {{0.115f, 0.247f, 0.40f, 0.95f, 0.187f, 0.50f, 1.68f},
-                                     {0.075f, 0.177f, 0.39f, 0.87f, 0.228f, 0.58f, 1.78f},
-                                     {0.090f, 0.260f, 0.61f, 2.20f, 0.476f, 1.82f, 9e9f},
-                                     {0.075f, 0.200f, 0.60f, 2.20f, 0.470f, 1.90f, 9e9f}};
-constexpr float ALONE_US[4][CUTS] = {{0.12f, 0.22f, 0.52f, 1.0f, 0.30f, 0.62f, 1.7f},
-                                     {0.10f, 0.20f, 0.68f, 1.1f, 0.47f, 0.59f, 1.8f},
-                                     {0.12f, 0.27f, 0.85f, 2.5f, 0.61f, 2.06f, 9e9f},
-                                     {0.10f, 0.23f, 0.88f, 2.5f, 0.59f, 1.95f, 9e9f}};
+constexpr float STAGE_US[4][CUTS] = {{0.115f, 0.247f, 0.40f, 0.95f, 0.187f, 0.50f, 1.68f, 0.24f},
+                                     {0.075f, 0.177f, 0.39f, 0.87f, 0.228f, 0.58f, 1.78f, 0.25f},
+                                     {0.090f, 0.260f, 0.61f, 2.20f, 0.476f, 1.82f, 9e9f, 9e9f},
+                                     {0.075f, 0.200f, 0.60f, 2.20f, 0.470f, 1.90f, 9e9f, 9e9f}};
+constexpr float ALONE_US[4][CUTS] = {{0.12f, 0.22f, 0.52f, 1.0f, 0.30f, 0.62f, 1.7f, 0.24f},
+                                     {0.10f, 0.20f, 0.68f, 1.1f, 0.47f, 0.59f, 1.8f, 0.25f},
+                                     {0.12f, 0.27f, 0.85f, 2.5f, 0.61f, 2.06f, 9e9f, 9e9f},
+                                     {0.10f, 0.23f, 0.88f, 2.5f, 0.59f, 1.95f, 9e9f, 9e9f}};
+constexpr float TWIN_US = 0.3f;  // filling its buffers and adding up
 constexpr float LAUNCH_US = 3.0f, PACK_US = 2.0f, COPY_BYTES_US = 3.5e6f;
 constexpr float OUT_BYTES_US = 20e3f;  // a CU's results to memory and back, with more than 4 waves at it
 constexpr int CUS = 256;
@@ -69,11 +70,13 @@ template <class F, class M> Plan make_plan(const Question& q, F&& tiles, M&& mos
     const double unit = tiles(tile_of(cut));
     for (int split = 1; split <= (cut <= DIRECT32 ? 1 : q.most_split); split *= 2) {
       if (split > 1 && stages < 4.0 * split) break;
-      const double each = rounds_of(cut, unit * split), deep = ceil(stages / split);
+      if (cut == TWIN64 && unit * split > CUS) break;  // a CU holds one of these: two of PIPE64 would overlap
+      const double each = rounds_of(cut, unit * split), sets = cut == TWIN64 ? 2 : 1, deep = sets * ceil(ceil(stages / split) / sets);
       double stage = each * STAGE_US[kind][cut];
       if (stage < ALONE_US[kind][cut]) stage = ALONE_US[kind][cut];
       const double tile_bytes = each * tile_of(cut) * tile_of(cut) * (split > 1 ? (q.size == 8 ? 8 : 4) : q.out_bytes);
       double us = LAUNCH_US + deep * stage + tile_bytes / (each > 1 || cut == PIPE256 ? OUT_BYTES_US : OUT_BYTES_US / 2);
+      if (cut == TWIN64) us += TWIN_US;
       if (split > 1) us += LAUNCH_US + (split + 1) * q.outputs * (q.size == 8 ? 8 : 4) / COPY_BYTES_US;
       if (pack) us += PACK_US + 2 * q.pack_bytes / COPY_BYTES_US;
       if (us < least) {

@@ -427,10 +427,10 @@ template <class T, int BM, int BN, int WX, int WW, bool XK, bool WK> struct Tile
   }
 };
 
-// The same tile for operands whose rows start on 16 bytes and lie in whole chunks, as a pipeline: two buffers of a stage each, filled by loads
-// that write LDS themselves (global_load_lds, 16 bytes a lane: no registers, no LDS stores, one 32-bit offset per lane
-// and load against a scalar base) and issued a whole stage ahead; the fragments of the next half stage are read while the
-// matrix instructions of this one run.
+// The same tile for operands whose rows start on 16 bytes and lie in whole chunks, as a pipeline: two buffers of a stage
+// each, filled by loads that write LDS themselves (global_load_lds, 16 bytes a lane: no registers, no LDS stores, one 32-bit
+// offset per lane and load against a scalar base) and issued a whole stage ahead; the fragments of the next half stage
+// are read while the matrix instructions of this one run.
 //   first half of stage b:   read the fragments of its second half; multiply those of the first.
 //   second half:             wait until stage b + 1 has arrived and this wave's own fragment reads of stage b are done;
 //                            barrier: both hold for every wave, so b's buffer is free; issue stage b + 2 into it; read
@@ -443,17 +443,24 @@ template <class T, int BM, int BN, int WX, int WW, bool XK, bool WK> struct Tile
 // TFLOP/s).  With few stages to a tile, by filling the pipeline and by the results of one round of tiles, which go to
 // memory all at once: 18000 x 512 x 500 in fp64 runs at 60 TFLOP/s.  Workgroups of one CU at unlike wave priorities, to
 // pull those apart, were no faster (159 us against 154).
+// SETS = 2: two sets of waves halve k between them, each a pipeline of three buffers, and add up in LDS: for few tiles of
+// long k, where a CU has one workgroup and one set of 4 waves waits for its loads, LDS reads and barriers in turn
+// (1000 x 1024 x 4096 in bf16: 21 us against 32, and 27 with k cut over workgroups; where tiles fill the chip one set is
+// faster, 700 rows of 2 groups, 4096 x 4096: 43 us against 61).  32- and 64-bit types have enough to multiply in a stage
+// and gain nothing.
 // Offsets inside a stage have 32 bits: pipe_fits() says whether an operand's do.
-template <class T, int BM, int BN, int WX, int WW, bool XK, bool WK> struct PipeTile {
+template <class T, int BM, int BN, int WX, int WW, bool XK, bool WK, int SETS = 1> struct PipeTile {
+  static constexpr int NBUF = SETS == 1 ? 2 : 3;
   static constexpr int NW = WX * WW, NT = 64 * NW, FA = BM / WX / 16, FB = BN / WW / 16;
   static constexpr int KE = KSTAGE<T>;
   static constexpr int XL = BM / 8 / NW, WL = BN / 8 / NW;  // loads of a wave per stage
-  static constexpr int BUF = (BM + BN) * 128, LDS_BYTES = 2 * BUF;
+  static constexpr int BUF = (BM + BN) * 128, LDS_BYTES = SETS * NBUF * BUF, L = XL + WL;
   static_assert(BM / 8 % NW == 0 && BN / 8 % NW == 0, "every wave loads the same share of either operand");
   using acc_t = typename Num<T>::acc;
   acc_t acc[FB][FA];
 
-  __device__ __forceinline__ int wave() const { return __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); }
+  __device__ __forceinline__ int set() const { return SETS == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)(threadIdx.x / NT)); }
+  __device__ __forceinline__ int wave() const { return __builtin_amdgcn_readfirstlane((int)(SETS == 1 ? threadIdx.x >> 6 : threadIdx.x % NT >> 6)); }
   __device__ __forceinline__ int x0() const { return wave() / WW * (BM / WX); }
   __device__ __forceinline__ int w0() const { return wave() % WW * (BN / WW); }
 
@@ -492,13 +499,20 @@ template <class T, int BM, int BN, int WX, int WW, bool XK, bool WK> struct Pipe
     const int64_t klen = scalar64(k_length);
     if (klen <= 0) return;
     const int64_t whole = klen / KE * KE;
-    const bool tail = whole < klen;
-    const int stages = (int)(klen / KE) + tail;
-    const uint32_t base = (uint32_t)(uintptr_t)(BGP_LDS char*)lds + wave() * 1024;
+    // every set's share of the stages, the part that k ends with counted as the first
+    const int all = (int)(klen / KE) + (whole < klen), most = (all + SETS - 1) / SETS;
+    const int before = set() * most, stages = all - before < most ? all - before : most;  // < 1: none
+    const bool tail = whole < klen && set() == 0;
+    char* mine = lds + set() * (NBUF * BUF);
+    const uint32_t base = (uint32_t)(uintptr_t)(BGP_LDS char*)mine + wave() * 1024;
     Source<BM, XK> sx;
     Source<BN, WK> sw;
     sx.start(x, wave());
     sw.start(w, wave());
+    if (set() > 0) {
+      sx.p += (before - (whole < klen)) * sx.step;
+      sw.p += (before - (whole < klen)) * sw.step;
+    }
     auto issue = [&](int buf) {
       sx.issue(base + buf * BUF);
       sw.issue(base + buf * BUF + BM * 128);
@@ -508,15 +522,24 @@ template <class T, int BM, int BN, int WX, int WW, bool XK, bool WK> struct Pipe
       Stage<T, BN, WK, NT> tw;
       tx.fetch_store_end(lds, x, whole, klen);
       tw.fetch_store_end(lds + BM * 128, w, whole, klen);
-    } else {
+    } else if (SETS == 1 || stages > 0) {
       issue(0);
     }
-    if (stages > 1) issue(1);
-    if (stages > 1 && !tail) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(XL + WL) : "memory");
+#pragma unroll
+    for (int i = 1; i < NBUF; ++i)
+      if (i < stages) issue(i);
+    // stage 0 is there for every wave
+    if (stages >= NBUF && !tail) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((NBUF - 1) * L) : "memory");
     else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    // stage s + 1 is, and this wave's reads of stage s are done
+    auto arrive = [&](int s) {
+      if (NBUF > 2 && s + NBUF <= stages) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NBUF - 2) * L) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    };
+    auto after = [](int buf) { return NBUF == 2 ? buf ^ 1 : buf + 1 == NBUF ? 0 : buf + 1; };
     chunk_t fx[2][FA], fw[2][FB];
     auto read = [&](int buf, int half) {
-      const char* at = lds + buf * BUF;
+      const char* at = mine + buf * BUF;
 #pragma unroll
       for (int a = 0; a < FA; ++a) fx[half][a] = fragment<T, BM, XK>(at, x0() + a * 16, half);
 #pragma unroll
@@ -531,25 +554,50 @@ template <class T, int BM, int BN, int WX, int WW, bool XK, bool WK> struct Pipe
       __builtin_amdgcn_sched_barrier(0);
     };
     if (x0() >= x.rows || w0() >= w.rows) {  // none of this wave's elements exist: it only loads
-      for (int s = 0, buf = 0; s < stages; ++s, buf ^= 1) {
-        asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-        if (s + 2 < stages) issue(buf);
+      for (int s = 0, buf = 0; s < stages; ++s, buf = after(buf)) {
+        arrive(s);
+        if (s + NBUF < stages) issue(buf);
       }
-      asm volatile("s_barrier" ::: "memory");
-      return;
+      if constexpr (SETS == 1) {
+        asm volatile("s_barrier" ::: "memory");
+        return;
+      }
+    } else {
+      if (SETS == 1 || stages > 0) read(0, 0);
+      for (int s = 0, buf = 0; s < stages; ++s, buf = after(buf)) {
+        __builtin_amdgcn_sched_barrier(0);
+        read(buf, 1);
+        multiply(0);
+        arrive(s);
+        if (s + NBUF < stages) issue(buf);
+        __builtin_amdgcn_sched_barrier(0);
+        read(after(buf), 0);  // behind the last stage: whatever is there, not used
+        multiply(1);
+      }
     }
-    read(0, 0);
-    for (int s = 0, buf = 0; s < stages; ++s, buf ^= 1) {
-      __builtin_amdgcn_sched_barrier(0);
-      read(buf, 1);
-      multiply(0);
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      if (s + 2 < stages) issue(buf);
-      __builtin_amdgcn_sched_barrier(0);
-      read(buf ^ 1, 0);  // behind the last stage: whatever is there, not used
-      multiply(1);
-    }
+    if (SETS > 1)
+      for (int s = stages > 0 ? stages : 0; s < most; ++s) asm volatile("s_barrier" ::: "memory");
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (SETS > 1) add_sets(lds + LDS_BYTES / 2);
+  }
+
+  // the other sets' sums to the first's; `lds`: half of it, whose other half is free for `out`
+  __device__ __forceinline__ void add_sets(char* lds) {
+    static_assert(SETS == 1 || (SETS - 1) * NT * FA * FB * (int)sizeof(acc_t) <= LDS_BYTES / 2, "the sets' sums fit");
+    acc_t* at = reinterpret_cast<acc_t*>(lds) + (threadIdx.x & (NT - 1));
+#pragma unroll
+    for (int b = 0; b < FB; ++b)
+#pragma unroll
+      for (int a = 0; a < FA; ++a)
+        if (set() > 0) at[(((set() - 1) * FB + b) * FA + a) * NT] = acc[b][a];
+    __syncthreads();
+    if (set() == 0)
+#pragma unroll
+      for (int o = 0; o < SETS - 1; ++o)
+#pragma unroll
+        for (int b = 0; b < FB; ++b)
+#pragma unroll
+          for (int a = 0; a < FA; ++a) acc[b][a] += at[((o * FB + b) * FA + a) * NT];
   }
 
   // the order the scheduler is to give an iteration: the LDS reads spread evenly over the matrix instructions
@@ -565,8 +613,8 @@ template <class T, int BM, int BN, int WX, int WW, bool XK, bool WK> struct Pipe
   }
 
   template <int E, class F> __device__ __forceinline__ void out(char* lds, int64_t rows, F&& f) const {
-    constexpr int C = BN / WW, REGION = LDS_BYTES / NW;
-    hand_out<T, C, E, REGION, FA, FB>(acc, lds + wave() * REGION, x0(), w0(), rows, f);
+    constexpr int C = BN / WW, REGION = LDS_BYTES / (SETS > 1 ? 2 * NW : NW);
+    if (set() == 0) hand_out<T, C, E, REGION, FA, FB>(acc, lds + wave() * REGION, x0(), w0(), rows, f);
   }
 };
 

@@ -656,3 +656,45 @@ def test_more_row_tiles_than_the_smallest_cut_could_launch(products):
             j = min(i + 25_000_000, b)  # sums of 8 products up to 16: exact in bf16 (128 < 256)
             assert torch.equal(y[i:j], (x[i:j].float() @ w[g].float().T).to(torch.bfloat16))
     assert not y[t - 3:].any()
+
+
+# ---- few tiles of long k, whose k two sets of waves may halve: one stage, two, odd numbers of them, parts of one, ragged edges ----
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("k", [64, 72, 128, 136, 192, 200, 264, 1048, 2056, 4104])
+@pytest.mark.parametrize("counts, n", [([70, 0, 3, 64], 200), ([300], 1000), ([1], 264), ([65, 129], 72)])
+def test_few_tiles_of_long_k(products, dtype, k, counts, n):
+    """whole numbers again: |sums| <= 4 * 4104 < 2^24"""
+    off = np.concatenate(([0], np.cumsum(counts))).tolist()
+    t, g = off[-1], len(counts)
+    x, w = gpu_whole((t, k), 1, dtype, 2), gpu_whole((g, n, k), 2, dtype, 2)
+    ref, od = gpu_grouped_ref(x, w, off).to(dtype), torch.tensor(off, device="cuda")
+    assert torch.equal(products.grouped_matmul(x, w, od), ref)
+    assert torch.equal(products.grouped_matmul(x, w.transpose(1, 2).contiguous().transpose(1, 2), od), ref)
+    out, rim = guarded((t, n), dtype)
+    products.grouped_matmul(x, w.transpose(1, 2).contiguous().transpose(1, 2), od, out=out)
+    assert torch.equal(out, ref)
+    rim()
+
+
+@pytest.mark.parametrize("counts", [[1], [64], [65, 0, 128], [200, 1], [1000], [63, 2000]])
+@pytest.mark.parametrize("n, k", [(200, 136), (512, 520), (72, 64)])
+def test_weight_gradients_of_few_tiles(products, counts, n, k):
+    off = np.concatenate(([0], np.cumsum(counts))).tolist()
+    dy, x = gpu_whole((off[-1], n), 1, torch.bfloat16, 2), gpu_whole((off[-1], k), 2, torch.bfloat16, 2)
+    _, dw = products.grouped_matmul_grad(dy, x, gpu_whole((len(counts), n, k), 3, torch.bfloat16), torch.tensor(off, device="cuda"), need_dx=False)
+    want = torch.stack([dy[a:b].double().T @ x[a:b].double() for a, b in rows_of(off)])
+    assert torch.equal(dw, want.to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("k", [128, 144, 256, 400, 2000, 4112, 8016])
+@pytest.mark.parametrize("m, n", [(300, 1000), (65, 130), (500, 900)])
+@pytest.mark.parametrize("dtype", ALL)
+def test_few_tiles_of_long_k_in_8_bits(products, m, n, k, dtype):
+    gen = torch.Generator(device="cuda").manual_seed(k)
+    a, b = (torch.randint(-128, 128, s, device="cuda", generator=gen, dtype=torch.int8) for s in ((m, k), (n, k)))
+    small = torch.full((max(m, n),), 2.0 ** -7, device="cuda", dtype=torch.float64 if dtype == torch.float64 else torch.float32)
+    ref = a.double() @ b.double().T * 2.0 ** -14  # exact; its magnitude is below 8016 and above 2^-14: normal in every type
+    got = products.int8_matmul(a, b, small[:m], small[:n], dtype=dtype)
+    assert ((got.double() - ref).abs() <= (torch.finfo(dtype).eps / 2 if dtype != torch.float64 else 0) * ref.abs()).all()
