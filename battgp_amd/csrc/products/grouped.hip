@@ -464,10 +464,11 @@ extern "C" int64_t bgp_grouped_gemm(int device, void* stream, int dtype, int64_t
   if (ldx < K || ldy < N || ldw < (w_trans ? N : K) || strideW < 0)
     return bgp_products_fail(-1, "%s: bad strides ldx=%lld ldw=%lld strideW=%lld ldy=%lld", what, (long long)ldx, (long long)ldw, (long long)strideW, (long long)ldy);
   const int size = size_of(dtype);
+  if (G == 0) K = 0;  // no row has weights: zeros, and neither operand is read (or copied): X and W may be NULL
   Laid x(X, 1, 0, T, ldx, K, size, true), w(W, strideW ? G : 1, strideW, w_trans ? K : N, ldw, w_trans ? N : K, size, !w_trans);
   const bool wide = K * size >= 16 && (!w_trans || N * size >= 16);
-  const Question q{size, wide && (!w_trans || size >= 4), x.ok && w.ok, pipe_fits(padded_row(x.extent, size), size, true, 256) && pipe_fits(padded_row(w.extent, size), size, !w_trans, 256),
-                   (double)K, (x.bytes(size) + w.bytes(size)), (double)T * N, size, G > 0 ? 16 : 1};
+  const Question q{size, wide && (!w_trans || size >= 4), x.ok && w.ok,
+                   G > 0 && pipe_fits(padded_row(x.extent, size), size, true, 256) && pipe_fits(padded_row(w.extent, size), size, !w_trans, 256), (double)K, (x.bytes(size) + w.bytes(size)), (double)T * N, size, G > 0 ? 16 : 1};
   const Plan plan = make_plan(
       q, [&](int b) { return expected_tiles(T, G, b) * ((N + b - 1) / b); }, [&](int b) { return ((double)(T / b) + G + 2) * ((N + b - 1) / b); });
   if (plan.cut == CUTS) return bgp_products_fail(-1, "%s: T=%lld N=%lld are more tiles than one launch holds", what, (long long)T, (long long)N);

@@ -38,7 +38,8 @@ const char* bgp_products_last_error(void);
  *   Y[t, n] = sum_k X[t, k] W_g[n, k]           n < N
  * W_g[n, k] = W[g * strideW + n * ldw + k], or W[g * strideW + k * ldw + n] with w_trans != 0; strideW = 0 gives all
  * groups the same weights.  offsets[G + 1] lies on the device, ascending, in [0, T] (values outside are clamped);
- * groups may be empty.  Rows in no group are set to 0 with zero_rest != 0 and left as they are otherwise.
+ * groups may be empty.  Rows in no group are set to 0 with zero_rest != 0 and left as they are otherwise; with G = 0 that is
+ * every row, and X and W are not read (NULL will do).
  * All of one type; sums in fp32 (fp64 for BGP_F64), rounded once.
  * The gradient with respect to X is the same product of dY[T, N] with w_trans turned round (and N, K exchanged). */
 int64_t bgp_grouped_gemm(int device, void* stream, int dtype, int64_t T, int64_t N, int64_t K, int64_t G, const void* X, int64_t ldx, const void* W,

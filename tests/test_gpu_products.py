@@ -698,3 +698,22 @@ def test_few_tiles_of_long_k_in_8_bits(products, m, n, k, dtype):
     ref = a.double() @ b.double().T * 2.0 ** -14  # exact; its magnitude is below 8016 and above 2^-14: normal in every type
     got = products.int8_matmul(a, b, small[:m], small[:n], dtype=dtype)
     assert ((got.double() - ref).abs() <= (torch.finfo(dtype).eps / 2 if dtype != torch.float64 else 0) * ref.abs()).all()
+
+
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("wt", [False, True])
+@pytest.mark.parametrize("t, n, k", [(1500, 1201, 1301), (5, 7, 9), (1, 8, 0)])
+def test_without_groups_all_rows_are_zero(products, dtype, wt, t, n, k):
+    """sizes and rows off the 16-byte chunks, whose operands would be copied if there were any"""
+    x, dy = gpu_whole((t, k), 1, dtype), gpu_whole((t, n), 2, dtype)
+    w = torch.empty((0, k, n) if wt else (0, n, k), dtype=dtype, device="cuda")
+    w, off = w.transpose(1, 2) if wt else w, torch.zeros(1, dtype=torch.int64, device="cuda")
+    y = products.grouped_matmul(x, w, off)
+    assert y.shape == (t, n) and not y.any()
+    dx, dw = products.grouped_matmul_grad(dy, x, w, off)
+    assert dx.shape == (t, k) and not dx.any() and dw.shape == (0, n, k)
+    out, rim = guarded((t, n), dtype)
+    out.fill_(5.0)
+    products.grouped_matmul(x, w, off, out=out)
+    assert (out == 5.0).all()
+    rim()

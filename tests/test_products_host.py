@@ -294,3 +294,19 @@ def test_int8_functions_refuse_and_pass_on(recorder):
     assert q.dtype == torch.int8 and s.dtype == torch.float32 and recorder.calls[-1][1]["ldx"] == 9 and recorder.calls[-1][1]["rest"] is None
     q, s, r = products.quantize_rows(torch.ones(4, 8, dtype=torch.float64), pow2=True, residual=True)
     assert s.dtype == r.dtype == torch.float64 and recorder.calls[-1][1]["pow2"] == 1
+
+
+# ---- calls without groups ----
+
+
+@pytest.mark.parametrize("dtype, t, n, k", [(_lib.BF16, 8192, 2049, 2049), (_lib.F16, 4096, 4096, 4001), (_lib.F32, 3001, 2999, 2001), (_lib.F64, 2700, 1000, 1001)])
+@pytest.mark.parametrize("trans", [0, 1])
+@pytest.mark.parametrize("x", [None, C.c_void_p(4096 + 8)])
+def test_without_groups_no_operand_is_copied(dtype, t, n, k, trans, x):
+    """an empty tensor's pointer is NULL: of rows and weights off the 16-byte chunks nothing may be read for aligned copies"""
+    lib = _lib.load_products()
+    args = {**GEMM, "device": 4095, "dtype": dtype, "T": t, "N": n, "K": k, "G": 0, "X": x, "ldx": k, "W": None, "sW": 0, "ldw": n if trans else k, "trans": trans,
+            "ldy": n}
+    assert lib.bgp_grouped_gemm(*args.values()) == -2  # no workspace is asked for: it got as far as the device
+    assert lib.bgp_grouped_gemm(*{**args, "ws": P, "wsb": 1 << 40}.values()) == -2
+    assert lib.bgp_grouped_gemm(*{**args, "zero": 0}.values()) == 0  # nothing to do at all
