@@ -13,6 +13,7 @@ no function records an autograd graph, and inputs that ask for one are refused.
 from __future__ import annotations
 
 import torch
+from torch.autograd.graph import increment_version  # a given output is written in place: autograd is to notice
 
 from . import _lib
 from .engine import EngineError
@@ -137,6 +138,7 @@ def _grouped(device, dtype, x, w, offsets, out, t, n, k, g):
     else:
         y = _output(out, "out", (t, n), x.dtype, device, (x, w, offsets))
         ldy = _rows("out", y, t, n)
+        increment_version(y)
     _call(
         "bgp_grouped_gemm", x, device, _stream(device), dtype, t, n, k, g, x.data_ptr(), ldx, w.data_ptr(), sw, ldw, trans,
         offsets.data_ptr(), y.data_ptr(), ldy, out is None,
@@ -280,6 +282,7 @@ def int8_matmul(
             inputs.append(c)
         y = _output(out, "out", (m, n), dtype, device, inputs)
         ldy = _rows("out", y, m, n)
+        increment_version(y)
     _call(
         "bgp_int8_gemm", a, device, _stream(device), code, m, n, k, a.data_ptr(), lda, b.data_ptr(), ldb, a_scale.data_ptr(),
         b_scale.data_ptr(), cp, ldc, y.data_ptr(), ldy,

@@ -310,3 +310,36 @@ def test_without_groups_no_operand_is_copied(dtype, t, n, k, trans, x):
     assert lib.bgp_grouped_gemm(*args.values()) == -2  # no workspace is asked for: it got as far as the device
     assert lib.bgp_grouped_gemm(*{**args, "ws": P, "wsb": 1 << 40}.values()) == -2
     assert lib.bgp_grouped_gemm(*{**args, "zero": 0}.values()) == 0  # nothing to do at all
+
+
+# ---- outputs that are given ----
+
+
+def _given_outputs():
+    x, w, o = _case(n=3)
+    a, sa = torch.ones(4, 8, dtype=torch.int8), torch.ones(4)
+    yield torch.zeros(6, 3), lambda out: products.grouped_matmul(x, w, o, out=out)
+    yield torch.zeros(4, 4), lambda out: products.int8_matmul(a, a, sa, sa, dtype=torch.float32, out=out)
+    yield torch.zeros(4, 4), lambda out: products.int8_matmul(a, a, sa, sa, c=out, dtype=torch.float32, out=out)
+
+
+@pytest.mark.parametrize("case", range(3))
+def test_autograd_notices_a_given_output(recorder, case):
+    """what was saved for a backward pass and is then written over raises there, as after torch's own operations in place"""
+    out, call = list(_given_outputs())[case]
+    p = torch.ones_like(out).requires_grad_()
+    z = p * out  # keeps out for p's gradient
+    assert call(out) is out and recorder.calls
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.sum().backward()
+    (p * out).sum().backward()
+    view = out.view(-1)
+    call(out)
+    assert view._version == out._version == 2
+    with torch.inference_mode():  # keeps no versions
+        fresh = torch.zeros_like(out)
+        assert call(fresh) is fresh
+    wrong = torch.zeros(1, 1)
+    with pytest.raises(ValueError):
+        call(wrong)
+    assert wrong._version == 0
