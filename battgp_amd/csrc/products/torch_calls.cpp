@@ -17,12 +17,12 @@ namespace {
 
 using at::Tensor;
 
-// a dense tensor on the GPU that no gradient is recorded for; NULL if it is anything else
+// a dense tensor on the GPU that no gradient is recorded for, in neither mode; NULL if it is anything else
 const Tensor* gpu_tensor(PyObject* o, int dim, int device = -1) {
   if (!THPVariable_Check(o)) return nullptr;
   const Tensor& t = THPVariable_Unpack(o);
   if (t.layout() != at::kStrided || !t.is_cuda() || t.dim() != dim || (device >= 0 && t.get_device() != device)) return nullptr;
-  if (t.is_neg() || (t.requires_grad() && c10::GradMode::is_enabled())) return nullptr;
+  if (t.is_neg() || (t.requires_grad() && c10::GradMode::is_enabled()) || t._fw_grad(0).defined()) return nullptr;
   return &t;
 }
 

@@ -7,12 +7,13 @@ be captured into a graph and come from several threads.  The kernels run in libb
 (``include/battgp_products.h``); there is no fallback.  An ordinary call goes there by way of ``_products_torch``
 (``csrc/products/torch_calls.cpp``); whatever that does not take - an ``out``, a part of the gradients, a wrong argument - goes
 through the checks below.  Like the engine's ``lml_grad``, gradients are calls of their own:
-no function records an autograd graph, and inputs that ask for one are refused.
+no function records an autograd graph, and inputs that ask for one, or that carry a forward-mode tangent, are refused.
 """
 
 from __future__ import annotations
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 from torch.autograd.graph import increment_version  # a given output is written in place: autograd is to notice
 
 from . import _lib
@@ -61,6 +62,8 @@ def _gpu_tensor(name: str, t, dim: int, device: int | None = None) -> int:
             raise ValueError(f"{name} is on {t.device}, the other operands are on device {device}")
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} requires a gradient: battgp_amd.products records no autograd graph; detach it and call the gradient's function")
+    if unpack_dual(t).tangent is not None:
+        raise ValueError(f"{name} has a tangent: battgp_amd.products does not carry forward-mode gradients along")
     return at
 
 

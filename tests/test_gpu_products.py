@@ -717,3 +717,27 @@ def test_without_groups_all_rows_are_zero(products, dtype, wt, t, n, k):
     products.grouped_matmul(x, w, off, out=out)
     assert (out == 5.0).all()
     rim()
+
+
+def operands_of_every_call(products):
+    """ordinary calls, as the compiled way takes them, with their floating point operands"""
+    x, w, dy, off = gpu_whole((6, 3), 1, torch.float32), gpu_whole((2, 4, 3), 2, torch.float32), gpu_whole((6, 4), 3, torch.float32), torch.tensor([0, 2, 6], device="cuda")
+    a, s, c = gpu_whole((6, 3), 4, torch.int8), gpu_whole((6,), 5, torch.float32), gpu_whole((6, 6), 6, torch.float32)
+    return [
+        (lambda x, w: products.grouped_matmul(x, w, off), (x, w)),
+        (lambda dy, x, w: products.grouped_matmul_grad(dy, x, w, off), (dy, x, w)),
+        (lambda x: products.quantize_rows(x), (x,)),
+        (lambda sa, sb, c: products.int8_matmul(a, a, sa, sb, c=c, dtype=torch.float32), (s, s, c)),
+    ]
+
+
+@pytest.mark.parametrize("i", range(4))
+def test_tangents_are_refused(products, i):
+    import torch.autograd.forward_ad as fw
+
+    call, operands = operands_of_every_call(products)[i]
+    for j, t in enumerate(operands):
+        with fw.dual_level():
+            with pytest.raises(ValueError, match="tangent"):
+                call(*operands[:j], fw.make_dual(t, torch.ones_like(t)), *operands[j + 1:])
+            call(*operands)

@@ -343,3 +343,48 @@ def test_autograd_notices_a_given_output(recorder, case):
     with pytest.raises(ValueError):
         call(wrong)
     assert wrong._version == 0
+
+
+# ---- tensors that stand for something else than the numbers in their memory ----
+
+
+class Wrapped(torch.Tensor):
+    """a wrapper without memory of its own"""
+
+    @staticmethod
+    def __new__(cls, inner):
+        return torch.Tensor._make_wrapper_subclass(cls, inner.shape, dtype=inner.dtype, device=inner.device)
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        raise NotImplementedError
+
+
+def _operands():
+    """every call with its floating point operands"""
+    x, w, o = _case(n=3)
+    yield lambda x, w: products.grouped_matmul(x, w, o), (x, w)
+    yield lambda x, w, out: products.grouped_matmul(x, w, o, out=out), (x, w, torch.zeros(6, 3))
+    yield lambda dy, x, w: products.grouped_matmul_grad(dy, x, w, o), (torch.ones(6, 3), x, w)
+    yield lambda x: products.quantize_rows(x), (x,)
+    a = torch.ones(6, 3, dtype=torch.int8)
+    yield lambda sa, sb, c: products.int8_matmul(a, a, sa, sb, c=c, dtype=torch.float32), (torch.ones(6), torch.ones(6), torch.zeros(6, 6))
+
+
+CALLS = [(i, j) for i, (_, operands) in enumerate(_operands()) for j in range(len(operands))]
+
+
+@pytest.mark.parametrize("i, j", CALLS)
+def test_operands_with_tangents_are_refused(recorder, i, j):
+    import torch.autograd.forward_ad as fw
+
+    call, operands = list(_operands())[i]
+    with fw.dual_level():
+        dual = fw.make_dual(operands[j], torch.ones_like(operands[j]))
+        with pytest.raises(ValueError, match="tangent"):
+            call(*operands[:j], dual, *operands[j + 1:])
+        with torch.no_grad(), pytest.raises(ValueError, match="tangent"):  # does not turn forward mode off
+            call(*operands[:j], dual, *operands[j + 1:])
+        assert not recorder.calls
+        call(*operands)
+    assert recorder.calls
