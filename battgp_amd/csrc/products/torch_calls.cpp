@@ -23,6 +23,7 @@ const Tensor* gpu_tensor(PyObject* o, int dim, int device = -1) {
   const Tensor& t = THPVariable_Unpack(o);
   if (t.layout() != at::kStrided || !t.is_cuda() || t.dim() != dim || (device >= 0 && t.get_device() != device)) return nullptr;
   if (t.is_neg() || (t.requires_grad() && c10::GradMode::is_enabled()) || t._fw_grad(0).defined()) return nullptr;
+  if (!t.has_storage() || (t.numel() > 0 && !t.const_data_ptr())) return nullptr;  // inside vmap and its like, wrappers
   return &t;
 }
 

@@ -741,3 +741,18 @@ def test_tangents_are_refused(products, i):
             with pytest.raises(ValueError, match="tangent"):
                 call(*operands[:j], fw.make_dual(t, torch.ones_like(t)), *operands[j + 1:])
             call(*operands)
+
+
+@pytest.mark.parametrize("i", range(4))
+def test_transformed_operands_are_refused(products, i):
+    call, operands = operands_of_every_call(products)[i]
+    for j, t in enumerate(operands):
+        def with_one(v):
+            return call(*operands[:j], v, *operands[j + 1:])
+
+        with pytest.raises(ValueError, match="own values"):
+            torch.func.vmap(with_one)(t[None])
+        with pytest.raises(ValueError, match="own values|tangent"):
+            torch.func.jvp(with_one, (t,), (t,))
+        with pytest.raises(ValueError, match="gradient"):
+            torch.func.grad(lambda v: with_one(v)[0].sum())(t)

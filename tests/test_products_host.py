@@ -388,3 +388,21 @@ def test_operands_with_tangents_are_refused(recorder, i, j):
         assert not recorder.calls
         call(*operands)
     assert recorder.calls
+
+
+@pytest.mark.parametrize("i, j", CALLS)
+def test_operands_without_memory_are_refused(recorder, i, j):
+    call, operands = list(_operands())[i]
+
+    def with_one(t):
+        return call(*operands[:j], t, *operands[j + 1:])
+
+    with pytest.raises(ValueError, match="own values"):
+        with_one(Wrapped(operands[j]))
+    with pytest.raises(ValueError, match="own values"):
+        torch.func.vmap(with_one)(operands[j][None])
+    with pytest.raises(ValueError, match="own values|tangent"):
+        torch.func.jvp(with_one, (operands[j],), (operands[j],))
+    with pytest.raises(ValueError, match="gradient"):
+        torch.func.grad(lambda t: with_one(t)[0].sum())(operands[j])
+    assert not recorder.calls
