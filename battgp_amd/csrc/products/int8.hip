@@ -180,22 +180,17 @@ template <class T, bool POW2, int TPR, int U, bool LONG> __global__ __launch_bou
     for (int j = 0; j < 8; ++j) {
       F t = 0, left = f[j];
       if (finite) {
-        if (sizeof(F) == 8 && !POW2) {
-          t = rint(f[j] / scale);
-          left = fma(-t, scale, f[j]);
-        } else {
-          // The product with the reciprocal is a hair off the quotient, so t may be the wrong neighbour where the quotient
-          // lies next to a half; what is left over says so, and it is exact: a multiple of half the last place of
-          // the scale, not larger than the scale.  (A power of two: the product is exact, and t right.)
-          t = rint(f[j] * inv);
-          left = fma(-t, scale, f[j]);
-          if (!POW2) {
-            const F twice = fabs(left) * 2;
-            if (twice > scale || (twice == scale && ((int)t & 1))) {
-              const F up = left > 0 ? (F)1 : (F)-1;
-              t += up;
-              left = fma(-up, scale, left);
-            }
+        // The product with the reciprocal is a hair off the quotient, so t may be the wrong neighbour where the quotient
+        // lies next to a half; what is left over says so, and it is exact: a multiple of half the last place of
+        // the scale, not larger than the scale.  (A power of two: the product is exact, and t right.)
+        t = rint(f[j] * inv);
+        left = fma(-t, scale, f[j]);
+        if (!POW2) {
+          const F twice = fabs(left) * 2;
+          if (twice > scale || (twice == scale && ((int)t & 1))) {
+            const F up = left > 0 ? (F)1 : (F)-1;
+            t += up;
+            left = fma(-up, scale, left);
           }
         }
       } else {

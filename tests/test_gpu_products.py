@@ -756,3 +756,33 @@ def test_transformed_operands_are_refused(products, i):
             torch.func.jvp(with_one, (t,), (t,))
         with pytest.raises(ValueError, match="gradient"):
             torch.func.grad(lambda v: with_one(v)[0].sum())(t)
+
+
+def test_fp64_codes_next_to_a_half(products):
+    """quotients that 64 bits round to a half which they are not: the code is the nearest to the quotient itself"""
+    from fractions import Fraction
+
+    rng = np.random.default_rng(3)
+    rows, want = [], []
+    while len(rows) < 60:
+        top = float(rng.uniform(0.5, 2.0) * 2.0 ** rng.integers(-40, 40))
+        scale = top / 127.0
+        row, codes = [top], [127]
+        for half in np.arange(0.5, 127.0):
+            for x in (half * scale, float(np.nextafter(half * scale, 0.0)), float(np.nextafter(half * scale, np.inf))):
+                exact = Fraction(x) / Fraction(scale)
+                if x / scale == half and exact != Fraction(half):
+                    nearest = int(half) + (exact > Fraction(half))
+                    if nearest != int(np.rint(half)):
+                        row += [x, -x]
+                        codes += [nearest, -nearest]
+        if len(row) > 1:
+            rows.append(row[:9] + [0.0] * (9 - len(row)))
+            want.append(codes[:9] + [0] * (9 - len(codes)))
+    x = torch.tensor(rows, dtype=torch.float64)
+    q, s, r = products.quantize_rows(x.cuda(), residual=True)
+    assert torch.equal(s.cpu(), x[:, 0] / 127.0)
+    assert torch.equal(q.cpu(), torch.tensor(want, dtype=torch.int8))
+    for xi, qi, si, ri in zip(x.tolist(), q.tolist(), s.tolist(), r.tolist()):
+        for a, b, c in zip(xi, qi, ri):  # what is left over is a number of 64 bits: exact
+            assert Fraction(c) == Fraction(a) - b * Fraction(si)
