@@ -482,6 +482,8 @@ template <class T, int BM, int BN, int WX, int WW, bool XK, bool WK, int SETS = 
         else at[l] = (uint32_t)row * (uint32_t)(o.ld * (int)sizeof(T)) + (c < last / CHE<T> ? c : last / CHE<T>) * 16;
       }
     }
+    // m0, where the load takes its LDS address from, is a reserved register: the compiler keeps nothing in it, and a clobber
+    // list may not name it.  No other instruction of these kernels uses it (the static test of their assembly looks).
     __device__ __forceinline__ void issue(uint32_t lds) {
       const int64_t from = scalar64(reinterpret_cast<int64_t>(p));
 #pragma unroll

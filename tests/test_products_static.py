@@ -51,3 +51,18 @@ def test_workgroups_fit_a_cu_as_their_launches_assume(code):
             assert 2 * r["lds"] <= 160 * 1024 and 2 * r["vgpr"] <= 512, name
         else:
             assert r["lds"] <= 160 * 1024 and r["wg"] // 256 * r["vgpr"] <= 512, name
+
+
+def test_nothing_but_the_loads_into_lds_uses_m0(code):
+    """The inline assembly of those loads sets m0 and can not say so: it is a reserved register, which a clobber list may
+    not name.  The compiler keeps no value of its own in it, but may use it for an instruction that takes it unnamed."""
+    unnamed = re.compile(r"movrel|s_set_gpr_idx|gws|sendmsg|ttrace|addtid|\blds\b|_interp_")
+    for text in {r["text"] for r in code.values()}:
+        lines = [line.split(";")[0].strip() for line in text.split("\n")]
+        sets = [i for i, line in enumerate(lines) if re.search(r"\bm0\b", line)]
+        assert len(sets) > 100
+        for i in sets:
+            assert re.fullmatch(r"s_mov_b32 m0, s\d+", lines[i]) and lines[i + 1] == "s_nop 0" and lines[i + 2].startswith("global_load_lds_dwordx4 "), lines[i]
+        loads = [line for line in lines if "global_load_lds" in line]
+        assert len(loads) == len(sets)
+        assert not [line for line in lines if unnamed.search(line) and not line.startswith(".")]
