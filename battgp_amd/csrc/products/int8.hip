@@ -458,7 +458,8 @@ extern "C" int bgp_quantize_rows(int device, void* stream, int dtype, int64_t M,
   if (M < 0 || K < 0) return bgp_products_fail(-1, "%s: bad sizes M=%lld K=%lld", what, (long long)M, (long long)K);
   if (M == 0) return 0;
   if (!scale || (K > 0 && (!x || !q))) return bgp_products_fail(-1, "%s: null pointer", what);
-  if (ldx < K || ldq < K || (rest && ldr < K)) return bgp_products_fail(-1, "%s: bad strides ldx=%lld ldq=%lld ldr=%lld", what, (long long)ldx, (long long)ldq, (long long)ldr);
+  if (ldx < K || ldq < K || (rest && (ldr < K || (rest == x && ldr != ldx && M > 1))))
+    return bgp_products_fail(-1, "%s: bad strides ldx=%lld ldq=%lld ldr=%lld", what, (long long)ldx, (long long)ldq, (long long)ldr);
   DeviceScope scope(device);
   if (int rc = scope.check(what)) return rc;
   const QuantArgs p{x, q, scale, rest, M, K, ldx, ldq, ldr};

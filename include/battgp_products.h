@@ -55,7 +55,7 @@ int64_t bgp_grouped_gemm_dw(int device, void* stream, int dtype, int64_t T, int6
  *           at least the smallest normal number of its type
  *   q     = x / scale rounded to the nearest whole number, ties to even
  *   rest  = x - scale * q, if not NULL (exact where the scale is a power of two): what the next slice starts from;
- *           rest == x is allowed
+ *           rest == x (ldr == ldx) is allowed
  * A row that holds an infinity or a NaN gets that as its scale, codes 0 and NaN for its rest. */
 int bgp_quantize_rows(int device, void* stream, int dtype, int64_t M, int64_t K, const void* x, int64_t ldx, int8_t* q, int64_t ldq, void* scale, int pow2,
                       void* rest, int64_t ldr);

@@ -406,3 +406,14 @@ def test_operands_without_memory_are_refused(recorder, i, j):
     with pytest.raises(ValueError, match="gradient"):
         torch.func.grad(lambda t: with_one(t)[0].sum())(operands[j])
     assert not recorder.calls
+
+
+@pytest.mark.parametrize("m, ldr, fits", [(4, 9, False), (4, 8, True), (1, 9, True)])
+def test_rest_in_place_with_another_leading_dimension_is_refused(m, ldr, fits):
+    """a row of the rest would lie over rows of x that are still to be read; with one row there is no other"""
+    lib = _lib.load_products()
+    rc = lib.bgp_quantize_rows(*{**QUANT, "device": 4095, "M": m, "rest": P, "ldr": ldr}.values())
+    assert rc == (-2 if fits else -1)  # -2: it got as far as the device
+    if not fits:
+        assert "strides" in lib.bgp_products_last_error().decode()
+    assert lib.bgp_quantize_rows(*{**QUANT, "device": 4095, "M": m, "K": 0, "x": None, "q": None, "ldr": ldr}.values()) == -2  # no rest, and nothing to read
