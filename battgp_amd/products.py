@@ -115,9 +115,12 @@ def _span(t: torch.Tensor) -> tuple[int, int]:
     return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
 
 
-def _output(out, name: str, shape, dtype, device: int, inputs) -> torch.Tensor:
+def _output(out, name: str, shape, dtype, device: int, inputs, added=None) -> torch.Tensor:
+    """``out``, checked; it may be ``added`` itself, and lies apart from everything else"""
     if _gpu_tensor(name, out, len(shape)) != device or out.dtype is not dtype or tuple(out.shape) != shape:
         raise ValueError(f"{name}: {shape} of {dtype} on device {device} is wanted, got {tuple(out.shape)} of {out.dtype} on {out.device}")
+    if added is not None and not (added.data_ptr() == out.data_ptr() and added.stride() == out.stride()):
+        inputs = (*inputs, added)
     lo, hi = _span(out)
     for t in inputs:
         a, b = _span(t)
@@ -290,10 +293,7 @@ def int8_matmul(
     if out is None:
         y, ldy = a.new_empty((m, n), dtype=dtype), n or 1
     else:
-        inputs = [a, b, a_scale, b_scale]
-        if c is not None and not (out.data_ptr() == cp and out.stride() == c.stride()):
-            inputs.append(c)
-        y = _output(out, "out", (m, n), dtype, device, inputs)
+        y = _output(out, "out", (m, n), dtype, device, (a, b, a_scale, b_scale), c)
         ldy = _rows("out", y, m, n)
         increment_version(y)
     _call(

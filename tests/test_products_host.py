@@ -417,3 +417,15 @@ def test_rest_in_place_with_another_leading_dimension_is_refused(m, ldr, fits):
     if not fits:
         assert "strides" in lib.bgp_products_last_error().decode()
     assert lib.bgp_quantize_rows(*{**QUANT, "device": 4095, "M": m, "K": 0, "x": None, "q": None, "ldr": ldr}.values()) == -2  # no rest, and nothing to read
+
+
+def test_outputs_that_are_no_tensors_are_refused_as_such(recorder):
+    a, s, c = torch.ones(4, 8, dtype=torch.int8), torch.ones(4), torch.zeros(4, 4)
+    for bad in (c.numpy(), [0.0]):
+        with pytest.raises(TypeError, match="out is not a torch tensor"):
+            products.int8_matmul(a, a, s, s, c=c, dtype=torch.float32, out=bad)
+        with pytest.raises(TypeError, match="out is not a torch tensor"):
+            products.int8_matmul(a, a, s, s, dtype=torch.float32, out=bad)
+    with pytest.raises(ValueError, match="own values"):  # nor one that has no memory
+        products.int8_matmul(a, a, s, s, c=c, dtype=torch.float32, out=Wrapped(c))
+    assert not recorder.calls
