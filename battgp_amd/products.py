@@ -115,6 +115,20 @@ def _span(t: torch.Tensor) -> tuple[int, int]:
     return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
 
 
+def _between_columns(out: torch.Tensor, t: torch.Tensor) -> bool:
+    """Whether ``t`` lies beside the columns of ``out``: both in pieces that recur at the same distance in memory."""
+    pitch, width, size = out.stride(0) * out.element_size(), 1, t.element_size()
+    if pitch == 0:
+        return False
+    for n, stride in zip(t.shape, t.stride()):
+        if n > 1 and stride == 1:
+            width += n - 1
+        elif n > 1 and stride * size % pitch:
+            return False
+    at = (t.data_ptr() - out.data_ptr()) % pitch
+    return at >= out.shape[1] * out.element_size() and at + width * size <= pitch
+
+
 def _output(out, name: str, shape, dtype, device: int, inputs, added=None) -> torch.Tensor:
     """``out``, checked; it may be ``added`` itself, and lies apart from everything else"""
     if _gpu_tensor(name, out, len(shape)) != device or out.dtype is not dtype or tuple(out.shape) != shape:
@@ -124,7 +138,7 @@ def _output(out, name: str, shape, dtype, device: int, inputs, added=None) -> to
     lo, hi = _span(out)
     for t in inputs:
         a, b = _span(t)
-        if a < hi and lo < b:
+        if a < hi and lo < b and not _between_columns(out, t):
             raise ValueError(f"{name} overlaps an input")
     return out
 

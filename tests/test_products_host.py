@@ -429,3 +429,40 @@ def test_outputs_that_are_no_tensors_are_refused_as_such(recorder):
     with pytest.raises(ValueError, match="own values"):  # nor one that has no memory
         products.int8_matmul(a, a, s, s, c=c, dtype=torch.float32, out=Wrapped(c))
     assert not recorder.calls
+
+
+def test_outputs_between_the_columns_of_an_input(recorder):
+    """columns of one wide matrix are apart, though each reaches over the other's rows"""
+    buf, o = torch.zeros(6, 12), torch.tensor([0, 2, 6])
+    x, w = buf[:, 2:5], torch.ones(2, 4, 3)
+    for at in (5, 8):
+        out = buf[:, at:at + 4]
+        assert products.grouped_matmul(x, w, o, out=out) is out
+    out = torch.as_strided(buf, (5, 4), (12, 1), 10)  # the last two columns and the next row's first two
+    assert products.grouped_matmul(buf[:5, 2:5], w, o, out=out) is out
+    assert len(recorder.calls) == 3
+    for bad in (buf[:, 1:5], buf[:, 4:8], torch.as_strided(buf, (5, 4), (12, 1), 11), torch.as_strided(buf, (6, 4), (11, 1), 5)):
+        t = bad.shape[0]
+        with pytest.raises(ValueError, match="overlaps"):
+            products.grouped_matmul(x[:t], w, o, out=bad)
+    # weights between the columns of the output, in either order of their axes; scales in its last one
+    big = torch.zeros(24, 12)
+    out = big[:6, :4]
+    assert products.grouped_matmul(torch.ones(6, 3), torch.as_strided(big, (2, 4, 3), (48, 12, 1), 4), o, out=out) is out
+    assert products.grouped_matmul(torch.ones(6, 3), torch.as_strided(big, (2, 4, 3), (36, 1, 12), 4), o, out=out) is out
+    with pytest.raises(ValueError, match="overlaps"):
+        products.grouped_matmul(torch.ones(6, 3), torch.as_strided(big, (2, 4, 3), (48, 12, 1), 3), o, out=out)
+    with pytest.raises(ValueError, match="overlaps"):
+        products.grouped_matmul(torch.ones(6, 3), torch.as_strided(big, (2, 4, 3), (50, 12, 1), 4), o, out=out)
+    a = torch.ones(6, 8, dtype=torch.int8)
+    assert products.int8_matmul(a, a[:4], torch.ones(6), big[0, 4:8], dtype=torch.float32, out=out) is out
+    with pytest.raises(ValueError, match="overlaps"):
+        products.int8_matmul(a, a[:4], torch.ones(6), big[0, 3:7], dtype=torch.float32, out=out)
+    one = torch.zeros(24)  # a single row, whose stride says nothing
+    for stride in (0, 2, 24):
+        out = torch.as_strided(one, (1, 4), (stride, 1))
+        with pytest.raises(ValueError, match="overlaps"):
+            products.grouped_matmul(one[None, 3:6], w, o, out=out)
+        assert products.grouped_matmul(one[None, 4:7], w, o, out=out) is out
+    with pytest.raises(ValueError, match="overlaps"):  # both axes of the weights next to each other
+        products.grouped_matmul(torch.ones(6, 3), torch.as_strided(big, (2, 4, 3), (48, 12, 1), 4)[:, :, :], o, out=big[:6, 1:5])
