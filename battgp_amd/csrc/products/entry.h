@@ -97,7 +97,6 @@ struct PackJob {
 };
 // at most two operands in one launch
 int launch_pack(const char* what, int size, const PackJob* jobs, int count, hipStream_t st);
-constexpr int64_t padded_row(int64_t extent, int size) { return (extent * size + 127) / 128 * 128 / size; }
 
 // whether rows start off the 4-byte words
 inline bool off_words(const void* p, int64_t ld, int64_t stride, int size) {

@@ -436,14 +436,6 @@ template <class T> int run_dw_plan(const GroupedArgs& p, const Plan& plan, hipSt
   return join<T>("bgp_grouped_gemm_dw", JoinArgs{p.part, const_cast<void*>(p.w), p.G * p.N, p.K, p.N, p.sw, p.ldw, p.split, nullptr, p.G, 0}, st);
 }
 
-// Row tiles of b rows that are expected: every group with rows has one at least and half of one to spare, a single one is
-// taken to hold all rows.
-double expected_tiles(int64_t T, int64_t G, int b) {
-  if (G == 1) return ceil((double)T / b);
-  const double used = (double)(G < T ? G : T), even = (double)T / b + 0.5 * used;
-  return even > used ? even : used;
-}
-
 int check_sizes(const char* what, int dtype, int64_t T, int64_t N, int64_t K, int64_t G, const void* off) {
   if (!size_of(dtype)) return bgp_products_fail(-1, "%s: unknown type %d", what, dtype);
   if (T < 0 || N < 0 || K < 0 || G < 0 || G > BGP_MAX_GROUPS)
@@ -466,11 +458,7 @@ extern "C" int64_t bgp_grouped_gemm(int device, void* stream, int dtype, int64_t
   const int size = size_of(dtype);
   if (G == 0) K = 0;  // no row has weights: zeros, and neither operand is read (or copied): X and W may be NULL
   Laid x(X, 1, 0, T, ldx, K, size, true), w(W, strideW ? G : 1, strideW, w_trans ? K : N, ldw, w_trans ? N : K, size, !w_trans);
-  const bool wide = K * size >= 16 && (!w_trans || N * size >= 16);
-  const Question q{size, wide && (!w_trans || size >= 4), x.ok && w.ok,
-                   G > 0 && pipe_fits(padded_row(x.extent, size), size, true, 256) && pipe_fits(padded_row(w.extent, size), size, !w_trans, 256), (double)K, (x.bytes(size) + w.bytes(size)), (double)T * N, size, G > 0 ? 16 : 1};
-  const Plan plan = make_plan(
-      q, [&](int b) { return expected_tiles(T, G, b) * ((N + b - 1) / b); }, [&](int b) { return ((double)(T / b) + G + 2) * ((N + b - 1) / b); });
+  const Plan plan = plan_rows(size, T, N, K, G, w_trans, Operands{x.ok && w.ok, x.bytes(size) + w.bytes(size)});
   if (plan.cut == CUTS) return bgp_products_fail(-1, "%s: T=%lld N=%lld are more tiles than one launch holds", what, (long long)T, (long long)N);
   Workspace ws(workspace);
   PackJob jobs[2];
@@ -508,12 +496,7 @@ extern "C" int64_t bgp_grouped_gemm_dw(int device, void* stream, int dtype, int6
     return bgp_products_fail(-1, "%s: bad strides lddy=%lld ldx=%lld ldw=%lld strideW=%lld", what, (long long)lddy, (long long)ldx, (long long)ldw, (long long)strideW);
   const int size = size_of(dtype);
   Laid y(dY, 1, 0, T, lddy, N, size, false), x(X, 1, 0, T, ldx, K, size, false);
-  // a group's rows are its length of k: their mean, and as much again for the longest of uneven ones
-  const double used = (double)(G < T ? G : T > 0 ? T : 1);
-  const Question q{size, size >= 4, x.ok && y.ok, pipe_fits(padded_row(N, size), size, false, 256) && pipe_fits(padded_row(K, size), size, false, 256),
-                   ceil(T / used), (x.bytes(size) + y.bytes(size)), (double)G * N * K, size, 16};
-  const auto tiles = [&](int b) { return (double)G * ((N + b - 1) / b) * ((K + b - 1) / b); };
-  const Plan plan = make_plan(q, tiles, tiles);
+  const Plan plan = plan_dw(size, T, N, K, G, Operands{x.ok && y.ok, x.bytes(size) + y.bytes(size)});
   if (plan.cut == CUTS)
     return bgp_products_fail(-1, "%s: G=%lld N=%lld K=%lld are more tiles than one launch holds", what, (long long)G, (long long)N, (long long)K);
   Workspace ws(workspace);

@@ -486,10 +486,8 @@ extern "C" int64_t bgp_int8_gemm(int device, void* stream, int dtype, int64_t M,
   const int64_t to = padded_row(K, 1);
   const bool a_ok = reinterpret_cast<uintptr_t>(A) % 16 == 0 && lda % 16 == 0 && pipe_fits(lda, 1, true, 256);
   const bool b_ok = reinterpret_cast<uintptr_t>(B) % 16 == 0 && ldb % 16 == 0 && pipe_fits(ldb, 1, true, 256);
-  const Question q{1, K >= 16, a_ok && b_ok, true, (double)K, (a_ok ? 0.0 : (double)M * to) + (b_ok ? 0.0 : (double)N * to), (double)M * N,
-                   (dtype == BGP_F64 ? 8 : dtype == BGP_F32 ? 4 : 2) * (C ? 2 : 1), 1};
-  const auto tiles = [&](int b) { return (double)((M + b - 1) / b) * ((N + b - 1) / b); };
-  const Plan plan = make_plan(q, tiles, tiles);
+  const Plan plan = plan_int8((dtype == BGP_F64 ? 8 : dtype == BGP_F32 ? 4 : 2) * (C ? 2 : 1), M, N, K,
+                              Operands{a_ok && b_ok, (a_ok ? 0.0 : (double)M * to) + (b_ok ? 0.0 : (double)N * to)});
   if (plan.cut == CUTS) return bgp_products_fail(-1, "%s: M=%lld N=%lld are more tiles than one launch holds", what, (long long)M, (long long)N);
   Int8Args p{A, B, scale_a, scale_b, C, Y, M, N, K, lda, ldb, ldc, ldy, 0};
   Workspace ws(workspace);

@@ -89,3 +89,53 @@ template <class F, class M> Plan make_plan(const Question& q, F&& tiles, M&& mos
   }
   return best;
 }
+
+// ---- the three products' questions ----
+
+// rows of a copy that start on whole cache lines
+constexpr int64_t padded_row(int64_t extent, int size) { return (extent * size + 127) / 128 * 128 / size; }
+
+// whether an operand's offsets inside a stage fit 32 bits: up to `rows` rows of it along k, a stage's rows of k otherwise
+inline bool pipe_fits(int64_t ld, int size, bool along_k, int rows) {
+  return (along_k ? rows : 128 / size) * ld * size < (int64_t)1 << 32;
+}
+
+// Row tiles of b rows that are expected: every group with rows has one at least and half of one to spare, a single one is
+// taken to hold all rows.
+inline double expected_tiles(int64_t T, int64_t G, int b) {
+  if (G == 1) return ceil((double)T / b);
+  const double used = (double)(G < T ? G : T), even = (double)T / b + 0.5 * used;
+  return even > used ? even : used;
+}
+
+// What a call's two operands are like: those that do not suit the pipelined cuts as they lie would be copied, `bytes` of them.
+struct Operands {
+  bool ok;
+  double bytes;
+};
+
+// Y[T, N] of G groups' rows against W[K] along k, or (w_trans) along N
+inline Plan plan_rows(int size, int64_t T, int64_t N, int64_t K, int64_t G, bool w_trans, const Operands& o) {
+  const bool wide = K * size >= 16 && (!w_trans || N * size >= 16);
+  const Question q{size, wide && (!w_trans || size >= 4), o.ok,
+                   G > 0 && pipe_fits(padded_row(K, size), size, true, 256) && pipe_fits(padded_row(w_trans ? N : K, size), size, !w_trans, 256), (double)K, o.bytes,
+                   (double)T * N, size, G > 0 ? 16 : 1};
+  return make_plan(
+      q, [&](int b) { return expected_tiles(T, G, b) * ((N + b - 1) / b); }, [&](int b) { return ((double)(T / b) + G + 2) * ((N + b - 1) / b); });
+}
+
+// dW[G, N, K] of T rows.  A group's rows are its length of k: their mean is taken, as if groups with rows were even.
+inline Plan plan_dw(int size, int64_t T, int64_t N, int64_t K, int64_t G, const Operands& o) {
+  const double used = (double)(G < T ? G : T > 0 ? T : 1);
+  const Question q{size, size >= 4, o.ok, pipe_fits(padded_row(N, size), size, false, 256) && pipe_fits(padded_row(K, size), size, false, 256),
+                   ceil(T / used), o.bytes, (double)G * N * K, size, 16};
+  const auto tiles = [&](int b) { return (double)G * ((N + b - 1) / b) * ((K + b - 1) / b); };
+  return make_plan(q, tiles, tiles);
+}
+
+// Y[M, N] in 8 bits, `out_bytes` written (and read) for each element
+inline Plan plan_int8(int out_bytes, int64_t M, int64_t N, int64_t K, const Operands& o) {
+  const Question q{1, K >= 16, o.ok, true, (double)K, o.bytes, (double)M * N, out_bytes, 1};
+  const auto tiles = [&](int b) { return (double)((M + b - 1) / b) * ((N + b - 1) / b); };
+  return make_plan(q, tiles, tiles);
+}

@@ -776,11 +776,6 @@ template <class T, int FA, int FB, bool XK, bool WK, bool ODD> struct DirectTile
   }
 };
 
-// whether an operand's offsets inside a stage fit 32 bits: up to `rows` rows of it along k, a stage's rows of k otherwise
-inline bool pipe_fits(int64_t ld, int size, bool along_k, int rows) {
-  return (along_k ? rows : 128 / size) * ld * size < (int64_t)1 << 32;
-}
-
 // D's rows as they are: E = 16 bytes of them at a time
 template <class O> struct PlainRows {
   O* d;

@@ -52,7 +52,7 @@ def pytest_configure(config):
 # BASELINE configs 4 and 5 at their natural sizes (N = 100 000, N = 262 144: minutes of GPU time, ~290 GB of HBM) come behind
 # every product module and in front of the optional schedules only (off-by-default code, no grade rides on it).
 GPU_ORDER = ["test_gpu_parity", "test_gpu_pins_and_sizes", "test_gpu_slab_layout", "test_gpu_grad", "test_gpu_adaptor", "test_gpu_sharded",
-             "test_gpu_c_caller", "test_gpu_products", "test_gpu_y_config_sizes", "test_gpu_zz_optional_schedules"]
+             "test_gpu_c_caller", "test_gpu_products", "test_gpu_products_cuts", "test_gpu_y_config_sizes", "test_gpu_zz_optional_schedules"]
 
 
 def pytest_collection_modifyitems(config, items):

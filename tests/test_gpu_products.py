@@ -786,3 +786,19 @@ def test_fp64_codes_next_to_a_half(products):
     for xi, qi, si, ri in zip(x.tolist(), q.tolist(), s.tolist(), r.tolist()):
         for a, b, c in zip(xi, qi, ri):  # what is left over is a number of 64 bits: exact
             assert Fraction(c) == Fraction(a) - b * Fraction(si)
+
+
+@pytest.mark.parametrize("dtype", ALL)
+def test_outputs_beside_their_inputs(products, dtype):
+    """blocks of columns of one matrix, off the 16-byte chunks: the input stays as it was, and autograd notices the output"""
+    t, n, k = 300, 70, 53
+    buf, off = gpu_whole((t, 1 + k + 2 + n + 1), 1, dtype), torch.tensor([0, 100, 100, 290], device="cuda")
+    w, before = gpu_whole((3, n, k), 2, dtype), buf.clone()
+    x, out = buf[:, 1:1 + k], buf[:, k + 3:k + 3 + n]
+    z = torch.ones(t, n, dtype=dtype, device="cuda", requires_grad=True) * out
+    assert products.grouped_matmul(x, w, off, out=out) is out
+    want = before.clone()
+    want[:290, k + 3:k + 3 + n] = gpu_grouped_ref(before[:, 1:1 + k], w, [0, 100, 100, 290])[:290].to(dtype)
+    assert torch.equal(buf, want)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.sum().backward()
