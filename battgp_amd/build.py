@@ -74,7 +74,11 @@ def build_products(force: bool = False, verbose: bool = True) -> str:
 def _build_torch_calls(verbose):
     import sysconfig
 
-    import torch
+    try:
+        import torch
+    except ImportError:  # the C entries do without; battgp_amd.products says what it misses
+        print(f"torch can not be imported: {os.path.basename(LIB_TORCH_CALLS)} is left out", file=sys.stderr)
+        return
 
     root = os.path.dirname(torch.__file__)
     rocm = os.path.dirname(os.path.dirname(_hipcc()))

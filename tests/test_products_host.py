@@ -466,3 +466,18 @@ def test_outputs_between_the_columns_of_an_input(recorder):
         assert products.grouped_matmul(one[None, 4:7], w, o, out=out) is out
     with pytest.raises(ValueError, match="overlaps"):  # both axes of the weights next to each other
         products.grouped_matmul(torch.ones(6, 3), torch.as_strided(big, (2, 4, 3), (48, 12, 1), 4)[:, :, :], o, out=big[:6, 1:5])
+
+
+def test_the_libraries_are_built_without_torch(monkeypatch, tmp_path, capsys):
+    """a program that calls the C entries needs hipcc only; the compiled calls from torch tensors are left out, in words"""
+    import sys
+
+    from battgp_amd import build
+
+    made = []
+    monkeypatch.setattr(build, "_compile", lambda folder, sources, flags, suffix, lib, verbose: made.append(lib))
+    monkeypatch.setattr(build, "LIB_TORCH_CALLS", str(tmp_path / "calls.so"))
+    monkeypatch.setattr(build.subprocess, "check_call", lambda cmd: pytest.fail("nothing to compile against"))
+    monkeypatch.setitem(sys.modules, "torch", None)
+    assert build.build_products(force=True, verbose=False) == build.LIB_PRODUCTS and made == [build.LIB_PRODUCTS]
+    assert "torch" in capsys.readouterr().err
