@@ -17,13 +17,20 @@ namespace {
 
 using at::Tensor;
 
+// What else than the numbers in its memory a tensor stands for: nothing, other tensors (inside vmap, jvp and grad, and
+// wrappers, whose pointer may read as NULL), or a dual number.
+enum Stands { FOR_ITSELF, FOR_OTHERS, WITH_TANGENT };
+Stands stands(const Tensor& t) {
+  if (!t.has_storage() || (t.numel() > 0 && !t.const_data_ptr())) return FOR_OTHERS;
+  return t._fw_grad(0).defined() ? WITH_TANGENT : FOR_ITSELF;
+}
+
 // a dense tensor on the GPU that no gradient is recorded for, in neither mode; NULL if it is anything else
 const Tensor* gpu_tensor(PyObject* o, int dim, int device = -1) {
   if (!THPVariable_Check(o)) return nullptr;
   const Tensor& t = THPVariable_Unpack(o);
   if (t.layout() != at::kStrided || !t.is_cuda() || t.dim() != dim || (device >= 0 && t.get_device() != device)) return nullptr;
-  if (t.is_neg() || (t.requires_grad() && c10::GradMode::is_enabled()) || t._fw_grad(0).defined()) return nullptr;
-  if (!t.has_storage() || (t.numel() > 0 && !t.const_data_ptr())) return nullptr;  // inside vmap and its like, wrappers
+  if (t.is_neg() || (t.requires_grad() && c10::GradMode::is_enabled()) || stands(t) != FOR_ITSELF) return nullptr;
   return &t;
 }
 
@@ -183,7 +190,18 @@ PyObject* int8(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-PyMethodDef methods[] = {{"grouped", (PyCFunction)(void*)grouped, METH_FASTCALL, nullptr},
+// of any tensor: one of Stands
+PyObject* stands_for(PyObject*, PyObject* o) {
+  int r = FOR_OTHERS;
+  try {
+    if (THPVariable_Check(o)) r = stands(THPVariable_Unpack(o));
+  } catch (...) {  // a pointer that is not to be asked for
+  }
+  return PyLong_FromLong(r);
+}
+
+PyMethodDef methods[] = {{"stands_for", (PyCFunction)stands_for, METH_O, nullptr},
+                         {"grouped", (PyCFunction)(void*)grouped, METH_FASTCALL, nullptr},
                          {"grouped_grad", (PyCFunction)(void*)grouped_grad, METH_FASTCALL, nullptr},
                          {"quantize", (PyCFunction)(void*)quantize, METH_FASTCALL, nullptr},
                          {"int8", (PyCFunction)(void*)int8, METH_FASTCALL, nullptr},

@@ -13,7 +13,6 @@ no function records an autograd graph, and inputs that ask for one, or that carr
 from __future__ import annotations
 
 import torch
-from torch.autograd.forward_ad import unpack_dual
 from torch.autograd.graph import increment_version  # a given output is written in place: autograd is to notice
 
 from . import _lib
@@ -46,14 +45,6 @@ def _call(name: str, like: torch.Tensor, *args) -> None:
         raise EngineError(lib.bgp_products_last_error().decode())
 
 
-def _has_memory(t: torch.Tensor) -> bool:
-    """False for what stands for other tensors: inside vmap, jvp and grad, and wrappers, whose pointer may read as NULL."""
-    try:
-        return t.data_ptr() != 0 or t.numel() == 0
-    except RuntimeError:
-        return False
-
-
 def _gpu_tensor(name: str, t, dim: int, device: int | None = None) -> int:
     """the index of the device that ``t`` is on (checks are written for the call that passes: they cost a call its time)"""
     if not isinstance(t, _Tensor):
@@ -70,9 +61,10 @@ def _gpu_tensor(name: str, t, dim: int, device: int | None = None) -> int:
             raise ValueError(f"{name} is on {t.device}, the other operands are on device {device}")
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} requires a gradient: battgp_amd.products records no autograd graph; detach it and call the gradient's function")
-    if not _has_memory(t):
+    other = _calls.stands_for(t)
+    if other == 1:  # inside vmap, jvp and grad, and wrappers, whose pointer may read as NULL
         raise ValueError(f"{name} is not a dense tensor that holds its own values")
-    if unpack_dual(t).tangent is not None:
+    if other == 2:
         raise ValueError(f"{name} has a tangent: battgp_amd.products does not carry forward-mode gradients along")
     return at
 
